@@ -465,6 +465,106 @@ int mono_layer_stack_forward(mono_layer* layer, void* stream);
  * no stale word. No counterpart in the reference. */
 int mono_layer_set_launch_ordinal(mono_layer* layer, uint64_t ordinal);
 
+/* ------------------------------------------------------- prompt-width operators
+ * The layer's work for steps of more rows than a decode launch takes (a prompt), on the
+ * same weights and caches, read and written in place. No counterpart in the reference,
+ * whose covered steps are decode steps; a wider step runs the model's own forward.
+ *
+ * These calls keep no state and own no memory: each takes a workspace of the caller's
+ * (256-byte aligned, at least what the _workspace function says, its content undefined
+ * before and after) that nothing else may use until the call's work has ended on its
+ * stream. Calls with workspaces and outputs of their own may run at once. Every launch
+ * goes to the current device, which must be the one that holds the tensors. A call of no
+ * rows launches nothing and looks at no pointer. Results do not depend on what else runs
+ * and are the same bit for bit from call to call.
+ *
+ * Rounding to FP8 (the rows of a product, and the experts' mids): for each row and each
+ * 128 columns a = max(max |x|, 2^-96), scale a / 448, code E4M3(448 x / a), ties to even.
+ * A block that holds a NaN or an infinity has scale NaN, and so do the row's outputs. */
+
+/* y[m, n] = sum over the 128-column blocks b of sx[m, b] s[n / 128, b] (xq[m, b] . w[n, b]):
+ * bf16 rows times an E4M3 matrix with a scale for each 128 x 128 block, f32 sums. */
+typedef struct {
+  const void* x;       /* bf16 [rows, k], rows x_stride elements apart */
+  int64_t x_stride;    /* a multiple of 8; x itself 16-byte aligned */
+  const void* w;       /* e4m3 [n, k], (16, 16)-shuffled */
+  const float* s;      /* f32 [ceil(n / 128), k / 128] */
+  void* out;           /* bf16 or f32 [rows, n], rows out_stride elements apart */
+  int64_t out_stride;  /* a multiple of 8; out itself 16-byte aligned */
+  int32_t out_f32;     /* 0: bf16 */
+  int64_t rows;        /* 0..1048576 */
+  int32_t n, k;        /* multiples of 16 and of 128, up to 65536 */
+  void* workspace;
+  int64_t workspace_bytes;
+} mono_prompt_product_args;
+
+/* Bytes of workspace of a product (-1: refused, see mono_last_error). */
+int64_t mono_prompt_product_workspace(int64_t rows, int32_t n, int32_t k);
+int mono_prompt_product(const mono_prompt_product_args* args, void* stream);
+
+/* Appends a prompt's keys to the MLA cache and the index plane, in the formats of
+ * mono_front_forward: for token i of request req[i] at position pos[i], at slot
+ * page_table[req, pos / 64] * 64 + pos % 64, the latent's RMSNorm and k_pe's RoPE (E4M3
+ * with one power-of-two scale, or raw), and the index key's LayerNorm, RoPE, Hadamard
+ * and FP4, each value rounded where the front rounds it and formed in f64 between. A
+ * token whose request, position or page is out of range is a pad: it writes nothing.
+ * Two tokens of one call must not share a slot. A latent that is not finite is stored as
+ * E4M3 NaNs, a 32-dim index block that is not finite with scale byte 255 (NaN). */
+typedef struct {
+  const void* kv_a;          /* bf16 or f32 [tokens, 576] latent 512 | k_pe 64, before norm and RoPE */
+  int64_t kv_stride;         /* elements from a row to the next; rows 16-byte aligned */
+  const void* ik;            /* bf16 or f32 [tokens, 128] index key, before norm and RoPE */
+  int64_t ik_stride;         /* even; ik itself 8-byte aligned */
+  int32_t f32;               /* kv_a and ik: 0 bf16, 1 f32 */
+  int64_t tokens;            /* 0..1048576 */
+  const int32_t* req;        /* [tokens] row of page_table */
+  const int32_t* pos;        /* [tokens] */
+  const int32_t* page_table; /* [requests, pt_stride] */
+  int32_t requests, pt_stride, n_pages, max_pos;
+  const void* g_kv;          /* bf16 [512] */
+  const float* g_ik;         /* f32 [128] */
+  const float* b_ik;         /* f32 [128] */
+  const float* rope_cos;     /* f32 [max_pos, 32] */
+  const float* rope_sin;     /* f32 [max_pos, 32] */
+  void* kv;                  /* u8 [n_pages * 64, 576], written in place */
+  float* kv_scale;           /* f32 [n_pages * 64], or NULL: raw E4M3 rows */
+  void* ikv;                 /* u8 [n_pages, 4, 64, 16] */
+  void* iks;                 /* u8 [n_pages, 4, 64] */
+} mono_prompt_append_args;
+
+int mono_prompt_append(const mono_prompt_append_args* args, void* stream);
+
+/* out[t] = residual[t] + shared(x[t]) + sum_j weights[t, j] expert_(ids[t, j])(x[t]), with
+ * expert(x) = w2 FP8(silu(gate) * up), (gate, up) = w13 FP8(x): the FP8 MoE of
+ * mono_moe_fp8_forward behind a router and a norm of the caller's. A pick outside
+ * [0, experts) is routed nowhere; an expert picked twice by a token counts twice. */
+typedef struct {
+  const void* x;            /* bf16 [tokens, hidden], the normed rows */
+  int64_t x_stride;         /* a multiple of 8 */
+  const int32_t* ids;       /* [tokens, picks] */
+  const float* weights;     /* f32 [tokens, picks] */
+  const void* w13;          /* e4m3 [E, 2 inter, hidden] gate rows then up rows, (16, 16)-shuffled */
+  const float* s13;         /* f32 [E, 2 inter / 128, hidden / 128] */
+  const void* w2;           /* e4m3 [E, hidden, inter], (16, 16)-shuffled */
+  const float* s2;          /* f32 [E, hidden / 128, inter / 128] */
+  const void* residual;     /* optional bf16 [tokens, hidden] added to the sum */
+  int64_t residual_stride;  /* a multiple of 8 */
+  void* out;                /* bf16 [tokens, hidden] */
+  int64_t out_stride;       /* a multiple of 8 */
+  int64_t tokens;           /* tokens x (picks + 1) up to 1048576 */
+  int32_t picks;            /* picks a token, 1..64 */
+  int32_t experts;          /* routed experts, 1..1024 */
+  int32_t shared;           /* 1: expert id `experts` is the shared one (weight 1, every token) */
+  int32_t hidden, inter;    /* multiples of 128 */
+  void* workspace;
+  int64_t workspace_bytes;
+} mono_prompt_experts_args;
+
+/* Bytes of workspace of an experts call of these sizes (pointers are not looked at; -1:
+ * refused, see mono_last_error). */
+int64_t mono_prompt_experts_workspace(const mono_prompt_experts_args* args);
+int mono_prompt_experts(const mono_prompt_experts_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,7 +17,7 @@ MONO_OK, MONO_EINVAL, MONO_EHIP, MONO_ESTATE, MONO_ENOMEM = 0, 1, 2, 3, 4
 ROUTER_SIGMOID_BIAS, ROUTER_SOFTMAX = 0, 1
 WEIGHT_FP8_BLOCK128, WEIGHT_MXFP4 = 0, 1
 
-_VP, _I32, _F32 = C.c_void_p, C.c_int32, C.c_float
+_VP, _I32, _I64, _F32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
 
 
 class MoeConfig(C.Structure):
@@ -93,6 +93,26 @@ class LayerArgs(C.Structure):
                 ("moe", C.POINTER(MoeFp8Args)), ("ticks", _VP)]
 
 
+class PromptProductArgs(C.Structure):
+    _fields_ = [("x", _VP), ("x_stride", _I64), ("w", _VP), ("s", _VP), ("out", _VP), ("out_stride", _I64),
+                ("out_f32", _I32), ("rows", _I64), ("n", _I32), ("k", _I32), ("workspace", _VP),
+                ("workspace_bytes", _I64)]
+
+
+class PromptAppendArgs(C.Structure):
+    _fields_ = [("kv_a", _VP), ("kv_stride", _I64), ("ik", _VP), ("ik_stride", _I64), ("f32", _I32), ("tokens", _I64),
+                ("req", _VP), ("pos", _VP), ("page_table", _VP), ("requests", _I32), ("pt_stride", _I32),
+                ("n_pages", _I32), ("max_pos", _I32), ("g_kv", _VP), ("g_ik", _VP), ("b_ik", _VP), ("rope_cos", _VP),
+                ("rope_sin", _VP), ("kv", _VP), ("kv_scale", _VP), ("ikv", _VP), ("iks", _VP)]
+
+
+class PromptExpertsArgs(C.Structure):
+    _fields_ = [("x", _VP), ("x_stride", _I64), ("ids", _VP), ("weights", _VP), ("w13", _VP), ("s13", _VP),
+                ("w2", _VP), ("s2", _VP), ("residual", _VP), ("residual_stride", _I64), ("out", _VP),
+                ("out_stride", _I64), ("tokens", _I64), ("picks", _I32), ("experts", _I32), ("shared", _I32),
+                ("hidden", _I32), ("inter", _I32), ("workspace", _VP), ("workspace_bytes", _I64)]
+
+
 # the phase boundaries a one-launch layer stamps per workgroup (mono_layer_args.ticks)
 LAYER_TICKS = ("begin", "front", "attn", "back", "plan", "end", "a_seen", "norm", "router", "route", "quant")
 LAYER_TICK_WORDS = 16
@@ -141,6 +161,11 @@ SIGNATURES = {
     "mono_layer_clear_errors": (C.c_int, [_VP]),
     "mono_layer_set_fault": (C.c_int, [_VP, C.c_int32, C.c_int64]),
     "mono_layer_set_launch_ordinal": (C.c_int, [_VP, C.c_uint64]),
+    "mono_prompt_product_workspace": (_I64, [_I64, _I32, _I32]),
+    "mono_prompt_product": (C.c_int, [C.POINTER(PromptProductArgs), _VP]),
+    "mono_prompt_append": (C.c_int, [C.POINTER(PromptAppendArgs), _VP]),
+    "mono_prompt_experts_workspace": (_I64, [C.POINTER(PromptExpertsArgs)]),
+    "mono_prompt_experts": (C.c_int, [C.POINTER(PromptExpertsArgs), _VP]),
 }
 GUARD_WORDS = 8
 # guard words: tag epochs, error (1 + site), failing tag, failing workgroup, u64 launches begun

@@ -1,0 +1,116 @@
+// Device pieces the prompt-width operators share: rounding a block of 128 values to
+// E4M3 with its scale.
+#pragma once
+
+#include "common.h"
+#include "prompt_ops.h"
+
+namespace mono {
+namespace prompt {
+
+constexpr float LEAST = 0x1p-96f;  // a block's largest magnitude counts as at least this
+
+// A block's scale and what its values are multiplied and divided by on the way to codes.
+struct BlockScale {
+  float scale;  // a / 448
+  float mant;   // a = mant 2^e, mant in [1/2, 1)
+  float rcp;    // 1 / mant
+  int shift;    // 9 - e
+  bool finite;
+};
+
+// From the block's largest magnitude as f32 bits (a NaN's bits are above infinity's).
+MONO_DEV BlockScale block_scale(uint32_t amax_bits) {
+  BlockScale b;
+  b.finite = amax_bits < 0x7f800000u;
+  const float a = fmaxf(b.finite ? __uint_as_float(amax_bits) : 1.0f, LEAST);
+  int e;
+  b.mant = frexpf(a, &e);
+  b.rcp = 1.0f / b.mant;
+  b.shift = 9 - e;
+  b.scale = b.finite ? a / FP8_MAX : __uint_as_float(0x7fc00000u);  // a block that is not finite: NaN
+  return b;
+}
+
+// 448 v / a, correctly rounded but for a last bit where that is no tie: the quotient of
+// two bf16 values is often exactly midway between two codes, and the product with a
+// rounded reciprocal alone would send such a tie either way. One residual step makes a
+// quotient that f32 can hold exact. v and a are scaled by a's exponent first, so nothing
+// overflows and only what rounds to zero is lost.
+MONO_DEV float to_code_range(float v, const BlockScale& b) {
+  const float n = ldexpf(v, b.shift) * 0.875f;
+  const float q = n * b.rcp;
+  const float r = fmaf(-q, b.mant, n);
+  return b.finite ? fminf(fmaxf(fmaf(r, b.rcp, q), -FP8_MAX), FP8_MAX) : 0.0f;
+}
+
+MONO_DEV uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// unsigned max over each 16 consecutive lanes
+MONO_DEV uint32_t row_umax16(uint32_t v) {
+  v = max(v, dpp_u<DPP_XOR1>(v));
+  v = max(v, dpp_u<DPP_XOR2>(v));
+  v = max(v, dpp_u<DPP_HALF_MIRROR>(v));
+  return max(v, dpp_u<DPP_MIRROR>(v));
+}
+
+// Eight values of a block that 16 lanes hold together -> their codes; every lane of the
+// 16 gets the block's scale.
+MONO_DEV u32x2 quant8(const float (&v)[8], float& scale) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+  const BlockScale b = block_scale(row_umax16(m));
+  float c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = to_code_range(v[i], b);
+  scale = b.scale;
+  return u32x2{fp8x4_pack(c[0], c[1], c[2], c[3]), fp8x4_pack(c[4], c[5], c[6], c[7])};
+}
+
+// Four of a lane's bytes, widened exactly to bf16.
+MONO_DEV void widen4(uint32_t w, bf16x8& to, int at) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
+  to[at] = a[0], to[at + 1] = a[1], to[at + 2] = b[0], to[at + 3] = b[1];
+}
+
+// A block's partial products, A[16 x 128] B[128 x 16]. The FP8 MFMA adds its 128 products
+// with fewer than f32's bits (1.4e-5 of the result, measured on N(0, 1) values): too few
+// for f32 outputs, whose codes are widened exactly to bf16 (6e-9) at half the rate.
+template <bool F32>
+MONO_DEV f32x4 mfma_block(const i32x8& a, const i32x8& b) {
+  f32x4 p = {0.f, 0.f, 0.f, 0.f};
+  if (!F32) return mfma_fp8(a, b, p);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    bf16x8 x, y;
+    widen4((uint32_t)a[2 * q], x, 0);
+    widen4((uint32_t)a[2 * q + 1], x, 4);
+    widen4((uint32_t)b[2 * q], y, 0);
+    widen4((uint32_t)b[2 * q + 1], y, 4);
+    p = mfma_bf16(x, y, p);
+  }
+  return p;
+}
+
+MONO_DEV void load8(const uint16_t* p, float (&v)[8]) {
+  const u32x4 u = ld_u32x4(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = u[i];
+    v[2 * i] = bf16_lo(w);
+    v[2 * i + 1] = bf16_hi(w);
+  }
+}
+MONO_DEV void load8(const float* p, float (&v)[8]) {
+  const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = a[i];
+    v[4 + i] = b[i];
+  }
+}
+
+}  // namespace prompt
+}  // namespace mono

@@ -1,0 +1,77 @@
+// Host-side declarations of the prompt-width operators (internal to the library): FP8
+// block products, paged cache appends and routed experts over any number of rows.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mono.h"
+
+namespace mono {
+namespace prompt {
+
+constexpr int BLK = 128;             // a scale's block of rows' and weights' columns
+constexpr int MAX_EXPERTS = 1024;    // routed experts (a sort block's LDS histogram)
+constexpr int MAX_DIM = 1 << 16;     // columns and outputs of a product
+constexpr int64_t MAX_ROWS = 1 << 20;  // rows a call; picks of all rows of an experts call
+
+constexpr int LATENT = 512, PE = 64, INDEX = 128, PAGE = 64;
+
+// Rows rounded to E4M3: codes [rows, k] and scales [k / 128, ld] (a block's scales of
+// consecutive rows lie together: a product's lanes hold one row each).
+struct Rows {
+  uint8_t* q;
+  float* s;
+  int ld;
+};
+
+// One tile of expert work: `count` sorted places from `first` on, of expert `expert`.
+struct Tile {
+  int expert, first, count, pad;
+};
+
+// The tokens sorted by expert. Place p < picks holds a routed pick, place picks + t
+// token t's row of the shared expert.
+struct Sorted {
+  int* token;  // [picks + tokens] token of each place
+  int* place;  // [picks] place of each pick (token * k + j), -1: routed nowhere
+  Tile* tiles; // [max_tiles]
+  int* n_tiles;
+};
+
+// The tile list's bound: the shared expert's tiles, then every routed expert's whole
+// tiles and at most one partial tile for each expert that is picked.
+inline int64_t max_tiles(int64_t tokens, int64_t picks, int experts, int bm, bool shared) {
+  const int64_t part = picks < experts ? picks : experts;
+  return (shared ? (tokens + bm - 1) / bm : 0) + picks / bm + part;
+}
+
+hipError_t quant_rows(const void* x, bool f32, int64_t stride, int64_t rows, int k, const Rows& out, hipStream_t st);
+hipError_t sort_quant(const void* x, int64_t stride, int64_t tokens, int k, const Rows& out, const int* ids, int picks_each,
+                      int experts, bool shared, int bm, const Sorted& sorted, hipStream_t st);
+hipError_t product(const Rows& x, int64_t rows, const void* w, const float* s, int n, int k, void* out, bool f32,
+                   int64_t out_stride, hipStream_t st);
+
+struct Experts {
+  Rows x, mid_q;
+  Sorted sorted;
+  float* mid;   // f32 [places, inter]
+  float* part;  // f32 [places, hidden]
+  const uint8_t *w13, *w2;
+  const float *s13, *s2, *weights;
+  const void* residual;
+  int64_t residual_stride;
+  void* out;
+  int64_t out_stride;
+  int64_t tokens, picks;
+  int picks_each, experts, hidden, inter, bm, tiles;
+  bool shared;
+};
+hipError_t experts_up(const Experts& a, hipStream_t st);
+hipError_t experts_down(const Experts& a, hipStream_t st);
+hipError_t experts_back(const Experts& a, hipStream_t st);
+
+hipError_t append(const mono_prompt_append_args& a, hipStream_t st);
+
+}  // namespace prompt
+}  // namespace mono

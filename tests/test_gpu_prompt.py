@@ -1,0 +1,393 @@
+"""The prompt-width operators on the GPU against their float64 restatements.
+
+Tolerances, from the formats. A bf16 output is off by half a step, 2^-8 of it. The FP8
+MFMA adds a block's 128 products with fewer bits than f32's (1.4e-5 of the result on
+N(0, 1) values): 2^-14 of the sum of the terms' magnitudes holds some thirty times that.
+An f32 product's K sums are each off by at most 2^-24 of what has been summed. Rows in
+bf16 have no code that hangs on a rounding (a quotient that is a tie is one exactly), a
+mid may: an error of 2^-14 moves at most 2^-9 of the mids (2^-14 of the distance 2^-4
+between borders, both sides) over one, each by 2^-3 of itself, so the sums by
+2^-3 sqrt(2^-9) < 0.0056 of their size. One output may lie further off: a single mid that
+moves by a code moves it by that step times a weight, whatever the sums' size, so two such
+steps are allowed in each of a token's experts (prompt_ref.experts' ``step``).
+Appended rows are formed in f64 on both sides: they are equal.
+"""
+
+import pytest
+import torch
+
+import prompt_ref as ref
+from oracle import attention as oatt
+from sgl_amd_mono_amd import prompt, workloads
+from sgl_amd_mono_amd.attn import AttnCaches, AttnRuntime, AttnStep
+from sgl_amd_mono_amd.layer import KV_LORA, N_QKV, PE_DIM, Q_LORA
+from sgl_amd_mono_amd.layouts import shuffle_16x16
+from sgl_amd_mono_amd.moe import FP8_MOE, MoeGeometry, MoeRuntime
+
+pytestmark = pytest.mark.gpu
+
+
+def _matrix(n, k, dev, seed):
+    return workloads._fp8_matrix(n, k, torch.Generator(device=dev).manual_seed(seed), dev)
+
+
+def _same(got, want, mag, f32, k):
+    """Within the tolerances of the module's head."""
+    # a sum past the type's largest value is its infinity, as the rounding of that sum is
+    far = want.abs() > torch.finfo(got.dtype).max
+    got, bad = got.cpu().double(), want.isnan()
+    assert bool((got.isnan() == bad).all()) and torch.equal(got[far], torch.inf * want[far].sign())
+    bad = bad | far
+    tol = k * 2.0**-24 * mag + 2.0**-24 * want.abs() if f32 else 2.0**-8 * want.abs() + 2.0**-14 * mag
+    over = ((got - want).abs() / tol.clamp_min(1e-30))[~bad]
+    assert float(over.max() if over.numel() else 0.0) <= 1.0, float(over.max())
+
+
+# ------------------------------------------------------------------- product
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("m,n,k", [(1, 16, 128), (1, 2112, 7168), (3, 144, 384), (16, 128, 7168), (17, 272, 1024),
+                                   (63, 64, 256), (65, 2112, 512), (129, 400, 1152), (300, 1536, 640)])
+def test_product(gpu_device, m, n, k, f32):
+    w, s = _matrix(n, k, gpu_device, 1)
+    x = workloads.rows_bf16(m, k, gpu_device, seed=2)
+    x[0, : k // 2] *= 100.0  # blocks of other sizes next to each other
+    got = prompt.product(x, w, s, dtype=torch.float32 if f32 else torch.bfloat16)
+    want, mag = ref.product(x.cpu(), w.cpu(), s.cpu())
+    _same(got, want, mag, f32, k)
+
+
+@pytest.mark.parametrize("m", [1, 15, 64, 200, 257, 530, 1025])
+@pytest.mark.parametrize("n", [16, 208, 256, 528])
+def test_product_of_small_integers_is_exact(gpu_device, m, n):
+    """Integers within a factor of 7 of each other: every code, product and sum is exact,
+    so a wrong place anywhere shows."""
+    k = 512
+    g = torch.Generator(device=gpu_device).manual_seed(m * n)
+    x = torch.randint(-7, 8, (m, k), generator=g, device=gpu_device).float()
+    x[:, ::128] = 7.0  # each block's scale is 7 / 448 = 1 / 64
+    w = torch.randint(-4, 5, (n, k), generator=g, device=gpu_device).float()
+    s = 2.0 ** torch.randint(-2, 3, (-(-n // 128), k // 128), generator=g, device=gpu_device).float()
+    got = prompt.product(x.to(torch.bfloat16), shuffle_16x16(w.to(torch.float8_e4m3fn)), s, dtype=torch.float32)
+    full = (w * s.repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)).double()
+    assert torch.equal(got.cpu().double(), x.cpu().double() @ full.cpu().T)
+
+
+def test_product_strided_rows_and_out(gpu_device):
+    m, n, k = 77, 192, 384
+    w, s = _matrix(n, k, gpu_device, 3)
+    wide = workloads.rows_bf16(m, k + 64, gpu_device, seed=4)
+    buf = torch.full((m + 2, n + 48), 3.0, dtype=torch.bfloat16, device=gpu_device)
+    got = prompt.product(wide[:, 64:], w, s, out=buf[1:-1, 16:-32])
+    assert torch.equal(got, prompt.product(wide[:, 64:].contiguous(), w, s))
+    assert bool((buf[0] == 3).all()) and bool((buf[-1] == 3).all())
+    assert bool((buf[:, :16] == 3).all()) and bool((buf[:, -32:] == 3).all())
+
+
+@pytest.mark.parametrize("m", [5, 70, 300])
+def test_product_non_finite_and_extreme_rows(gpu_device, m):
+    n, k = 64, 512
+    w, s = _matrix(n, k, gpu_device, 5)
+    x = workloads.rows_bf16(m, k, gpu_device, seed=6)
+    x[1, 130] = float("nan")
+    x[2, 511] = float("-inf")
+    x[3] = 0.0
+    x[4, :128] = torch.finfo(torch.bfloat16).max
+    x[4, 128:256] = 1e-39  # below the least block size
+    got = prompt.product(x, w, s, dtype=torch.float32)
+    want, mag = ref.product(x.cpu(), w.cpu(), s.cpu())
+    assert bool(got[1:3].isnan().all()) and bool((got[3] == 0).all())
+    _same(got, want, mag, True, k)
+
+
+def test_product_of_no_rows(gpu_device):
+    w, s = _matrix(64, 256, gpu_device, 7)
+    assert prompt.product(torch.empty(0, 256, dtype=torch.bfloat16, device=gpu_device), w, s).shape == (0, 64)
+
+
+# -------------------------------------------------------------------- append
+def _append_case(dev, spans, f32, raw, pads=0, wide=0, seed=11):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    need = [-(-(a + n) // 64) for a, n in spans]
+    pages, width = sum(need) + 3, max(need) + 1
+    table = torch.zeros(len(spans), width, dtype=torch.int32)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed))
+    at = 0
+    for r, u in enumerate(need):
+        table[r, :u] = order[at:at + u]
+        at += u
+    req = torch.cat([torch.full((n,), r) for r, (_, n) in enumerate(spans)] + [torch.full((pads,), -1)]).int()
+    pos = torch.cat([torch.arange(a, a + n) for a, n in spans] + [torch.zeros(pads)]).int()
+    t, dt = len(req), torch.float32 if f32 else torch.bfloat16
+    kv_a = (2.0 * torch.randn(t, 576 + wide, generator=g, device=dev)).to(dt)[:, wide:]
+    ik = (torch.randn(t, 128 + wide, generator=g, device=dev) + 0.2).to(dt)[:, wide:]
+    u8 = dict(generator=g, device=dev, dtype=torch.uint8)
+    caches = AttnCaches(ikv=torch.randint(0, 256, (pages, 4, 64, 16), **u8), iks=torch.randint(120, 130, (pages, 4, 64), **u8),
+                        kv=torch.randint(0, 126, (pages * 64, 576), **u8),
+                        kv_scale=None if raw else torch.rand(pages * 64, generator=g, device=dev))
+    cos, sin = workloads.rope_tables(width * 64 - 5, dev)
+    w = dict(g_kv=(1 + 0.1 * torch.randn(512, generator=g, device=dev)).to(torch.bfloat16),
+             g_ik=1 + 0.1 * torch.randn(128, generator=g, device=dev), b_ik=0.1 * torch.randn(128, generator=g, device=dev))
+    return dict(kv_a=kv_a, ik=ik, req=req.to(dev), pos=pos.to(dev), page_table=table.to(dev), caches=caches, **w,
+                rope_cos=cos, rope_sin=sin)
+
+
+def _append_both(c):
+    """Run the operator on c's caches; returns (what it left, what it should leave)."""
+    want = {k: None if v is None else v.cpu().clone() for k, v in vars(c["caches"]).items()}
+    cpu = {k: v.cpu() for k, v in c.items() if k != "caches"}
+    ref.append(cpu["kv_a"], cpu["ik"], cpu["req"], cpu["pos"], cpu["page_table"], want, cpu["g_kv"], cpu["g_ik"],
+               cpu["b_ik"], cpu["rope_cos"], cpu["rope_sin"])
+    prompt.append(**c)
+    return {k: None if v is None else v.cpu() for k, v in vars(c["caches"]).items()}, want
+
+
+def _equal(got, want):
+    for k, v in want.items():
+        assert (v is None and got[k] is None) or torch.equal(got[k], v), k
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("raw", [False, True], ids=["scaled", "raw"])
+@pytest.mark.parametrize("spans,pads,wide", [([(0, 1)], 0, 0), ([(700, 1), (63, 1), (64, 1)], 2, 0),
+                                             ([(0, 64), (60, 9), (1, 130)], 5, 16), ([(0, 333)], 0, 1536)])
+def test_append(gpu_device, spans, pads, wide, f32, raw):
+    _equal(*_append_both(_append_case(gpu_device, spans, f32, raw, pads, wide)))
+
+
+def test_append_out_of_range_tokens_write_nothing(gpu_device):
+    c = _append_case(gpu_device, [(0, 70), (10, 60)], False, False, pads=4)
+    pages = c["caches"].ikv.shape[0]
+    c["req"][3], c["req"][4] = 2, -7  # no such request
+    c["pos"][5], c["pos"][6] = -1, 1 << 30  # no such position
+    c["pos"][7] = c["rope_cos"].shape[0]  # no angle
+    c["page_table"][1, 0] = pages  # bad pages
+    c["page_table"][0, 1] = -1
+    _equal(*_append_both(c))
+
+
+def test_append_extreme_rows(gpu_device):
+    c = _append_case(gpu_device, [(0, 12)], True, False)
+    c["kv_a"][0] = 0.0
+    c["ik"][0] = 0.0
+    c["kv_a"][1] = 1e-30
+    c["ik"][1] = 5.0  # no variance: the bias alone
+    c["kv_a"][2, :512] *= 1e18
+    c["kv_a"][3, 512:] = 1e6
+    c["kv_a"][4, 512:] = 448.0 * 2.0**-3  # an amax that is exactly a scale's border, before rotation
+    c["pos"][4] = 0
+    c["pos"][0] = 4
+    _equal(*_append_both(c))
+
+
+@pytest.mark.parametrize("raw", [False, True], ids=["scaled", "raw"])
+def test_append_non_finite(gpu_device, raw):
+    """A NaN stays a NaN that a reader sees, and stays in its own token."""
+    c = _append_case(gpu_device, [(0, 8)], False, raw)
+    clean = _append_case(gpu_device, [(0, 8)], False, raw)
+    c["kv_a"][2, 5] = float("nan")
+    c["ik"][3, 9] = float("inf")
+    prompt.append(**c)
+    prompt.append(**clean)
+    got, want = c["caches"], clean["caches"]
+    page = int(c["page_table"][0, 0])
+    assert bool(((got.kv[page * 64 + 2, :512] & 0x7F) == 0x7F).all())
+    assert bool((got.iks[page, :, 3 * 4] == 255).all())
+    others = [t for t in range(64) if t != 2]
+    assert torch.equal(got.kv.view(-1, 64, 576)[page, others], want.kv.view(-1, 64, 576)[page, others])
+    others = [t for t in range(64) if t != 3]
+    assert torch.equal(got.ikv[page, :, others], want.ikv[page, :, others])
+
+
+def test_append_of_nothing(gpu_device):
+    c = _append_case(gpu_device, [(0, 3)], False, False)
+    before = c["caches"].kv.clone()
+    for k in ("kv_a", "ik", "req", "pos"):
+        c[k] = c[k][:0]
+    prompt.append(**c)
+    assert torch.equal(c["caches"].kv, before)
+
+
+# ------------------------------------------------------------------- experts
+def _experts_case(dev, t, h, i, e, k, seed=21, shared=True):
+    geo = MoeGeometry(h, e, k, i, 1.0, 1e-6, "sigmoid_bias", "fp8_block128")
+    m = workloads.fp8_moe_weights(geo, dev, seed=seed)
+    m.s13 *= 448.0 / (1.25 * h**0.5)
+    m.s2 *= 448.0 / (1.25 * i**0.5)
+    g = torch.Generator(device=dev).manual_seed(seed + 1)
+    ids = torch.rand(t, e, generator=g, device=dev).argsort(1)[:, :k].int().contiguous()
+    wts = torch.rand(t, k, generator=g, device=dev) + 0.1
+    x = workloads.rows_bf16(t, h, dev, seed=seed + 2)
+    n = e + 1 if shared else e
+    return dict(x=x, ids=ids, weights=wts, w13=m.w13[:n].contiguous(), s13=m.s13[:n].contiguous(), w2=m.w2[:n].contiguous(),
+                s2=m.s2[:n].contiguous(), residual=workloads.rows_bf16(t, h, dev, seed=seed + 3), shared=shared)
+
+
+def _check_experts(c, got):
+    cpu = {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    want, y, step = ref.experts(cpu["x"], cpu["ids"], cpu["weights"], cpu["w13"], cpu["s13"], cpu["w2"], cpu["s2"],
+                                cpu["residual"], cpu["shared"])
+    d = got.cpu().double() - want
+    assert not bool(d.isnan().any())
+    over = d.abs() / (2.0**-8 * want.abs() + 2 * step[:, None] + 1e-30)
+    assert float(over.max()) <= 1.0, float(over.max())
+    assert float(d.norm()) <= 0.0056 * float(y.norm()) + 2.0**-8 * float(want.norm())
+
+
+@pytest.mark.parametrize("t,h,i,e,k", [(1, 256, 128, 4, 1), (1, 512, 256, 16, 8), (9, 384, 128, 5, 5), (40, 256, 384, 8, 2),
+                                       (130, 512, 128, 3, 2), (300, 256, 256, 33, 4), (700, 128, 128, 2, 1)])
+def test_experts(gpu_device, t, h, i, e, k):
+    c = _experts_case(gpu_device, t, h, i, e, k)
+    _check_experts(c, prompt.experts(**c))
+
+
+def test_experts_without_shared_or_residual(gpu_device):
+    c = _experts_case(gpu_device, 50, 256, 128, 8, 2, shared=False)
+    got = prompt.experts(**dict(c, residual=None))
+    c["residual"] = torch.zeros_like(c["x"])
+    _check_experts(c, got)
+
+
+@pytest.mark.parametrize("t", [6, 90, 400])
+def test_experts_odd_picks(gpu_device, t):
+    """Picks of no expert, tokens without any, one expert twice, an expert that all pick."""
+    c = _experts_case(gpu_device, t, 256, 128, 8, 4)
+    c["ids"][:, 0] = 5
+    c["ids"][1] = -1
+    c["ids"][2, 1:] = torch.tensor([8, 9, 1 << 30], device=gpu_device).int()  # 8 is the shared one: not a pick
+    c["ids"][3] = torch.tensor([2, 2, 2, 6], device=gpu_device).int()
+    c["weights"][1] = float("nan")  # the weight of no pick
+    _check_experts(dict(c, weights=c["weights"].nan_to_num(0.0)), prompt.experts(**c))
+    c["ids"][:] = -1  # no pick at all: the shared expert alone
+    c["weights"][1] = 1.0
+    _check_experts(c, prompt.experts(**c))
+    c = dict(_experts_case(gpu_device, t, 256, 128, 8, 4, shared=False), residual=None)
+    c["ids"][:] = 8
+    assert bool((prompt.experts(**c) == 0).all())
+
+
+def test_experts_strided_in_place(gpu_device):
+    c = _experts_case(gpu_device, 33, 256, 128, 8, 2)
+    want = prompt.experts(**c)
+    buf = torch.zeros(33, 256 + 40, dtype=torch.bfloat16, device=gpu_device)
+    buf[:, 8:-32] = c["residual"]
+    xw = torch.zeros(33, 256 + 8, dtype=torch.bfloat16, device=gpu_device)
+    xw[:, 8:] = c["x"]
+    got = prompt.experts(**dict(c, x=xw[:, 8:], residual=buf[:, 8:-32], out=buf[:, 8:-32]))
+    assert torch.equal(got, want) and bool((buf[:, :8] == 0).all()) and bool((buf[:, -32:] == 0).all())
+
+
+def test_experts_of_no_tokens(gpu_device):
+    c = _experts_case(gpu_device, 4, 256, 128, 8, 2)
+    for k in ("x", "ids", "weights", "residual"):
+        c[k] = c[k][:0]
+    assert prompt.experts(**c).shape == (0, 256)
+
+
+# ---------------------------------------------------- streams, graphs, repeats
+def test_repeats_and_streams(gpu_device):
+    """The same bits from call to call, and from two streams at once."""
+    c = _experts_case(gpu_device, 200, 512, 256, 16, 4)
+    w, s = _matrix(528, 512, gpu_device, 9)
+    want, wantp = prompt.experts(**c), prompt.product(c["x"], w, s)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(gpu_device) for _ in range(2)]
+    got = []
+    for _ in range(4):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append((prompt.experts(**c), prompt.product(c["x"], w, s)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want) and torch.equal(b, wantp) for a, b in got)
+
+
+def test_graph_replays(gpu_device):
+    """Captured calls replayed on new inputs with eager work between, two graphs in turn."""
+    c = _experts_case(gpu_device, 70, 256, 128, 8, 2)
+    a = _append_case(gpu_device, [(0, 70)], False, False)
+    w, s = _matrix(144, 256, gpu_device, 13)
+    graphs = []
+    for _ in range(2):
+        prompt.experts(**c), prompt.product(c["x"], w, s), prompt.append(**a)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs = prompt.experts(**c), prompt.product(c["x"], w, s)
+            prompt.append(**a)
+        graphs.append((gr, outs))
+    for step in range(4):
+        c["x"].copy_(workloads.rows_bf16(70, 256, gpu_device, seed=90 + step))
+        c["ids"].copy_(torch.randint(-1, 8, (70, 2), device=gpu_device).int())
+        a["kv_a"].copy_(torch.randn(70, 576, device=gpu_device))
+        for gr, outs in graphs:
+            a["caches"].kv.zero_()
+            gr.replay()
+            kv = a["caches"].kv.clone()
+            want = prompt.experts(**c), prompt.product(c["x"], w, s)
+            a["caches"].kv.zero_()
+            prompt.append(**a)
+            torch.cuda.synchronize()
+            assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(kv, a["caches"].kv)
+
+
+# ------------------------------------------------------------- used together
+def test_prompt_then_decode_attention(gpu_device):
+    """Two prompts' normed rows through the projections' own weights into the caches, which
+    the decode attention then reads: its selection and output against the oracle on the
+    same caches."""
+    dev, lens, ctx = gpu_device, [2300, 77], 4096
+    w = workloads.proj_weights(dev, seed=31)
+    step, caches = workloads.attn_case(lens, dev, seed=32, max_ctx=ctx)
+    caches.kv.zero_(), caches.ikv.zero_(), caches.iks.zero_(), caches.kv_scale.zero_()
+    cos, sin = workloads.rope_tables(ctx, dev)
+    req = torch.cat([torch.full((n,), r, device=dev) for r, n in enumerate(lens)]).int()
+    pos = torch.cat([torch.arange(n, device=dev) for n in lens]).int()
+    x = workloads.rows_bf16(sum(lens), 7168, dev, seed=33)
+    qkv = prompt.product(x, w.w_qkv, w.s_qkv)
+    ik = prompt.product(x, w.w_ik, w.s_ik)
+    assert qkv.shape == (sum(lens), N_QKV)
+    prompt.append(qkv[:, Q_LORA:], ik, req, pos, step.page_table, caches, w.g_kv, w.g_ik, w.b_ik, cos, sin)
+    rt = AttnRuntime(2, ctx, device=dev)
+    out, dbg = rt.forward(step, caches, debug=True)
+    torch.cuda.synchronize()
+    rt.check_errors()
+    rt.close()
+    seq, pt, sel = step.seq_lens.cpu(), step.page_table.cpu(), dbg["topk"].cpu()
+    assert torch.equal(sel, oatt.select_topk(dbg["scores"].cpu(), seq, pt))
+    want = oatt.sparse_mla(step.q.cpu(), caches.kv.cpu(), caches.kv_scale.cpu(), sel)
+    err = (out.cpu().float() - want.float()).abs()
+    assert bool((err <= 2e-2 + 1e-2 * want.float().abs()).all()), float(err.max())  # the attention's own bounds
+    # the rows are the projections': dequantised latents against the norm of the f64 products
+    for r, n in enumerate(lens):
+        t = torch.tensor([0, n // 2, n - 1])
+        slots = pt[r, t // 64].long() * 64 + t % 64
+        row = caches.kv.cpu()[slots].view(torch.float8_e4m3fn).double() * caches.kv_scale.cpu()[slots].double()[:, None]
+        at = t + sum(lens[:r])
+        y, _ = ref.product(x[at.to(dev)].cpu(), w.w_qkv.cpu(), w.s_qkv.cpu())
+        lat = y[:, Q_LORA:Q_LORA + KV_LORA]
+        lat = lat / (lat.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.g_kv.cpu().double()
+        # product and latent in bf16 (2^-8 each), E4M3 (2^-4), a subnormal's half step 2^-10 of a scale
+        # (<= 2^-7 of the largest)
+        tol = (2.0**-8 + 2.0**-8 + 2.0**-4 + 2.0**-9) * lat.abs() + 2.0**-16 * row.abs().amax(-1, keepdim=True)
+        assert bool(((row[:, :KV_LORA] - lat).abs() <= tol + 2.0**-7 * lat.square().mean().sqrt()).all())
+        assert row.shape[1] == KV_LORA + PE_DIM
+
+
+def test_experts_against_the_decode_launch(gpu_device):
+    """A decode step's MoE and the prompt's experts on its own routing: the same products
+    (the launch rounds its f32 normed rows to FP8, the prompt's rows come in bf16)."""
+    dev = gpu_device
+    w = workloads.fp8_moe_weights(FP8_MOE, dev, seed=41)
+    a = workloads.rows_bf16(8, FP8_MOE.hidden, dev, seed=42)
+    rt = MoeRuntime(FP8_MOE, 8, device=dev)
+    want, dbg = rt.forward_fp8(a, w, debug=True)
+    torch.cuda.synchronize()
+    rt.check_errors()
+    rt.close()
+    x = a.float() * torch.rsqrt(a.float().square().mean(-1, keepdim=True) + FP8_MOE.eps) * w.g_post.float()
+    got = prompt.experts(x.to(torch.bfloat16), dbg["topk_ids"], dbg["topk_w"], w.w13, w.s13, w.w2, w.s2, residual=a)
+    # a bf16 row is 2^-8 off: at most 2^-8 / 2^-4 of the codes a step (2^-3) over, 2^-3 sqrt(2^-4) = 0.031 of
+    # each product at the very worst (all of them at a border); the sums' sizes are the launch's own
+    y = dbg["y"].double()
+    d = (got.double() - want.double())
+    assert float(d.norm()) <= 2 * 0.031 * float(y.norm()) + 2.0**-7 * float(want.double().norm())
+    assert bool((d.abs() <= 6 * 2 * 0.031 * y.square().mean().sqrt() + 2.0**-7 * want.double().abs()).all())
