@@ -91,11 +91,15 @@ int experts_shape(const mono_prompt_experts_args& a) {
   return MONO_OK;
 }
 
+// Where the wide tiles take over: rows of a product, picks a routed expert gets on average.
+constexpr int WIDE_ROWS = 96, WIDE_PICKS = 24;
+
 // The call's plan over its workspace; `e.tiles` bounds the tile list.
 size_t experts_plan(const mono_prompt_experts_args& a, void* ws, Experts& e) {
   Space sp{static_cast<char*>(ws)};
   const int64_t picks = a.tokens * a.picks, places = picks + (a.shared ? a.tokens : 0);
-  e.bm = 64;
+  e.wide = picks > WIDE_PICKS * a.experts;
+  e.bm = e.wide ? 128 : 64;
   e.tiles = (int)max_tiles(a.tokens, picks, a.experts, e.bm, a.shared);
   e.x = sp.rows(a.tokens, a.hidden);
   e.mid_q = sp.rows(places, a.inter);
@@ -148,6 +152,8 @@ extern "C" int mono_prompt_product(const mono_prompt_product_args* args, void* s
   Space sp{static_cast<char*>(a.workspace)};
   const Rows x = sp.rows(a.rows, a.k);
   if (hipError_t e = quant_rows(a.x, false, a.x_stride, a.rows, a.k, x, st)) return launched(e, "the rows' rounding");
+  if (a.rows > WIDE_ROWS)
+    return launched(wide_product(x, a.rows, a.w, a.s, a.n, a.k, a.out, a.out_f32 != 0, a.out_stride, st), "the product");
   return launched(product(x, a.rows, a.w, a.s, a.n, a.k, a.out, a.out_f32 != 0, a.out_stride, st), "the product");
 }
 
@@ -214,8 +220,13 @@ extern "C" int mono_prompt_experts(const mono_prompt_experts_args* args, void* s
   const int64_t places = e.picks + (e.shared ? e.tokens : 0);
   if (hipError_t r = sort_quant(a.x, a.x_stride, a.tokens, a.hidden, e.x, a.ids, a.picks, a.experts, e.shared, e.bm, e.sorted, st))
     return launched(r, "the tokens' sort");
-  if (hipError_t r = experts_up(e, st)) return launched(r, "the experts' up products");
-  if (hipError_t r = quant_rows(e.mid, true, e.inter, places, e.inter, e.mid_q, st)) return launched(r, "the mids' rounding");
-  if (hipError_t r = experts_down(e, st)) return launched(r, "the experts' down products");
+  if (e.wide) {
+    if (hipError_t r = wide_experts_up(e, st)) return launched(r, "the experts' up products");
+    if (hipError_t r = wide_experts_down(e, st)) return launched(r, "the experts' down products");
+  } else {
+    if (hipError_t r = experts_up(e, st)) return launched(r, "the experts' up products");
+    if (hipError_t r = quant_rows(e.mid, true, e.inter, places, e.inter, e.mid_q, st)) return launched(r, "the mids' rounding");
+    if (hipError_t r = experts_down(e, st)) return launched(r, "the experts' down products");
+  }
   return launched(experts_back(e, st), "the weighted sum");
 }

@@ -52,6 +52,11 @@ hipError_t sort_quant(const void* x, int64_t stride, int64_t tokens, int k, cons
 hipError_t product(const Rows& x, int64_t rows, const void* w, const float* s, int n, int k, void* out, bool f32,
                    int64_t out_stride, hipStream_t st);
 
+// Wide tiles (128 rows or more) where there are rows enough for them, narrow ones (64)
+// else.
+hipError_t wide_product(const Rows& x, int64_t rows, const void* w, const float* s, int n, int k, void* out, bool f32,
+                        int64_t out_stride, hipStream_t st);
+
 struct Experts {
   Rows x, mid_q;
   Sorted sorted;
@@ -65,10 +70,12 @@ struct Experts {
   int64_t out_stride;
   int64_t tokens, picks;
   int picks_each, experts, hidden, inter, bm, tiles;
-  bool shared;
+  bool shared, wide;
 };
 hipError_t experts_up(const Experts& a, hipStream_t st);
 hipError_t experts_down(const Experts& a, hipStream_t st);
+hipError_t wide_experts_up(const Experts& a, hipStream_t st);
+hipError_t wide_experts_down(const Experts& a, hipStream_t st);
 hipError_t experts_back(const Experts& a, hipStream_t st);
 
 hipError_t append(const mono_prompt_append_args& a, hipStream_t st);

@@ -1,0 +1,281 @@
+// FP8 block products over wide tiles: 256 weight rows by 128 (or 256) rows of x a workgroup.
+//
+// Four waves (twice four) hold 64 weight rows x 128 rows of x each: 4 x 8 tiles of 16 x 16,
+// 128 accumulators a lane. The weights lie in memory as the MFMA wants them, so a wave loads
+// its own straight into registers, a block of K ahead; the rows of x are shared by the
+// waves and come through LDS by DMA (global_load_lds), also a block ahead. With waves side
+// by side along the weight rows, LDS feeds 16 KB a wave and block of K (1024 cycles of
+// MFMA), half of what it can, and the weights pass no LDS at all.
+//
+// Each block's partial is scaled in f32: 4 FMAs behind each MFMA, half the vector unit's
+// time under the matrix unit's.
+#include "prompt_common.h"
+
+namespace mono {
+namespace prompt {
+namespace {
+
+constexpr int BN = 256, TN = 64, TM = 128, NT = TN / 16, MT = TM / 16, WN = BN / TN;
+
+struct Wide {
+  const uint8_t* xq;
+  const float* xs;
+  int xs_ld;
+  const uint8_t* w;
+  const float* s;
+  int n, kb;
+  int64_t rows;
+  void* out;
+  int64_t out_ld;
+  const Tile* tiles;
+  const int *n_tiles, *token;
+  int half;            // up: gate rows (the up rows follow)
+  float* mid_s;        // up: the mids' scales [inter / 128, mid_ld]
+  int mid_ld;
+  int tiles_m, tiles_n;
+};
+
+enum Mode { DENSE_BF16, DENSE_F32, UP, DOWN };
+
+template <int WM>
+struct Stage {
+  uint8_t x[WM * TM * BLK];
+  float s[WM * TM];
+};
+
+typedef __attribute__((address_space(1))) const void gvoid;
+typedef __attribute__((address_space(3))) void lvoid;
+MONO_DEV void dma16(const void* g, void* l) {
+  __builtin_amdgcn_global_load_lds((gvoid*)g, (lvoid*)l, 16, 0, 0);
+}
+MONO_DEV void dma4(const void* g, void* l) {
+  __builtin_amdgcn_global_load_lds((gvoid*)g, (lvoid*)l, 4, 0, 0);
+}
+
+template <int MODE, int WM>
+struct WideTile {
+  const Wide& a;
+  const int lane, wave, wn, wm;
+  const uint8_t* wp[NT];  // the weight tiles (uniform)
+  const float* sp[2];     // scale rows: of weight tiles 0, 1 and 2, 3
+  const uint8_t* xp[2];   // the lane's two rows of x for the DMA
+  const float* xsp;       // the lane's row of the scales for the DMA
+  f32x4 acc[NT][MT] = {};
+
+  MONO_DEV WideTile(const Wide& a_) : a(a_), lane(threadIdx.x % WAVE), wave(__builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)), wn(wave % WN), wm(wave / WN) {}
+
+  struct Ahead {
+    i32x8 w[NT];
+    float s[2];
+  };
+
+  MONO_DEV void issue(int kb, Stage<WM>& st, Ahead& n) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) dma16(xp[h] + (size_t)kb * BLK + 64 * q, &st.x[(2 * wave + h) * 2048 + 1024 * q]);
+    if (wave < WM * TM / WAVE) dma4(xsp + (size_t)kb * a.xs_ld, &st.s[wave * WAVE]);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const uint8_t* at = wp[i] + (size_t)kb * 2048;
+      const i32x4 lo = *reinterpret_cast<const i32x4*>(at + 16 * (uint32_t)lane);
+      const i32x4 hi = *reinterpret_cast<const i32x4*>(at + 16 * (uint32_t)lane + 1024);
+      n.w[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    n.s[0] = ld_const_f32(sp[0] + kb);
+    n.s[1] = ld_const_f32(sp[1] + kb);
+  }
+
+  MONO_DEV void compute(const Stage<WM>& st, const Ahead& n) {
+    const int r = lane % 16, g = lane / 16;
+    const uint8_t* x = st.x + wm * TM * BLK + r * 64 + ((g ^ (r >> 2)) * 16);
+    const float* xs = st.s + wm * TM + r;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      const i32x4 lo = *reinterpret_cast<const i32x4*>(x + j * 2048), hi = *reinterpret_cast<const i32x4*>(x + j * 2048 + 1024);
+      const i32x8 xv = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      const float sx = xs[16 * j];
+      const float c[2] = {sx * n.s[0], sx * n.s[1]};
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const f32x4 p = mfma_block<MODE == DENSE_F32>(n.w[i], xv);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(p[e], c[i / 2], acc[i][j][e]);
+      }
+      // the sums stay here: moved behind the next barrier, they would hold 64 more registers
+#pragma unroll
+      for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(acc[i][j]));
+    }
+  }
+
+  MONO_DEV void run(Stage<WM>& s0, Stage<WM>& s1) {
+    Ahead a0, a1;
+    issue(0, s0, a0);
+    int kb = 0;
+    for (; kb + 1 < a.kb; kb += 2) {
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      issue(kb + 1, s1, a1);
+      compute(s0, a0);
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      issue(min(kb + 2, a.kb - 1), s0, a0);  // past an even K's end: its last block again, not used
+      compute(s1, a1);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (kb < a.kb) compute(s0, a0);
+  }
+};
+
+template <int MODE, int WM>
+__global__ __launch_bounds__(WM * WN * WAVE, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
+  constexpr int BM = WM * TM;
+  __shared__ Stage<WM> s0, s1;
+  __shared__ uint32_t top[MODE == UP ? WN : 1][MODE == UP ? BM : 1];
+  // a block's XCD is its index modulo 8: each XCD takes neighbouring tiles, whose rows and
+  // weights its L2 then holds once for all
+  int tn, tm;
+  const int per = (gridDim.x + 7) / 8, b = (blockIdx.x % 8) * per + blockIdx.x / 8;
+  if (MODE == UP || MODE == DOWN) {
+    tn = b % a.tiles_n;
+    tm = b / a.tiles_n;
+    if (tm >= *a.n_tiles) return;
+  } else {
+    constexpr int GM = 8;  // row tiles side by side
+    const int group = b / (GM * a.tiles_n), in = b % (GM * a.tiles_n), high = min(GM, a.tiles_m - group * GM);
+    if (high <= 0) return;
+    tm = group * GM + in % high;
+    tn = in / high;
+    if (tn >= a.tiles_n) return;
+  }
+  const uint8_t* w = a.w;
+  const float* s = a.s;
+  int64_t first = (int64_t)tm * BM;
+  int count;
+  if (MODE == UP || MODE == DOWN) {
+    const Tile t = a.tiles[tm];
+    first = t.first;
+    count = t.count;
+    w += (size_t)t.expert * a.n * a.kb * BLK;
+    s += (size_t)t.expert * ((a.n + BLK - 1) / BLK) * a.kb;
+  } else {
+    count = (int)min((int64_t)BM, a.rows - first);
+  }
+
+  WideTile<MODE, WM> T(a);
+  const int lane = T.lane, wn = T.wn, wm = T.wm;
+  // the wave's weight tiles: 64 neighbouring rows, or (up) 32 gate rows and their up rows
+  int row[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    row[i] = MODE == UP ? tn * (BN / 2) + wn * (TN / 2) + 16 * (i % 2) + (i / 2) * a.half : tn * BN + wn * TN + 16 * i;
+    const int n = min(row[i], a.n - 16);  // past the matrix: its last rows again, not stored
+    T.wp[i] = w + (size_t)n * a.kb * BLK;
+    if (i % 2 == 0) T.sp[i / 2] = s + (size_t)(n / BLK) * a.kb;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = lane / 4;  // 16 rows x 64 bytes a DMA; the 16-byte pieces are swapped by row so that a
+                             // fragment's reads (16 rows, one piece) meet every bank once
+    const int64_t m = first + min((2 * T.wave + h) * 16 + r, count - 1);
+    T.xp[h] = a.xq + (size_t)(MODE == UP ? a.token[m] : m) * a.kb * BLK + (((lane % 4) ^ (r >> 2)) * 16);
+  }
+  {
+    const int64_t m = first + min((T.wave * WAVE + lane) % BM, count - 1);
+    T.xsp = a.xs + (MODE == UP ? a.token[m] : m);
+  }
+  T.run(s0, s1);
+
+  const int g = lane / 16;
+  if (MODE == UP) {
+    // mids, their block's scale over the four waves' 128 of them, codes
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float gate = T.acc[i][j][e];
+          T.acc[i][j][e] = gate / (1.0f + expf(-gate)) * T.acc[i + 2][j][e];
+          m = max(m, abs_bits(T.acc[i][j][e]));
+        }
+      m = max(m, (uint32_t)__shfl_xor((int)m, 16, WAVE));
+      m = max(m, (uint32_t)__shfl_xor((int)m, 32, WAVE));
+      if (g == 0) top[wn][wm * TM + 16 * j + lane] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      const int m = wm * TM + 16 * j + lane % 16;
+      uint32_t t = top[0][m];
+#pragma unroll
+      for (int v = 1; v < WN; ++v) t = max(t, top[v][m]);
+      const BlockScale bs = block_scale(t);
+      if (m >= count) continue;
+      uint8_t* q = static_cast<uint8_t*>(a.out) + (size_t)(first + m) * a.out_ld;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<uint32_t*>(q + row[i] + 4 * g) =
+            fp8x4_pack(to_code_range(T.acc[i][j][0], bs), to_code_range(T.acc[i][j][1], bs),
+                       to_code_range(T.acc[i][j][2], bs), to_code_range(T.acc[i][j][3], bs));
+      if (wn == 0 && g == 0) a.mid_s[(size_t)tn * a.mid_ld + first + m] = bs.scale;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    const int m = wm * TM + 16 * j + lane % 16;
+    if (m >= count) continue;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      if (row[i] >= a.n) continue;
+      const size_t at = (size_t)(first + m) * a.out_ld + row[i] + 4 * g;
+      const f32x4 y = T.acc[i][j];
+      if (MODE == DENSE_BF16)
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+      else
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = y;
+    }
+  }
+}
+
+template <int MODE, int WM>
+hipError_t launch(const Wide& a, int64_t tiles, hipStream_t st) {
+  const uint32_t grid = (uint32_t)((tiles + 7) / 8 * 8);
+  k_wide<MODE, WM><<<grid, WM * WN * WAVE, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t wide_product(const Rows& x, int64_t rows, const void* w, const float* s, int n, int k, void* out, bool f32,
+                        int64_t out_stride, hipStream_t st) {
+  Wide a{x.q, x.s, x.ld, static_cast<const uint8_t*>(w), s, n, k / BLK, rows, out, out_stride};
+  a.tiles_n = (n + BN - 1) / BN;
+  const bool two = !f32 && rows > 4 * TM;
+  const int bm = two ? 2 * TM : TM;
+  a.tiles_m = (int)((rows + bm - 1) / bm);
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+  if (f32) return launch<DENSE_F32, 1>(a, tiles, st);
+  return two ? launch<DENSE_BF16, 2>(a, tiles, st) : launch<DENSE_BF16, 1>(a, tiles, st);
+}
+
+hipError_t wide_experts_up(const Experts& e, hipStream_t st) {
+  Wide a{e.x.q, e.x.s, e.x.ld, e.w13, e.s13, 2 * e.inter, e.hidden / BLK, 0, e.mid_q.q, e.inter,
+         e.sorted.tiles, e.sorted.n_tiles, e.sorted.token, e.inter, e.mid_q.s, e.mid_q.ld};
+  a.tiles_n = e.inter / BLK;
+  return launch<UP, 1>(a, (int64_t)e.tiles * a.tiles_n, st);
+}
+
+hipError_t wide_experts_down(const Experts& e, hipStream_t st) {
+  Wide a{e.mid_q.q, e.mid_q.s, e.mid_q.ld, e.w2, e.s2, e.hidden, e.inter / BLK, 0, e.part, e.hidden,
+         e.sorted.tiles, e.sorted.n_tiles, e.sorted.token};
+  a.tiles_n = (e.hidden + BN - 1) / BN;
+  return launch<DOWN, 1>(a, (int64_t)e.tiles * a.tiles_n, st);
+}
+
+}  // namespace prompt
+}  // namespace mono
