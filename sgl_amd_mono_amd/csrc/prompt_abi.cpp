@@ -100,12 +100,14 @@ size_t experts_plan(const mono_prompt_experts_args& a, void* ws, Experts& e) {
   const int64_t picks = a.tokens * a.picks, places = picks + (a.shared ? a.tokens : 0);
   e.wide = picks > WIDE_PICKS * a.experts;
   e.bm = e.wide ? 128 : 64;
-  e.tiles = (int)max_tiles(a.tokens, picks, a.experts, e.bm, a.shared);
+  e.tiles = (int)all_tiles(a.tokens, picks, a.experts, e.bm, a.shared);
   e.x = sp.rows(a.tokens, a.hidden);
   e.mid_q = sp.rows(places, a.inter);
-  e.sorted = Sorted{sp.take<int>(places), sp.take<int>(picks), sp.take<Tile>(e.tiles), sp.take<int>(1)};
-  e.mid = sp.take<float>((size_t)places * a.inter);
-  e.part = sp.take<float>((size_t)places * a.hidden);
+  e.sorted = Sorted{sp.take<int>(places), sp.take<int>(picks), sp.take<Tile>(e.tiles)};
+  e.mid = e.wide ? nullptr : sp.take<float>((size_t)places * a.inter);
+  e.part.v = sp.take<uint16_t>((size_t)places * a.hidden);
+  e.part.s = sp.take<float>((size_t)places * (a.hidden / PART));
+  e.part.ld = a.hidden;
   e.w13 = static_cast<const uint8_t*>(a.w13);
   e.w2 = static_cast<const uint8_t*>(a.w2);
   e.s13 = a.s13;

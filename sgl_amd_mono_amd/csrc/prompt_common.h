@@ -112,5 +112,32 @@ MONO_DEV void load8(const float* p, float (&v)[8]) {
   }
 }
 
+MONO_DEV float half_to_f32(uint32_t bits) { return (float)__builtin_bit_cast(_Float16, (uint16_t)bits); }
+MONO_DEV uint32_t pack_halves(float a, float b) {
+  return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
+}
+
+// Store one place's share of a wave's 16 x NT tiles x MT: lane l holds columns 16 i + 4 (l /
+// 16) .. + 3 of 64 (NT = 4), the four lane groups together a block of Parts.
+MONO_DEV void store_part(const Parts& p, int64_t place, int col, const f32x4 (&y)[4], bool in) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = max(m, abs_bits(y[i][e]));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 16, WAVE));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 32, WAVE));
+  // 2^14 / 2^floor(log2 max); a block that is not finite keeps its values as they are
+  const int e = m < 0x7f800000u ? max((int)(m >> 23), 27) : 127 + 14;
+  const float inv = __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
+  if (!in) return;
+  const int g = lane_id() / 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<u32x2*>(p.v + place * p.ld + col + 16 * i + 4 * g) =
+        u32x2{pack_halves(y[i][0] * inv, y[i][1] * inv), pack_halves(y[i][2] * inv, y[i][3] * inv)};
+  if (g == 0) p.s[place * (p.ld / PART) + col / PART] = __uint_as_float((uint32_t)(e - 14) << 23);
+}
+
 }  // namespace prompt
 }  // namespace mono

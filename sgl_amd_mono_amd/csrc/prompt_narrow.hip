@@ -25,11 +25,11 @@ struct Narrow {
   void* out;
   int64_t out_ld;
   const Tile* tiles;   // experts: the tile list and its length
-  const int *n_tiles, *token;
+  const int* token;
   int half;            // up: gate rows (the up rows follow)
 };
 
-enum Mode { DENSE_BF16, DENSE_F32, UP, DOWN };
+enum Mode { DENSE_BF16, DENSE_F32, UP };
 
 MONO_DEV i32x8 ld_pair(const uint8_t* p, size_t far) {
   const i32x4 a = *reinterpret_cast<const i32x4*>(p), b = *reinterpret_cast<const i32x4*>(p + far);
@@ -123,14 +123,14 @@ __global__ __launch_bounds__(T) void k_narrow(Narrow a) {
   __shared__ f32x4 red[WV * NT * 4 * WAVE];
   const int n0 = blockIdx.x * 16;
   int64_t first = (int64_t)blockIdx.y * BM;
-  int count = MODE == UP || MODE == DOWN ? 0 : (int)min((int64_t)BM, a.rows - first);
+  int count = MODE == UP ? 0 : (int)min((int64_t)BM, a.rows - first);
   const uint8_t* w = a.w;
   const float* s = a.s;
-  if (MODE == UP || MODE == DOWN) {
-    if ((int)blockIdx.y >= *a.n_tiles) return;
+  if (MODE == UP) {
     const Tile t = a.tiles[blockIdx.y];
     first = t.first;
     count = t.count;
+    if (count == 0) return;
     w += (size_t)t.expert * a.n * a.kb * BLK;
     s += (size_t)t.expert * ((a.n + BLK - 1) / BLK) * a.kb;
   }
@@ -142,11 +142,76 @@ __global__ __launch_bounds__(T) void k_narrow(Narrow a) {
     narrow_tile<MODE, NT, 4>(a, red, w, s, n0, first, count);
 }
 
+// The experts' down products: K is the mids' few blocks, so the waves share out the weight
+// rows (64 each) and not K, and each ends with whole sums.
+constexpr int DT = 256, DN = 256, DW = DN / (DT / WAVE) / 16;
+static_assert(16 * DW == PART, "a wave's weight rows are a block of Parts");
+
+template <int MT>
+MONO_DEV void down_tile(const Experts& a, const Tile& t, int n0) {
+  constexpr int U = MT == 1 ? 4 : MT == 2 ? 2 : 1;
+  const int lane = threadIdx.x % WAVE, kb = a.inter / BLK;
+  const uint8_t* w = a.w2 + ((size_t)t.expert * a.hidden + n0) * a.inter;
+  const float* s = a.s2 + ((size_t)t.expert * (a.hidden / BLK) + n0 / BLK) * kb;
+  const uint8_t* xp[MT];
+  const float* xsp[MT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    const int m = t.first + min(16 * j + lane % 16, t.count - 1);
+    xp[j] = a.mid_q.q + (size_t)m * a.inter + 16 * (lane / 16);
+    xsp[j] = a.mid_q.s + m;
+  }
+  f32x4 acc[MT][DW] = {};
+  for (int b0 = 0; b0 < kb; b0 += U) {
+    i32x8 wv[U][DW], xv[U][MT];
+    float c[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int b = min(b0 + u, kb - 1);
+      const float sw = b0 + u < kb ? s[b] : 0.f;  // past the end: the last block again, scaled by zero
+#pragma unroll
+      for (int i = 0; i < DW; ++i) wv[u][i] = ld_pair(w + (size_t)i * 16 * a.inter + (size_t)b * 2048 + 16 * lane, 1024);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        xv[u][j] = ld_pair(xp[j] + (size_t)b * BLK, 64);
+        c[u][j] = xsp[j][(size_t)b * a.mid_q.ld] * sw;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int i = 0; i < DW; ++i) {
+          const f32x4 p = mfma_block<false>(wv[u][i], xv[u][j]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(p[r], c[u][j], acc[j][i][r]);
+        }
+  }
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    const int m = 16 * j + lane % 16;
+    store_part(a.part, t.first + m, n0, acc[j], m < t.count);
+  }
+}
+
+__global__ __launch_bounds__(DT) void k_down(Experts a) {
+  const Tile t = a.sorted.tiles[blockIdx.y];
+  const int n0 = blockIdx.x * DN + threadIdx.x / WAVE * PART;
+  if (t.count == 0 || n0 >= a.hidden) return;
+  if (t.count <= 16)
+    down_tile<1>(a, t, n0);
+  else if (t.count <= 32)
+    down_tile<2>(a, t, n0);
+  else
+    down_tile<4>(a, t, n0);
+}
+
 }  // namespace
 
 hipError_t product(const Rows& x, int64_t rows, const void* w, const float* s, int n, int k, void* out, bool f32,
                    int64_t out_stride, hipStream_t st) {
-  Narrow a{x.q, x.s, x.ld, static_cast<const uint8_t*>(w), s, n, k / BLK, rows, out, out_stride, nullptr, nullptr, nullptr, 0};
+  Narrow a{x.q, x.s, x.ld, static_cast<const uint8_t*>(w), s, n, k / BLK, rows, out, out_stride, nullptr, nullptr, 0};
   const dim3 grid(n / 16, (uint32_t)((rows + BM - 1) / BM));
   if (f32)
     k_narrow<DENSE_F32><<<grid, T, 0, st>>>(a);
@@ -157,15 +222,13 @@ hipError_t product(const Rows& x, int64_t rows, const void* w, const float* s, i
 
 hipError_t experts_up(const Experts& e, hipStream_t st) {
   Narrow a{e.x.q, e.x.s, e.x.ld, e.w13, e.s13, 2 * e.inter, e.hidden / BLK, 0, e.mid, e.inter,
-           e.sorted.tiles, e.sorted.n_tiles, e.sorted.token, e.inter};
+           e.sorted.tiles, e.sorted.token, e.inter};
   k_narrow<UP><<<dim3(e.inter / 16, e.tiles), T, 0, st>>>(a);
   return hipGetLastError();
 }
 
 hipError_t experts_down(const Experts& e, hipStream_t st) {
-  Narrow a{e.mid_q.q, e.mid_q.s, e.mid_q.ld, e.w2, e.s2, e.hidden, e.inter / BLK, 0, e.part, e.hidden,
-           e.sorted.tiles, e.sorted.n_tiles, e.sorted.token, 0};
-  k_narrow<DOWN><<<dim3(e.hidden / 16, e.tiles), T, 0, st>>>(a);
+  k_down<<<dim3((e.hidden + DN - 1) / DN, e.tiles), DT, 0, st>>>(e);
   return hipGetLastError();
 }
 

@@ -11,7 +11,7 @@ namespace mono {
 namespace prompt {
 
 constexpr int BLK = 128;             // a scale's block of rows' and weights' columns
-constexpr int MAX_EXPERTS = 1024;    // routed experts (a sort block's LDS histogram)
+constexpr int MAX_EXPERTS = 1024;    // routed experts (a sort block each)
 constexpr int MAX_DIM = 1 << 16;     // columns and outputs of a product
 constexpr int64_t MAX_ROWS = 1 << 20;  // rows a call; picks of all rows of an experts call
 
@@ -35,16 +35,26 @@ struct Tile {
 struct Sorted {
   int* token;  // [picks + tokens] token of each place
   int* place;  // [picks] place of each pick (token * k + j), -1: routed nowhere
-  Tile* tiles; // [max_tiles]
-  int* n_tiles;
+  Tile* tiles; // [all_tiles], some of them empty (count 0)
 };
 
-// The tile list's bound: the shared expert's tiles, then every routed expert's whole
-// tiles and at most one partial tile for each expert that is picked.
-inline int64_t max_tiles(int64_t tokens, int64_t picks, int experts, int bm, bool shared) {
-  const int64_t part = picks < experts ? picks : experts;
-  return (shared ? (tokens + bm - 1) / bm : 0) + picks / bm + part;
+// The tile list's length: the shared expert's tiles, then room for every routed expert's
+// whole tiles and a partial one of each (and never more than one for each pick).
+inline int64_t all_tiles(int64_t tokens, int64_t picks, int experts, int bm, bool shared) {
+  const int64_t routed = picks / bm + experts;
+  return (shared ? (tokens + bm - 1) / bm : 0) + (picks < routed ? picks : routed);
 }
+
+// The experts' outputs before their weighted sum, [places, ld]: f16 values and, for each 64
+// columns of a place, the power of two that they are multiplied by, which puts the largest
+// of them into [2^14, 2^15). 16 bits halve the bytes of the largest tensor of a call, and
+// against bf16's 2^-9 such a block's values are 2^-12 off.
+constexpr int PART = 64;
+struct Parts {
+  uint16_t* v;
+  float* s;
+  int ld;
+};
 
 hipError_t quant_rows(const void* x, bool f32, int64_t stride, int64_t rows, int k, const Rows& out, hipStream_t st);
 hipError_t sort_quant(const void* x, int64_t stride, int64_t tokens, int k, const Rows& out, const int* ids, int picks_each,
@@ -60,8 +70,8 @@ hipError_t wide_product(const Rows& x, int64_t rows, const void* w, const float*
 struct Experts {
   Rows x, mid_q;
   Sorted sorted;
-  float* mid;   // f32 [places, inter]
-  float* part;  // f32 [places, hidden]
+  float* mid;  // f32 [places, inter]
+  Parts part;
   const uint8_t *w13, *w2;
   const float *s13, *s2, *weights;
   const void* residual;

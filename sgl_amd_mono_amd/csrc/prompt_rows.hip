@@ -6,7 +6,7 @@ namespace mono {
 namespace prompt {
 namespace {
 
-constexpr int T = 512;      // threads of the row kernels
+constexpr int T = 1024;     // threads of the row kernels
 constexpr int WV = T / WAVE;
 
 // 16 lanes round one block of 128 columns, 8 a lane. `block` counts the blocks of all
@@ -32,10 +32,14 @@ __global__ __launch_bounds__(T) void k_quant_rows(const V* x, int64_t stride, ui
 
 // Blocks [0, experts) sort, the others round rows: neither needs the other.
 //
-// Sort block e counts every expert's picks in LDS (integer atomics: the order does not
-// show), so it knows where its own places and tiles begin without another launch, then
-// lists its picks in the tokens' order: each wave takes one contiguous share, counts
-// its matches, and writes them behind those of the waves before it.
+// Sort block e counts the picks of expert e and those of the experts before it, so it knows
+// its first place, and writes its picks there, in an order that is its threads' own (a
+// place's position among its expert's decides nothing: a row's sums are its own). Its tiles
+// go where the counts alone say, too: the experts before e have b places in at most
+// min(b, b / bm + e) tiles, so that is where its own begin, and what it has no tile for up
+// to the next expert's is left empty (count 0).
+MONO_DEV int tiles_before(int places, int e, int bm) { return min(places, places / bm + e); }
+
 __global__ __launch_bounds__(T) void k_sort_quant(const uint16_t* x, int64_t stride, uint32_t n_blocks, int kb, Rows out,
                                                   const int* ids, int tokens, int k, int experts, int shared, int bm,
                                                   Sorted S) {
@@ -44,57 +48,53 @@ __global__ __launch_bounds__(T) void k_sort_quant(const uint16_t* x, int64_t str
     quant_block(x, stride, n_blocks, kb, out, (blockIdx.x - experts) * (T / 16) + tid / 16, tid % 16);
     return;
   }
-  __shared__ int hist[MAX_EXPERTS];
-  __shared__ int part[WV][3], found[WV];
+  __shared__ int part[WV][2];
   const int picks = tokens * k, sh_tiles = shared ? (tokens + bm - 1) / bm : 0;
-  for (int i = tid; i < experts; i += T) hist[i] = 0;
-  __syncthreads();
+  int mine = 0, less = 0;
+#pragma unroll 8
   for (int i = tid; i < picks; i += T) {
     const int id = ids[i];
-    if (id >= 0 && id < experts) atomicAdd(&hist[id], 1);
-    else if (e == 0) S.place[i] = -1;
+    mine += id == e ? 1 : 0;
+    less += id >= 0 && id < e ? 1 : 0;
+    if (e == 0 && (id < 0 || id >= experts)) S.place[i] = -1;
   }
+  const int incl = wave_incl_scan(mine), all_less = wave_sum_i(less);
+  if (lane == WAVE - 1) part[wave][0] = incl, part[wave][1] = all_less;
   __syncthreads();
-  // places and tiles of the experts before this one, and (for the list's length) all tiles
-  int before = 0, tiles = 0, all = 0;
-  for (int j = tid; j < experts; j += T) {
-    const int t = (hist[j] + bm - 1) / bm;
-    all += t;
-    if (j < e) before += hist[j], tiles += t;
-  }
-  before = wave_sum_i(before), tiles = wave_sum_i(tiles), all = wave_sum_i(all);
-  if (lane == 0) part[wave][0] = before, part[wave][1] = tiles, part[wave][2] = all;
-  __syncthreads();
-  before = 0, tiles = sh_tiles, all = sh_tiles;
+  int first = 0, count = 0, at = incl - mine;
 #pragma unroll
-  for (int w = 0; w < WV; ++w) before += part[w][0], tiles += part[w][1], all += part[w][2];
-  const int count = hist[e];
-  for (int j = tid; j < (count + bm - 1) / bm; j += T) S.tiles[tiles + j] = Tile{e, before + j * bm, min(bm, count - j * bm), 0};
-  if (e == 0 && tid == 0) *S.n_tiles = all;
+  for (int w = 0; w < WV; ++w) {
+    at += w < wave ? part[w][0] : 0;
+    count += part[w][0];
+    first += part[w][1];
+  }
+  const int t0 = tiles_before(first, e, bm);
+  const int t1 = e == experts - 1 ? tiles_before(picks, experts, bm) : tiles_before(first + count, e + 1, bm);
+  for (int j = tid; j < t1 - t0; j += T)
+    S.tiles[sh_tiles + t0 + j] = Tile{e, first + j * bm, max(0, min(bm, count - j * bm)), 0};
   if (shared) {
     for (int t = e * T + tid; t < tokens; t += experts * T) S.token[picks + t] = t;
     for (int j = e * T + tid; j < sh_tiles; j += experts * T)
       S.tiles[j] = Tile{experts, picks + j * bm, min(bm, tokens - j * bm), 0};
   }
   if (count == 0) return;
-  const int share = ((picks + WV - 1) / WV + WAVE - 1) / WAVE * WAVE;  // whole waves of picks
-  const int i0 = min(picks, wave * share), i1 = min(picks, i0 + share);
-  int mine = 0;
-  for (int i = i0; i < i1; i += WAVE) mine += __popcll(__ballot(i + lane < i1 && ids[min(i + lane, i1 - 1)] == e));
-  if (lane == 0) found[wave] = mine;
-  __syncthreads();
-  int at = before;
-#pragma unroll
-  for (int w = 0; w < WV; ++w) at += w < wave ? found[w] : 0;
-  for (int i = i0; i < i1; i += WAVE) {
-    const bool hit = i + lane < i1 && ids[min(i + lane, i1 - 1)] == e;
-    const uint64_t bal = __ballot(hit);
-    if (hit) {
-      const int p = at + __popcll(bal & ((1ull << lane) - 1ull));
-      S.place[i + lane] = p;
-      S.token[p] = (i + lane) / k;
+  at += first;
+#pragma unroll 8
+  for (int i = tid; i < picks; i += T)
+    if (ids[i] == e) {
+      S.place[i] = at;
+      S.token[at++] = i / k;
     }
-    at += __popcll(bal);
+}
+
+MONO_DEV void load_part(const Parts& p, int64_t place, int c, float (&v)[8]) {
+  const u32x4 u = ld_u32x4(p.v + place * p.ld + c);
+  const float s = p.s[place * (p.ld / PART) + c / PART];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = u[i];
+    v[2 * i] = half_to_f32(w) * s;
+    v[2 * i + 1] = half_to_f32(w >> 16) * s;
   }
 }
 
@@ -103,22 +103,32 @@ __global__ __launch_bounds__(T) void k_sort_quant(const uint16_t* x, int64_t str
 __global__ __launch_bounds__(128) void k_back(Experts a) {
   const int t = blockIdx.x, c = (blockIdx.y * 128 + threadIdx.x) * 8;
   if (c >= a.hidden) return;
-  float y[8], v[8];
+  constexpr int U = 8;  // picks loaded together
+  float y[8], v[U][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = 0.f;
-  if (a.shared) load8(a.part + (size_t)(a.picks + t) * a.hidden + c, y);
-  for (int j = 0; j < a.picks_each; ++j) {
-    const int p = a.sorted.place[(size_t)t * a.picks_each + j];
-    if (p < 0) continue;
-    const float w = a.weights[(size_t)t * a.picks_each + j];
-    load8(a.part + (size_t)p * a.hidden + c, v);
+  if (a.shared) load_part(a.part, a.picks + t, c, y);
+  for (int j0 = 0; j0 < a.picks_each; j0 += U) {
+    float w[U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = fmaf(w, v[i], y[i]);
+    for (int u = 0; u < U; ++u) {
+      const int64_t j = (int64_t)t * a.picks_each + min(j0 + u, a.picks_each - 1);
+      const int p = j0 + u < a.picks_each ? a.sorted.place[j] : -1;
+      load_part(a.part, max(p, 0), c, v[u]);  // no place: any place's, not added
+      w[u] = p < 0 ? 0.f : a.weights[j];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[u][i] = p < 0 ? 0.f : v[u][i];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = fmaf(w[u], v[u][i], y[i]);
   }
   if (a.residual) {
-    load8(static_cast<const uint16_t*>(a.residual) + (int64_t)t * a.residual_stride + c, v);
+    float r[8];
+    load8(static_cast<const uint16_t*>(a.residual) + (int64_t)t * a.residual_stride + c, r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] += v[i];
+    for (int i = 0; i < 8; ++i) y[i] += r[i];
   }
   *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + (int64_t)t * a.out_stride + c) =
       u32x4{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7])};

@@ -28,14 +28,16 @@ struct Wide {
   void* out;
   int64_t out_ld;
   const Tile* tiles;
-  const int *n_tiles, *token;
+  const int* token;
   int half;            // up: gate rows (the up rows follow)
   float* mid_s;        // up: the mids' scales [inter / 128, mid_ld]
   int mid_ld;
+  Parts part;          // down
   int tiles_m, tiles_n;
 };
 
 enum Mode { DENSE_BF16, DENSE_F32, UP, DOWN };
+static_assert(TN == PART, "a wave's weight rows are a block of Parts");
 
 template <int WM>
 struct Stage {
@@ -140,7 +142,7 @@ __global__ __launch_bounds__(WM * WN * WAVE, MODE == DENSE_F32 ? 1 : 2) void k_w
   if (MODE == UP || MODE == DOWN) {
     tn = b % a.tiles_n;
     tm = b / a.tiles_n;
-    if (tm >= *a.n_tiles) return;
+    if (tm >= a.tiles_m) return;
   } else {
     constexpr int GM = 8;  // row tiles side by side
     const int group = b / (GM * a.tiles_n), in = b % (GM * a.tiles_n), high = min(GM, a.tiles_m - group * GM);
@@ -157,6 +159,7 @@ __global__ __launch_bounds__(WM * WN * WAVE, MODE == DENSE_F32 ? 1 : 2) void k_w
     const Tile t = a.tiles[tm];
     first = t.first;
     count = t.count;
+    if (count == 0) return;
     w += (size_t)t.expert * a.n * a.kb * BLK;
     s += (size_t)t.expert * ((a.n + BLK - 1) / BLK) * a.kb;
   } else {
@@ -228,6 +231,11 @@ __global__ __launch_bounds__(WM * WN * WAVE, MODE == DENSE_F32 ? 1 : 2) void k_w
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
     const int m = wm * TM + 16 * j + lane % 16;
+    if (MODE == DOWN) {
+      const f32x4 y[NT] = {T.acc[0][j], T.acc[1][j], T.acc[2][j], T.acc[3][j]};
+      store_part(a.part, first + m, row[0], y, m < count && row[0] < a.n);
+      continue;
+    }
     if (m >= count) continue;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -265,14 +273,17 @@ hipError_t wide_product(const Rows& x, int64_t rows, const void* w, const float*
 
 hipError_t wide_experts_up(const Experts& e, hipStream_t st) {
   Wide a{e.x.q, e.x.s, e.x.ld, e.w13, e.s13, 2 * e.inter, e.hidden / BLK, 0, e.mid_q.q, e.inter,
-         e.sorted.tiles, e.sorted.n_tiles, e.sorted.token, e.inter, e.mid_q.s, e.mid_q.ld};
+         e.sorted.tiles, e.sorted.token, e.inter, e.mid_q.s, e.mid_q.ld};
+  a.tiles_m = e.tiles;
   a.tiles_n = e.inter / BLK;
   return launch<UP, 1>(a, (int64_t)e.tiles * a.tiles_n, st);
 }
 
 hipError_t wide_experts_down(const Experts& e, hipStream_t st) {
-  Wide a{e.mid_q.q, e.mid_q.s, e.mid_q.ld, e.w2, e.s2, e.hidden, e.inter / BLK, 0, e.part, e.hidden,
-         e.sorted.tiles, e.sorted.n_tiles, e.sorted.token};
+  Wide a{e.mid_q.q, e.mid_q.s, e.mid_q.ld, e.w2, e.s2, e.hidden, e.inter / BLK, 0, nullptr, 0,
+         e.sorted.tiles, e.sorted.token};
+  a.part = e.part;
+  a.tiles_m = e.tiles;
   a.tiles_n = (e.hidden + BN - 1) / BN;
   return launch<DOWN, 1>(a, (int64_t)e.tiles * a.tiles_n, st);
 }
