@@ -1,7 +1,7 @@
-// FP8 block products over wide tiles: 256 weight rows by 128 (or 256) rows of x a workgroup.
+// FP8 block products over wide tiles: 256 weight rows by 128 (or 64) rows of x a workgroup.
 //
-// Four waves (twice four) hold 64 weight rows x 128 rows of x each: 4 x 8 tiles of 16 x 16,
-// 128 accumulators a lane. The weights lie in memory as the MFMA wants them, so a wave loads
+// Four waves hold 64 weight rows x 128 rows of x each: 4 x 8 tiles of 16 x 16, 128
+// accumulators a lane. The weights lie in memory as the MFMA wants them, so a wave loads
 // its own straight into registers, a block of K ahead; the rows of x are shared by the
 // waves and come through LDS by DMA (global_load_lds), also a block ahead. With waves side
 // by side along the weight rows, LDS feeds 16 KB a wave and block of K (1024 cycles of
@@ -15,7 +15,7 @@ namespace mono {
 namespace prompt {
 namespace {
 
-constexpr int BN = 256, TN = 64, TM = 128, NT = TN / 16, MT = TM / 16, WN = BN / TN;
+constexpr int BN = 256, TN = 64, NT = TN / 16, WN = BN / TN, T = WN * WAVE;
 
 struct Wide {
   const uint8_t* xq;
@@ -39,10 +39,10 @@ struct Wide {
 enum Mode { DENSE_BF16, DENSE_F32, UP, DOWN };
 static_assert(TN == PART, "a wave's weight rows are a block of Parts");
 
-template <int WM>
+template <int MT>
 struct Stage {
-  uint8_t x[WM * TM * BLK];
-  float s[WM * TM];
+  uint8_t x[16 * MT * BLK];
+  float s[MT == 4 ? WN : 1][16 * MT];  // (64 rows: a copy a wave, so that every wave issues the same loads)
 };
 
 typedef __attribute__((address_space(1))) const void gvoid;
@@ -54,29 +54,33 @@ MONO_DEV void dma4(const void* g, void* l) {
   __builtin_amdgcn_global_load_lds((gvoid*)g, (lvoid*)l, 4, 0, 0);
 }
 
-template <int MODE, int WM>
+template <int MODE, int MT>
 struct WideTile {
+  static constexpr int XD = MT / 4;  // groups of 16 rows of x that a wave brings
   const Wide& a;
-  const int lane, wave, wn, wm;
+  const int lane, wave;
   const uint8_t* wp[NT];  // the weight tiles (uniform)
   const float* sp[2];     // scale rows: of weight tiles 0, 1 and 2, 3
-  const uint8_t* xp[2];   // the lane's two rows of x for the DMA
+  const uint8_t* xp[XD];  // the lane's rows of x for the DMA
   const float* xsp;       // the lane's row of the scales for the DMA
   f32x4 acc[NT][MT] = {};
 
-  MONO_DEV WideTile(const Wide& a_) : a(a_), lane(threadIdx.x % WAVE), wave(__builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)), wn(wave % WN), wm(wave / WN) {}
+  MONO_DEV WideTile(const Wide& a_) : a(a_), lane(threadIdx.x % WAVE), wave(__builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)) {}
 
   struct Ahead {
     i32x8 w[NT];
     float s[2];
   };
 
-  MONO_DEV void issue(int kb, Stage<WM>& st, Ahead& n) {
+  MONO_DEV void issue(int kb, Stage<MT>& st, Ahead& n) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < XD; ++h)
 #pragma unroll
-      for (int q = 0; q < 2; ++q) dma16(xp[h] + (size_t)kb * BLK + 64 * q, &st.x[(2 * wave + h) * 2048 + 1024 * q]);
-    if (wave < WM * TM / WAVE) dma4(xsp + (size_t)kb * a.xs_ld, &st.s[wave * WAVE]);
+      for (int q = 0; q < 2; ++q) dma16(xp[h] + (size_t)kb * BLK + 64 * q, &st.x[(XD * wave + h) * 2048 + 1024 * q]);
+    if (MT == 4)
+      dma4(xsp + (size_t)kb * a.xs_ld, st.s[wave]);
+    else if (wave < MT / 4)
+      dma4(xsp + (size_t)kb * a.xs_ld, &st.s[0][wave * WAVE]);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const uint8_t* at = wp[i] + (size_t)kb * 2048;
@@ -88,52 +92,97 @@ struct WideTile {
     n.s[1] = ld_const_f32(sp[1] + kb);
   }
 
-  MONO_DEV void compute(const Stage<WM>& st, const Ahead& n) {
+  MONO_DEV void compute(const Stage<MT>& st, const Ahead& n) {
     const int r = lane % 16, g = lane / 16;
-    const uint8_t* x = st.x + wm * TM * BLK + r * 64 + ((g ^ (r >> 2)) * 16);
-    const float* xs = st.s + wm * TM + r;
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
+    const uint8_t* x = st.x + r * 64 + ((g ^ (r >> 2)) * 16);
+    const float* xs = st.s[MT == 4 ? wave : 0] + r;
+    i32x8 xv[2];  // a fragment ahead: its LDS latency lies under the MFMAs of the one before
+    float sx[2];
+    const auto load = [&](int j) {
       const i32x4 lo = *reinterpret_cast<const i32x4*>(x + j * 2048), hi = *reinterpret_cast<const i32x4*>(x + j * 2048 + 1024);
-      const i32x8 xv = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      const float sx = xs[16 * j];
-      const float c[2] = {sx * n.s[0], sx * n.s[1]};
+      xv[j % 2] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      sx[j % 2] = xs[16 * j];
+    };
+    load(0);
+    // each MFMA ahead of the FMAs of the one before it: neither waits for the other
+    f32x4 p[2];
+    float c[2][2];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const f32x4 p = mfma_block<MODE == DENSE_F32>(n.w[i], xv);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(p[e], c[i / 2], acc[i][j][e]);
+    for (int t = 0; t <= MT * NT; ++t) {
+      const int i = t % NT, j = t / NT, v = t - 1;
+      if (t < MT * NT) {
+        if (i == 0 && j + 1 < MT) load(j + 1);
+        p[t % 2] = mfma_block<MODE == DENSE_F32>(n.w[i], xv[j % 2]);
+        if (i == 0) c[j % 2][0] = sx[j % 2] * n.s[0], c[j % 2][1] = sx[j % 2] * n.s[1];
+        __builtin_amdgcn_sched_barrier(0);
       }
-      // the sums stay here: moved behind the next barrier, they would hold 64 more registers
+      if (t > 0) {
+        f32x4& to = acc[v % NT][v / NT];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(acc[i][j]));
+        for (int e = 0; e < 4; ++e) to[e] = fmaf(p[v % 2][e], c[v / NT % 2][v % NT / 2], to[e]);
+        // the sums stay here: moved behind the next barrier, they would hold 64 more registers
+        asm volatile("" : "+v"(to));
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
-  MONO_DEV void run(Stage<WM>& s0, Stage<WM>& s1) {
+  // The wave's loads but the last `LEFT` have come, and every wave's: a stage is whole.
+  template <int LEFT>
+  MONO_DEV void arrive() {
+    __builtin_amdgcn_s_waitcnt((LEFT & 15) | 7 << 4 | (LEFT >> 4) << 14);  // (and lgkmcnt 0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+
+  // 128 rows: one block of K ahead. Past the end the last block comes again and is not used.
+  MONO_DEV void run(Stage<MT>& s0, Stage<MT>& s1) {
     Ahead a0, a1;
     issue(0, s0, a0);
     int kb = 0;
     for (; kb + 1 < a.kb; kb += 2) {
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
+      arrive<0>();
       issue(kb + 1, s1, a1);
       compute(s0, a0);
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
-      issue(min(kb + 2, a.kb - 1), s0, a0);  // past an even K's end: its last block again, not used
+      arrive<0>();
+      issue(min(kb + 2, a.kb - 1), s0, a0);
       compute(s1, a1);
     }
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
+    arrive<0>();
     if (kb < a.kb) compute(s0, a0);
+  }
+
+  // 64 rows: half the MFMA time a block to hide the same latency under, so two blocks ahead.
+  MONO_DEV void run(Stage<MT>& s0, Stage<MT>& s1, Stage<MT>& s2) {
+    constexpr int EACH = 2 * XD + 1 + 2 * NT;  // a stage's loads, the same for every wave
+    const int last = a.kb - 1;
+    Ahead a0, a1, a2;
+    issue(0, s0, a0);
+    issue(min(1, last), s1, a1);
+    int kb = 0;
+    for (; kb + 2 < a.kb; kb += 3) {
+      arrive<EACH>();
+      issue(min(kb + 2, last), s2, a2);
+      compute(s0, a0);
+      arrive<EACH>();
+      issue(min(kb + 3, last), s0, a0);
+      compute(s1, a1);
+      arrive<EACH>();
+      issue(min(kb + 4, last), s1, a1);
+      compute(s2, a2);
+    }
+    arrive<0>();
+    if (kb < a.kb) compute(s0, a0);
+    if (kb + 1 < a.kb) compute(s1, a1);
   }
 };
 
-template <int MODE, int WM>
-__global__ __launch_bounds__(WM * WN * WAVE, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
-  constexpr int BM = WM * TM;
-  __shared__ Stage<WM> s0, s1;
+template <int MODE, int MT>
+__global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
+  constexpr int BM = 16 * MT;
+  __shared__ Stage<MT> s0, s1;
+  __shared__ Stage<4> s2;
   __shared__ uint32_t top[MODE == UP ? WN : 1][MODE == UP ? BM : 1];
   // a block's XCD is its index modulo 8: each XCD takes neighbouring tiles, whose rows and
   // weights its L2 then holds once for all
@@ -166,29 +215,32 @@ __global__ __launch_bounds__(WM * WN * WAVE, MODE == DENSE_F32 ? 1 : 2) void k_w
     count = (int)min((int64_t)BM, a.rows - first);
   }
 
-  WideTile<MODE, WM> T(a);
-  const int lane = T.lane, wn = T.wn, wm = T.wm;
+  WideTile<MODE, MT> W(a);
+  const int lane = W.lane, wn = W.wave;
   // the wave's weight tiles: 64 neighbouring rows, or (up) 32 gate rows and their up rows
   int row[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     row[i] = MODE == UP ? tn * (BN / 2) + wn * (TN / 2) + 16 * (i % 2) + (i / 2) * a.half : tn * BN + wn * TN + 16 * i;
     const int n = min(row[i], a.n - 16);  // past the matrix: its last rows again, not stored
-    T.wp[i] = w + (size_t)n * a.kb * BLK;
-    if (i % 2 == 0) T.sp[i / 2] = s + (size_t)(n / BLK) * a.kb;
+    W.wp[i] = w + (size_t)n * a.kb * BLK;
+    if (i % 2 == 0) W.sp[i / 2] = s + (size_t)(n / BLK) * a.kb;
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < W.XD; ++h) {
     const int r = lane / 4;  // 16 rows x 64 bytes a DMA; the 16-byte pieces are swapped by row so that a
                              // fragment's reads (16 rows, one piece) meet every bank once
-    const int64_t m = first + min((2 * T.wave + h) * 16 + r, count - 1);
-    T.xp[h] = a.xq + (size_t)(MODE == UP ? a.token[m] : m) * a.kb * BLK + (((lane % 4) ^ (r >> 2)) * 16);
+    const int64_t m = first + min((W.XD * W.wave + h) * 16 + r, count - 1);
+    W.xp[h] = a.xq + (size_t)(MODE == UP ? a.token[m] : m) * a.kb * BLK + (((lane % 4) ^ (r >> 2)) * 16);
   }
   {
-    const int64_t m = first + min((T.wave * WAVE + lane) % BM, count - 1);
-    T.xsp = a.xs + (MODE == UP ? a.token[m] : m);
+    const int64_t m = first + min((W.wave * WAVE + lane) % BM, count - 1);
+    W.xsp = a.xs + (MODE == UP ? a.token[m] : m);
   }
-  T.run(s0, s1);
+  if constexpr (MT == 4)
+    W.run(s0, s1, s2);
+  else
+    W.run(s0, s1);
 
   const int g = lane / 16;
   if (MODE == UP) {
@@ -201,18 +253,18 @@ __global__ __launch_bounds__(WM * WN * WAVE, MODE == DENSE_F32 ? 1 : 2) void k_w
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float gate = T.acc[i][j][e];
-          T.acc[i][j][e] = gate / (1.0f + expf(-gate)) * T.acc[i + 2][j][e];
-          m = max(m, abs_bits(T.acc[i][j][e]));
+          const float gate = W.acc[i][j][e];
+          W.acc[i][j][e] = gate / (1.0f + expf(-gate)) * W.acc[i + 2][j][e];
+          m = max(m, abs_bits(W.acc[i][j][e]));
         }
       m = max(m, (uint32_t)__shfl_xor((int)m, 16, WAVE));
       m = max(m, (uint32_t)__shfl_xor((int)m, 32, WAVE));
-      if (g == 0) top[wn][wm * TM + 16 * j + lane] = m;
+      if (g == 0) top[wn][16 * j + lane] = m;
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
-      const int m = wm * TM + 16 * j + lane % 16;
+      const int m = 16 * j + lane % 16;
       uint32_t t = top[0][m];
 #pragma unroll
       for (int v = 1; v < WN; ++v) t = max(t, top[v][m]);
@@ -222,17 +274,17 @@ __global__ __launch_bounds__(WM * WN * WAVE, MODE == DENSE_F32 ? 1 : 2) void k_w
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         *reinterpret_cast<uint32_t*>(q + row[i] + 4 * g) =
-            fp8x4_pack(to_code_range(T.acc[i][j][0], bs), to_code_range(T.acc[i][j][1], bs),
-                       to_code_range(T.acc[i][j][2], bs), to_code_range(T.acc[i][j][3], bs));
+            fp8x4_pack(to_code_range(W.acc[i][j][0], bs), to_code_range(W.acc[i][j][1], bs),
+                       to_code_range(W.acc[i][j][2], bs), to_code_range(W.acc[i][j][3], bs));
       if (wn == 0 && g == 0) a.mid_s[(size_t)tn * a.mid_ld + first + m] = bs.scale;
     }
     return;
   }
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
-    const int m = wm * TM + 16 * j + lane % 16;
+    const int m = 16 * j + lane % 16;
     if (MODE == DOWN) {
-      const f32x4 y[NT] = {T.acc[0][j], T.acc[1][j], T.acc[2][j], T.acc[3][j]};
+      const f32x4 y[NT] = {W.acc[0][j], W.acc[1][j], W.acc[2][j], W.acc[3][j]};
       store_part(a.part, first + m, row[0], y, m < count && row[0] < a.n);
       continue;
     }
@@ -241,7 +293,7 @@ __global__ __launch_bounds__(WM * WN * WAVE, MODE == DENSE_F32 ? 1 : 2) void k_w
     for (int i = 0; i < NT; ++i) {
       if (row[i] >= a.n) continue;
       const size_t at = (size_t)(first + m) * a.out_ld + row[i] + 4 * g;
-      const f32x4 y = T.acc[i][j];
+      const f32x4 y = W.acc[i][j];
       if (MODE == DENSE_BF16)
         *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
       else
@@ -250,10 +302,11 @@ __global__ __launch_bounds__(WM * WN * WAVE, MODE == DENSE_F32 ? 1 : 2) void k_w
   }
 }
 
-template <int MODE, int WM>
-hipError_t launch(const Wide& a, int64_t tiles, hipStream_t st) {
-  const uint32_t grid = (uint32_t)((tiles + 7) / 8 * 8);
-  k_wide<MODE, WM><<<grid, WM * WN * WAVE, 0, st>>>(a);
+template <int MODE, int MT>
+hipError_t launch(Wide a, int64_t rows, hipStream_t st) {
+  if (rows) a.tiles_m = (int)((rows + 16 * MT - 1) / (16 * MT));
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+  k_wide<MODE, MT><<<(uint32_t)((tiles + 7) / 8 * 8), T, 0, st>>>(a);
   return hipGetLastError();
 }
 
@@ -263,12 +316,9 @@ hipError_t wide_product(const Rows& x, int64_t rows, const void* w, const float*
                         int64_t out_stride, hipStream_t st) {
   Wide a{x.q, x.s, x.ld, static_cast<const uint8_t*>(w), s, n, k / BLK, rows, out, out_stride};
   a.tiles_n = (n + BN - 1) / BN;
-  const bool two = !f32 && rows > 4 * TM;
-  const int bm = two ? 2 * TM : TM;
-  a.tiles_m = (int)((rows + bm - 1) / bm);
-  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
-  if (f32) return launch<DENSE_F32, 1>(a, tiles, st);
-  return two ? launch<DENSE_BF16, 2>(a, tiles, st) : launch<DENSE_BF16, 1>(a, tiles, st);
+  const bool low = (rows + 127) / 128 * a.tiles_n < 256;
+  if (f32) return launch<DENSE_F32, 4>(a, rows, st);
+  return low ? launch<DENSE_BF16, 4>(a, rows, st) : launch<DENSE_BF16, 8>(a, rows, st);
 }
 
 hipError_t wide_experts_up(const Experts& e, hipStream_t st) {
@@ -276,7 +326,7 @@ hipError_t wide_experts_up(const Experts& e, hipStream_t st) {
          e.sorted.tiles, e.sorted.token, e.inter, e.mid_q.s, e.mid_q.ld};
   a.tiles_m = e.tiles;
   a.tiles_n = e.inter / BLK;
-  return launch<UP, 1>(a, (int64_t)e.tiles * a.tiles_n, st);
+  return e.bm == 64 ? launch<UP, 4>(a, 0, st) : launch<UP, 8>(a, 0, st);
 }
 
 hipError_t wide_experts_down(const Experts& e, hipStream_t st) {
@@ -285,7 +335,7 @@ hipError_t wide_experts_down(const Experts& e, hipStream_t st) {
   a.part = e.part;
   a.tiles_m = e.tiles;
   a.tiles_n = (e.hidden + BN - 1) / BN;
-  return launch<DOWN, 1>(a, (int64_t)e.tiles * a.tiles_n, st);
+  return e.bm == 64 ? launch<DOWN, 4>(a, 0, st) : launch<DOWN, 8>(a, 0, st);
 }
 
 }  // namespace prompt
