@@ -99,7 +99,7 @@ size_t experts_plan(const mono_prompt_experts_args& a, void* ws, Experts& e) {
   Space sp{static_cast<char*>(ws)};
   const int64_t picks = a.tokens * a.picks, places = picks + (a.shared ? a.tokens : 0);
   e.wide = picks > WIDE_PICKS * a.experts;
-  e.bm = picks > 96 * (int64_t)a.experts ? 128 : 64;
+  e.bm = e.wide ? 128 : 64;
   e.tiles = (int)all_tiles(a.tokens, picks, a.experts, e.bm, a.shared);
   e.x = sp.rows(a.tokens, a.hidden);
   e.mid_q = sp.rows(places, a.inter);

@@ -72,29 +72,37 @@ struct WideTile {
     float s[2];
   };
 
-  MONO_DEV void issue(int kb, Stage<MT>& st, Ahead& n) {
+  // The loads of block kb in the order they go out: part 0 the rows' DMA and the scales, part
+  // 1 + i weight tile i.
+  MONO_DEV void issue(int kb, Stage<MT>& st, Ahead& n, int part) {
+    if (part == 0) {
 #pragma unroll
-    for (int h = 0; h < XD; ++h)
+      for (int h = 0; h < XD; ++h)
 #pragma unroll
-      for (int q = 0; q < 2; ++q) dma16(xp[h] + (size_t)kb * BLK + 64 * q, &st.x[(XD * wave + h) * 2048 + 1024 * q]);
-    if (MT == 4)
-      dma4(xsp + (size_t)kb * a.xs_ld, st.s[wave]);
-    else if (wave < MT / 4)
-      dma4(xsp + (size_t)kb * a.xs_ld, &st.s[0][wave * WAVE]);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const uint8_t* at = wp[i] + (size_t)kb * 2048;
+        for (int q = 0; q < 2; ++q) dma16(xp[h] + (size_t)kb * BLK + 64 * q, &st.x[(XD * wave + h) * 2048 + 1024 * q]);
+      if (MT == 4)
+        dma4(xsp + (size_t)kb * a.xs_ld, st.s[wave]);
+      else if (wave < MT / 4)
+        dma4(xsp + (size_t)kb * a.xs_ld, &st.s[0][wave * WAVE]);
+      n.s[0] = ld_const_f32(sp[0] + kb);
+      n.s[1] = ld_const_f32(sp[1] + kb);
+    } else if (part <= NT) {
+      const uint8_t* at = wp[part - 1] + (size_t)kb * 2048;
       const i32x4 lo = *reinterpret_cast<const i32x4*>(at + 16 * (uint32_t)lane);
       const i32x4 hi = *reinterpret_cast<const i32x4*>(at + 16 * (uint32_t)lane + 1024);
-      n.w[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      n.w[part - 1] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
-    n.s[0] = ld_const_f32(sp[0] + kb);
-    n.s[1] = ld_const_f32(sp[1] + kb);
+  }
+  MONO_DEV void issue(int kb, Stage<MT>& st, Ahead& n) {
+#pragma unroll
+    for (int part = 0; part <= NT; ++part) issue(kb, st, n, part);
   }
 
-  MONO_DEV void compute(const Stage<MT>& st, const Ahead& n) {
+  // One block's MFMAs, with `ahead(part)` (the loads of a later block) spread among them.
+  template <class F>
+  MONO_DEV void compute(const Stage<MT>& st, const Ahead& n, F ahead) {
     const int r = lane % 16, g = lane / 16;
-    const uint8_t* x = st.x + r * 64 + ((g ^ (r >> 2)) * 16);
+    const uint8_t* x = st.x + r * 64 + ((g ^ (r >> 1 & 3)) * 16);
     const float* xs = st.s[MT == 4 ? wave : 0] + r;
     i32x8 xv[2];  // a fragment ahead: its LDS latency lies under the MFMAs of the one before
     float sx[2];
@@ -123,8 +131,12 @@ struct WideTile {
         // the sums stay here: moved behind the next barrier, they would hold 64 more registers
         asm volatile("" : "+v"(to));
       }
+      if (t % 2 == 0 && t / 2 <= NT) ahead(t / 2);
       __builtin_amdgcn_sched_barrier(0);
     }
+  }
+  MONO_DEV void compute(const Stage<MT>& st, const Ahead& n) {
+    compute(st, n, [](int) {});
   }
 
   // The wave's loads but the last `LEFT` have come, and every wave's: a stage is whole.
@@ -143,11 +155,9 @@ struct WideTile {
     int kb = 0;
     for (; kb + 1 < a.kb; kb += 2) {
       arrive<0>();
-      issue(kb + 1, s1, a1);
-      compute(s0, a0);
+      compute(s0, a0, [&](int part) { issue(kb + 1, s1, a1, part); });
       arrive<0>();
-      issue(min(kb + 2, a.kb - 1), s0, a0);
-      compute(s1, a1);
+      compute(s1, a1, [&](int part) { issue(min(kb + 2, a.kb - 1), s0, a0, part); });
     }
     arrive<0>();
     if (kb < a.kb) compute(s0, a0);
@@ -163,14 +173,11 @@ struct WideTile {
     int kb = 0;
     for (; kb + 2 < a.kb; kb += 3) {
       arrive<EACH>();
-      issue(min(kb + 2, last), s2, a2);
-      compute(s0, a0);
+      compute(s0, a0, [&](int part) { issue(min(kb + 2, last), s2, a2, part); });
       arrive<EACH>();
-      issue(min(kb + 3, last), s0, a0);
-      compute(s1, a1);
+      compute(s1, a1, [&](int part) { issue(min(kb + 3, last), s0, a0, part); });
       arrive<EACH>();
-      issue(min(kb + 4, last), s1, a1);
-      compute(s2, a2);
+      compute(s2, a2, [&](int part) { issue(min(kb + 4, last), s1, a1, part); });
     }
     arrive<0>();
     if (kb < a.kb) compute(s0, a0);
@@ -178,43 +185,19 @@ struct WideTile {
   }
 };
 
-template <int MODE, int MT>
-__global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
-  constexpr int BM = 16 * MT;
-  __shared__ Stage<MT> s0, s1;
-  __shared__ Stage<4> s2;
-  __shared__ uint32_t top[MODE == UP ? WN : 1][MODE == UP ? BM : 1];
-  // a block's XCD is its index modulo 8: each XCD takes neighbouring tiles, whose rows and
-  // weights its L2 then holds once for all
-  int tn, tm;
-  const int per = (gridDim.x + 7) / 8, b = (blockIdx.x % 8) * per + blockIdx.x / 8;
-  if (MODE == UP || MODE == DOWN) {
-    tn = b % a.tiles_n;
-    tm = b / a.tiles_n;
-    if (tm >= a.tiles_m) return;
-  } else {
-    constexpr int GM = 8;  // row tiles side by side
-    const int group = b / (GM * a.tiles_n), in = b % (GM * a.tiles_n), high = min(GM, a.tiles_m - group * GM);
-    if (high <= 0) return;
-    tm = group * GM + in % high;
-    tn = in / high;
-    if (tn >= a.tiles_n) return;
-  }
-  const uint8_t* w = a.w;
-  const float* s = a.s;
-  int64_t first = (int64_t)tm * BM;
-  int count;
-  if (MODE == UP || MODE == DOWN) {
-    const Tile t = a.tiles[tm];
-    first = t.first;
-    count = t.count;
-    if (count == 0) return;
-    w += (size_t)t.expert * a.n * a.kb * BLK;
-    s += (size_t)t.expert * ((a.n + BLK - 1) / BLK) * a.kb;
-  } else {
-    count = (int)min((int64_t)BM, a.rows - first);
-  }
+// Where a tile lies: its weight columns and scales, its rows of x.
+struct Place {
+  const uint8_t* w;
+  const float* s;
+  int64_t first;
+  int count, tn;
+};
 
+template <int MODE, int MT, class... Stages>
+MONO_DEV void tile(const Wide& a, const Place& at, uint32_t (*top)[128], Stages&... stages) {
+  constexpr int BM = 16 * MT;
+  const int64_t first = at.first;
+  const int count = at.count, tn = at.tn;
   WideTile<MODE, MT> W(a);
   const int lane = W.lane, wn = W.wave;
   // the wave's weight tiles: 64 neighbouring rows, or (up) 32 gate rows and their up rows
@@ -223,24 +206,21 @@ __global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
   for (int i = 0; i < NT; ++i) {
     row[i] = MODE == UP ? tn * (BN / 2) + wn * (TN / 2) + 16 * (i % 2) + (i / 2) * a.half : tn * BN + wn * TN + 16 * i;
     const int n = min(row[i], a.n - 16);  // past the matrix: its last rows again, not stored
-    W.wp[i] = w + (size_t)n * a.kb * BLK;
-    if (i % 2 == 0) W.sp[i / 2] = s + (size_t)(n / BLK) * a.kb;
+    W.wp[i] = at.w + (size_t)n * a.kb * BLK;
+    if (i % 2 == 0) W.sp[i / 2] = at.s + (size_t)(n / BLK) * a.kb;
   }
 #pragma unroll
   for (int h = 0; h < W.XD; ++h) {
     const int r = lane / 4;  // 16 rows x 64 bytes a DMA; the 16-byte pieces are swapped by row so that a
                              // fragment's reads (16 rows, one piece) meet every bank once
     const int64_t m = first + min((W.XD * W.wave + h) * 16 + r, count - 1);
-    W.xp[h] = a.xq + (size_t)(MODE == UP ? a.token[m] : m) * a.kb * BLK + (((lane % 4) ^ (r >> 2)) * 16);
+    W.xp[h] = a.xq + (size_t)(MODE == UP ? a.token[m] : m) * a.kb * BLK + (((lane % 4) ^ (r >> 1 & 3)) * 16);
   }
   {
     const int64_t m = first + min((W.wave * WAVE + lane) % BM, count - 1);
     W.xsp = a.xs + (MODE == UP ? a.token[m] : m);
   }
-  if constexpr (MT == 4)
-    W.run(s0, s1, s2);
-  else
-    W.run(s0, s1);
+  W.run(stages...);
 
   const int g = lane / 16;
   if (MODE == UP) {
@@ -292,14 +272,52 @@ __global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       if (row[i] >= a.n) continue;
-      const size_t at = (size_t)(first + m) * a.out_ld + row[i] + 4 * g;
+      const size_t to = (size_t)(first + m) * a.out_ld + row[i] + 4 * g;
       const f32x4 y = W.acc[i][j];
       if (MODE == DENSE_BF16)
-        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + to) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
       else
-        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = y;
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = y;
     }
   }
+}
+
+template <int MODE, int MT>
+__global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
+  // (objects of their own: the compiler then knows that a stage's reads need not wait for
+  // another's DMA)
+  __shared__ Stage<4> l0, l1, l2;
+  __shared__ Stage<8> h0, h1;
+  __shared__ uint32_t top[MODE == UP ? WN : 1][128];
+  // a block's XCD is its index modulo 8: each XCD takes neighbouring tiles, whose rows and
+  // weights its L2 then holds once for all
+  const int per = gridDim.x / 8, b = (blockIdx.x % 8) * per + blockIdx.x / 8;
+  Place at{a.w, a.s, 0, 0, 0};
+  if (MODE == UP || MODE == DOWN) {
+    const int tm = b / a.tiles_n;
+    if (tm >= a.tiles_m) return;
+    const Tile t = a.tiles[tm];
+    if (t.count == 0) return;
+    at.tn = b % a.tiles_n;
+    at.first = t.first;
+    at.count = t.count;
+    at.w += (size_t)t.expert * a.n * a.kb * BLK;
+    at.s += (size_t)t.expert * ((a.n + BLK - 1) / BLK) * a.kb;
+  } else {
+    constexpr int GM = 8;  // row tiles side by side
+    const int group = b / (GM * a.tiles_n), in = b % (GM * a.tiles_n), high = min(GM, a.tiles_m - group * GM);
+    if (high <= 0) return;
+    at.tn = in / high;
+    if (at.tn >= a.tiles_n) return;
+    at.first = (int64_t)(group * GM + in % high) * (16 * MT);
+    at.count = (int)min((int64_t)(16 * MT), a.rows - at.first);
+  }
+  if constexpr (MT == 4)
+    tile<MODE, 4>(a, at, top, l0, l1, l2);
+  else if ((MODE == UP || MODE == DOWN) && at.count <= 64)
+    tile<MODE, 4>(a, at, top, l0, l1, l2);
+  else
+    tile<MODE, 8>(a, at, top, h0, h1);
 }
 
 template <int MODE, int MT>
@@ -326,7 +344,7 @@ hipError_t wide_experts_up(const Experts& e, hipStream_t st) {
          e.sorted.tiles, e.sorted.token, e.inter, e.mid_q.s, e.mid_q.ld};
   a.tiles_m = e.tiles;
   a.tiles_n = e.inter / BLK;
-  return e.bm == 64 ? launch<UP, 4>(a, 0, st) : launch<UP, 8>(a, 0, st);
+  return launch<UP, 8>(a, 0, st);
 }
 
 hipError_t wide_experts_down(const Experts& e, hipStream_t st) {
@@ -335,7 +353,7 @@ hipError_t wide_experts_down(const Experts& e, hipStream_t st) {
   a.part = e.part;
   a.tiles_m = e.tiles;
   a.tiles_n = (e.hidden + BN - 1) / BN;
-  return e.bm == 64 ? launch<DOWN, 4>(a, 0, st) : launch<DOWN, 8>(a, 0, st);
+  return launch<DOWN, 8>(a, 0, st);
 }
 
 }  // namespace prompt
