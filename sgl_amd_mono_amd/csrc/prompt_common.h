@@ -117,9 +117,9 @@ MONO_DEV uint32_t pack_halves(float a, float b) {
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
 }
 
-// Store one place's share of a wave's 16 x NT tiles x MT: lane l holds columns 16 i + 4 (l /
-// 16) .. + 3 of 64 (NT = 4), the four lane groups together a block of Parts.
-MONO_DEV void store_part(const Parts& p, int64_t place, int col, const f32x4 (&y)[4], bool in) {
+// A lane's 16 of one place's 64 columns (tiles of 16 weight rows i, columns 16 i + 4 g + e of
+// lane group g) as halves of a Parts block: the scale, and the values divided by it.
+MONO_DEV float part_block(const f32x4 (&y)[4], u32x2 (&h)[4]) {
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -130,13 +130,37 @@ MONO_DEV void store_part(const Parts& p, int64_t place, int col, const f32x4 (&y
   // 2^14 / 2^floor(log2 max); a block that is not finite keeps its values as they are
   const int e = m < 0x7f800000u ? max((int)(m >> 23), 27) : 127 + 14;
   const float inv = __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
-  if (!in) return;
-  const int g = lane_id() / 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = u32x2{pack_halves(y[i][0] * inv, y[i][1] * inv), pack_halves(y[i][2] * inv, y[i][3] * inv)};
+  return __uint_as_float((uint32_t)(e - 14) << 23);
+}
+
+// 16 rows of 64 two-byte values as the MFMA leaves them (lane r + 16 g: columns 16 i + 4 g ..
+// + 3 of row r) stored as whole 128-byte rows, through 2 KB of LDS that are the wave's own:
+// straight from the lanes a store would touch 32 bytes of each of 16 rows. `store(row,
+// column, 16 bytes)`; the 16-byte pieces are swapped by row, so neither side meets a bank twice.
+template <class F>
+MONO_DEV void store_rows(uint8_t* buf, const u32x2 (&h)[4], F store) {
+  const int lane = lane_id(), r = lane % 16, g = lane / 16;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    *reinterpret_cast<u32x2*>(p.v + place * p.ld + col + 16 * i + 4 * g) =
-        u32x2{pack_halves(y[i][0] * inv, y[i][1] * inv), pack_halves(y[i][2] * inv, y[i][3] * inv)};
-  if (g == 0) p.s[place * (p.ld / PART) + col / PART] = __uint_as_float((uint32_t)(e - 14) << 23);
+    *reinterpret_cast<u32x2*>(buf + r * 128 + (((2 * i + g / 2) ^ (r & 7)) * 16) + (g & 1) * 8) = h[i];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int row = lane / 8 + 8 * k, unit = lane % 8;
+    store(row, 8 * unit, *reinterpret_cast<const u32x4*>(buf + row * 128 + ((unit ^ (row & 7)) * 16)));
+  }
+}
+
+// One place's row of a wave's 64 columns into Parts (16 places a call, place `first` + r).
+MONO_DEV void store_part(uint8_t* buf, const Parts& p, int64_t first, int count, int col, const f32x4 (&y)[4]) {
+  u32x2 h[4];
+  const float s = part_block(y, h);
+  const int lane = lane_id();
+  if (lane < 16 && lane < count) p.s[(first + lane) * (p.ld / PART) + col / PART] = s;
+  store_rows(buf, h, [&](int row, int c, u32x4 v) {
+    if (row < count) *reinterpret_cast<u32x4*>(p.v + (first + row) * p.ld + col + c) = v;
+  });
 }
 
 }  // namespace prompt

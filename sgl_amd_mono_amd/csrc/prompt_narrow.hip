@@ -148,7 +148,7 @@ constexpr int DT = 256, DN = 256, DW = DN / (DT / WAVE) / 16;
 static_assert(16 * DW == PART, "a wave's weight rows are a block of Parts");
 
 template <int MT>
-MONO_DEV void down_tile(const Experts& a, const Tile& t, int n0) {
+MONO_DEV void down_tile(const Experts& a, const Tile& t, int n0, uint8_t* buf) {
   constexpr int U = MT == 1 ? 4 : MT == 2 ? 2 : 1;
   const int lane = threadIdx.x % WAVE, kb = a.inter / BLK;
   const uint8_t* w = a.w2 + ((size_t)t.expert * a.hidden + n0) * a.inter;
@@ -190,21 +190,22 @@ MONO_DEV void down_tile(const Experts& a, const Tile& t, int n0) {
   }
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
-    const int m = 16 * j + lane % 16;
-    store_part(a.part, t.first + m, n0, acc[j], m < t.count);
+    store_part(buf, a.part, t.first + 16 * j, t.count - 16 * j, n0, acc[j]);
   }
 }
 
 __global__ __launch_bounds__(DT) void k_down(Experts a) {
+  __shared__ uint8_t bufs[DT / WAVE][2048];
+  uint8_t* buf = bufs[threadIdx.x / WAVE];
   const Tile t = a.sorted.tiles[blockIdx.y];
   const int n0 = blockIdx.x * DN + threadIdx.x / WAVE * PART;
   if (t.count == 0 || n0 >= a.hidden) return;
   if (t.count <= 16)
-    down_tile<1>(a, t, n0);
+    down_tile<1>(a, t, n0, buf);
   else if (t.count <= 32)
-    down_tile<2>(a, t, n0);
+    down_tile<2>(a, t, n0, buf);
   else
-    down_tile<4>(a, t, n0);
+    down_tile<4>(a, t, n0, buf);
 }
 
 }  // namespace

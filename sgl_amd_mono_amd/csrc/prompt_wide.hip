@@ -34,6 +34,7 @@ struct Wide {
   int mid_ld;
   Parts part;          // down
   int tiles_m, tiles_n;
+  int groups;          // resident down: workgroups that share out a tile's weight columns
 };
 
 enum Mode { DENSE_BF16, DENSE_F32, UP, DOWN };
@@ -99,7 +100,8 @@ struct WideTile {
   }
 
   // One block's MFMAs, with `ahead(part)` (the loads of a later block) spread among them.
-  template <class F>
+  // FIRST: the sums begin with this block's.
+  template <bool FIRST = false, class F>
   MONO_DEV void compute(const Stage<MT>& st, const Ahead& n, F ahead) {
     const int r = lane % 16, g = lane / 16;
     const uint8_t* x = st.x + r * 64 + ((g ^ (r >> 1 & 3)) * 16);
@@ -112,22 +114,26 @@ struct WideTile {
       sx[j % 2] = xs[16 * j];
     };
     load(0);
-    // each MFMA ahead of the FMAs of the one before it: neither waits for the other
-    f32x4 p[2];
+    // each MFMA's partial is scaled while the two after it run: neither waits for the other
+    constexpr int LAG = MT == 4 ? 2 : 1;  // (128 rows have no registers for two)
+    f32x4 p[LAG + 1];
     float c[2][2];
 #pragma unroll
-    for (int t = 0; t <= MT * NT; ++t) {
-      const int i = t % NT, j = t / NT, v = t - 1;
+    for (int t = 0; t < MT * NT + LAG; ++t) {
+      const int i = t % NT, j = t / NT, v = t - LAG;
       if (t < MT * NT) {
         if (i == 0 && j + 1 < MT) load(j + 1);
-        p[t % 2] = mfma_block<MODE == DENSE_F32>(n.w[i], xv[j % 2]);
+        p[t % (LAG + 1)] = mfma_block<MODE == DENSE_F32>(n.w[i], xv[j % 2]);
         if (i == 0) c[j % 2][0] = sx[j % 2] * n.s[0], c[j % 2][1] = sx[j % 2] * n.s[1];
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (t > 0) {
+      if (v >= 0) {
         f32x4& to = acc[v % NT][v / NT];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) to[e] = fmaf(p[v % 2][e], c[v / NT % 2][v % NT / 2], to[e]);
+        for (int e = 0; e < 4; ++e) {
+          const float f = c[v / NT % 2][v % NT / 2];
+          to[e] = FIRST ? p[v % (LAG + 1)][e] * f : fmaf(p[v % (LAG + 1)][e], f, to[e]);
+        }
         // the sums stay here: moved behind the next barrier, they would hold 64 more registers
         asm volatile("" : "+v"(to));
       }
@@ -194,7 +200,7 @@ struct Place {
 };
 
 template <int MODE, int MT, class... Stages>
-MONO_DEV void tile(const Wide& a, const Place& at, uint32_t (*top)[128], Stages&... stages) {
+MONO_DEV void tile(const Wide& a, const Place& at, uint32_t (*top)[128], uint8_t* buf, Stages&... stages) {
   constexpr int BM = 16 * MT;
   const int64_t first = at.first;
   const int count = at.count, tn = at.tn;
@@ -262,24 +268,95 @@ MONO_DEV void tile(const Wide& a, const Place& at, uint32_t (*top)[128], Stages&
   }
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
-    const int m = 16 * j + lane % 16;
+    const f32x4 y[NT] = {W.acc[0][j], W.acc[1][j], W.acc[2][j], W.acc[3][j]};
     if (MODE == DOWN) {
-      const f32x4 y[NT] = {W.acc[0][j], W.acc[1][j], W.acc[2][j], W.acc[3][j]};
-      store_part(a.part, first + m, row[0], y, m < count && row[0] < a.n);
-      continue;
-    }
-    if (m >= count) continue;
+      if (row[0] < a.n) store_part(buf, a.part, first + 16 * j, count - 16 * j, row[0], y);
+    } else if (MODE == DENSE_BF16) {
+      u32x2 h[NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      if (row[i] >= a.n) continue;
-      const size_t to = (size_t)(first + m) * a.out_ld + row[i] + 4 * g;
-      const f32x4 y = W.acc[i][j];
-      if (MODE == DENSE_BF16)
-        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + to) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-      else
-        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = y;
+      for (int i = 0; i < NT; ++i) h[i] = u32x2{pack_bf16x2(y[i][0], y[i][1]), pack_bf16x2(y[i][2], y[i][3])};
+      store_rows(buf, h, [&](int r, int c, u32x4 v) {
+        if (16 * j + r < count && row[0] + c < a.n)
+          *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + (first + 16 * j + r) * a.out_ld + row[0] + c) = v;
+      });
+    } else if (16 * j + lane % 16 < count) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        if (row[i] < a.n)
+          *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + (first + 16 * j + lane % 16) * a.out_ld + row[i] + 4 * g) = y[i];
     }
   }
+}
+
+// The experts' down products where K is short (a few blocks of mids): the tile's rows stay in
+// LDS whole and each wave goes through its weight columns, 64 at a time, without a barrier;
+// the next weights are on their way at every moment, also while sums are stored.
+template <int KB, int MT>
+MONO_DEV void resident_tile(const Wide& a, const Place& at, int group, uint8_t* buf, Stage<MT> (&st)[KB]) {
+  WideTile<DOWN, MT> W(a);
+  const int lane = W.lane, r = lane / 4, last = a.kb - 1;
+  using Ahead = typename WideTile<DOWN, MT>::Ahead;
+#pragma unroll
+  for (int h = 0; h < W.XD; ++h)
+    W.xp[h] = a.xq + (size_t)(at.first + min((W.XD * W.wave + h) * 16 + r, at.count - 1)) * a.kb * BLK +
+              (((lane % 4) ^ (r >> 1 & 3)) * 16);
+  W.xsp = a.xs + at.first + min((W.wave * WAVE + lane) % (16 * MT), at.count - 1);
+  W.sp[0] = W.sp[1] = at.s;
+  Ahead n[2];
+  // block kb of the 64 columns from col on; past K's end (an odd number of blocks) the last one, scaled by zero
+  const auto weights = [&](int col, int kb, Ahead& to, int part) {
+    const int c = min(col, a.n - PART), b = min(kb, last);
+    if (part == 0) {
+      const float v = ld_const_f32(at.s + (size_t)(c / BLK) * a.kb + b);
+      to.s[0] = to.s[1] = kb <= last ? v : 0.f;
+    } else if (part <= NT) {
+      const uint8_t* p = at.w + (size_t)(c + 16 * (part - 1)) * a.kb * BLK + (size_t)b * 2048;
+      const i32x4 lo = *reinterpret_cast<const i32x4*>(p + 16 * (uint32_t)lane);
+      const i32x4 hi = *reinterpret_cast<const i32x4*>(p + 16 * (uint32_t)lane + 1024);
+      to.w[part - 1] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  };
+  int col = group * BN + W.wave * TN;
+  const int step = a.groups * BN;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) W.issue(min(kb, last), st[kb], n[0], 0);
+#pragma unroll
+  for (int part = 0; part <= NT; ++part) weights(col, 0, n[0], part);
+  W.template arrive<0>();
+  for (; col < a.n; col += step) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const auto ahead = [&](int part) {
+        weights(kb + 1 < KB ? col : col + step, kb + 1 < KB ? kb + 1 : 0, n[(kb + 1) % 2], part);
+      };
+      if (kb == 0)
+        W.template compute<true>(st[kb], n[kb % 2], ahead);
+      else
+        W.compute(st[kb], n[kb % 2], ahead);
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      const f32x4 y[NT] = {W.acc[0][j], W.acc[1][j], W.acc[2][j], W.acc[3][j]};
+      store_part(buf, a.part, at.first + 16 * j, at.count - 16 * j, col, y);
+    }
+  }
+}
+
+template <int KB>
+__global__ __launch_bounds__(T, 2) void k_down_resident(Wide a) {
+  static_assert(KB % 2 == 0, "the weights' two register sets alternate");
+  __shared__ Stage<8> st[KB];
+  __shared__ uint8_t bufs[WN][2048];
+  const int per = gridDim.x / 8, b = (blockIdx.x % 8) * per + blockIdx.x / 8, tm = b / a.groups;
+  if (tm >= a.tiles_m) return;
+  const Tile t = a.tiles[tm];
+  if (t.count == 0) return;
+  const Place at{a.w + (size_t)t.expert * a.n * a.kb * BLK, a.s + (size_t)t.expert * (a.n / BLK) * a.kb, t.first, t.count, 0};
+  uint8_t* buf = bufs[threadIdx.x / WAVE];
+  if (t.count <= 64)
+    resident_tile<KB, 4>(a, at, b % a.groups, buf, reinterpret_cast<Stage<4>(&)[KB]>(st));
+  else
+    resident_tile<KB, 8>(a, at, b % a.groups, buf, st);
 }
 
 template <int MODE, int MT>
@@ -289,6 +366,8 @@ __global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
   __shared__ Stage<4> l0, l1, l2;
   __shared__ Stage<8> h0, h1;
   __shared__ uint32_t top[MODE == UP ? WN : 1][128];
+  __shared__ uint8_t bufs[MODE == UP || MODE == DENSE_F32 ? 1 : WN][2048];
+  uint8_t* buf = bufs[MODE == UP || MODE == DENSE_F32 ? 0 : threadIdx.x / WAVE];
   // a block's XCD is its index modulo 8: each XCD takes neighbouring tiles, whose rows and
   // weights its L2 then holds once for all
   const int per = gridDim.x / 8, b = (blockIdx.x % 8) * per + blockIdx.x / 8;
@@ -313,11 +392,11 @@ __global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
     at.count = (int)min((int64_t)(16 * MT), a.rows - at.first);
   }
   if constexpr (MT == 4)
-    tile<MODE, 4>(a, at, top, l0, l1, l2);
+    tile<MODE, 4>(a, at, top, buf, l0, l1, l2);
   else if ((MODE == UP || MODE == DOWN) && at.count <= 64)
-    tile<MODE, 4>(a, at, top, l0, l1, l2);
+    tile<MODE, 4>(a, at, top, buf, l0, l1, l2);
   else
-    tile<MODE, 8>(a, at, top, h0, h1);
+    tile<MODE, 8>(a, at, top, buf, h0, h1);
 }
 
 template <int MODE, int MT>
@@ -353,7 +432,14 @@ hipError_t wide_experts_down(const Experts& e, hipStream_t st) {
   a.part = e.part;
   a.tiles_m = e.tiles;
   a.tiles_n = (e.hidden + BN - 1) / BN;
-  return launch<DOWN, 8>(a, 0, st);
+  if (a.kb > 4) return launch<DOWN, 8>(a, 0, st);
+  a.groups = min(a.tiles_n, 4);
+  const uint32_t grid = (uint32_t)(((int64_t)a.tiles_m * a.groups + 7) / 8 * 8);
+  if (a.kb > 2)
+    k_down_resident<4><<<grid, T, 0, st>>>(a);
+  else
+    k_down_resident<2><<<grid, T, 0, st>>>(a);
+  return hipGetLastError();
 }
 
 }  // namespace prompt
