@@ -498,7 +498,7 @@ typedef struct {
   int64_t workspace_bytes;
 } mono_prompt_product_args;
 
-/* Bytes of workspace of a product (-1: refused, see mono_last_error). */
+/* Bytes of workspace of a product (0: none; -1: refused, see mono_last_error). */
 int64_t mono_prompt_product_workspace(int64_t rows, int32_t n, int32_t k);
 int mono_prompt_product(const mono_prompt_product_args* args, void* stream);
 
@@ -514,7 +514,7 @@ typedef struct {
   const void* kv_a;          /* bf16 or f32 [tokens, 576] latent 512 | k_pe 64, before norm and RoPE */
   int64_t kv_stride;         /* elements from a row to the next; rows 16-byte aligned */
   const void* ik;            /* bf16 or f32 [tokens, 128] index key, before norm and RoPE */
-  int64_t ik_stride;         /* even; ik itself 8-byte aligned */
+  int64_t ik_stride;         /* as kv_stride */
   int32_t f32;               /* kv_a and ik: 0 bf16, 1 f32 */
   int64_t tokens;            /* 0..1048576 */
   const int32_t* req;        /* [tokens] row of page_table */
@@ -522,7 +522,7 @@ typedef struct {
   const int32_t* page_table; /* [requests, pt_stride] */
   int32_t requests, pt_stride, n_pages, max_pos;
   const void* g_kv;          /* bf16 [512] */
-  const float* g_ik;         /* f32 [128] */
+  const float* g_ik;         /* f32 [128] (these four 16-byte aligned) */
   const float* b_ik;         /* f32 [128] */
   const float* rope_cos;     /* f32 [max_pos, 32] */
   const float* rope_sin;     /* f32 [max_pos, 32] */

@@ -78,6 +78,15 @@ int product_shape(int64_t rows, int32_t n, int32_t k) {
   return MONO_OK;
 }
 
+// A product's plan over its workspace: the rows' codes and scales, and its parts.
+size_t product_space(void* ws, Product& p) {
+  Space sp{static_cast<char*>(ws)};
+  p.plan = product_plan(p.rows, p.n, p.k);
+  if (p.plan.kind != ProductPlan::FEW) p.q = sp.rows(p.rows, p.k);
+  if (p.plan.splits > 1) p.part = sp.take<float>((size_t)p.plan.splits * p.rows * p.n);
+  return sp.off;
+}
+
 int experts_shape(const mono_prompt_experts_args& a) {
   if (int rc = need_rows(a.tokens, "tokens")) return rc;
   if (a.experts < 1 || a.experts > MAX_EXPERTS) return refuse("experts must be in [1, %d], got %d", MAX_EXPERTS, a.experts);
@@ -91,8 +100,8 @@ int experts_shape(const mono_prompt_experts_args& a) {
   return MONO_OK;
 }
 
-// Where the wide tiles take over: rows of a product, picks a routed expert gets on average.
-constexpr int WIDE_ROWS = 96, WIDE_PICKS = 24;
+// Where the wide tiles take over: picks a routed expert gets on average.
+constexpr int WIDE_PICKS = 24;
 
 // The call's plan over its workspace; `e.tiles` bounds the tile list.
 size_t experts_plan(const mono_prompt_experts_args& a, void* ws, Experts& e) {
@@ -131,10 +140,10 @@ size_t experts_plan(const mono_prompt_experts_args& a, void* ws, Experts& e) {
 
 extern "C" int64_t mono_prompt_product_workspace(int64_t rows, int32_t n, int32_t k) {
   if (product_shape(rows, n, k)) return -1;
-  Space sp{nullptr};
-  sp.rows(rows, k);
+  Product p{};
+  p.rows = rows, p.n = n, p.k = k;
   mono::abi_ok();
-  return (int64_t)sp.off;
+  return rows ? (int64_t)product_space(nullptr, p) : 0;
 }
 
 extern "C" int mono_prompt_product(const mono_prompt_product_args* args, void* stream) {
@@ -142,21 +151,22 @@ extern "C" int mono_prompt_product(const mono_prompt_product_args* args, void* s
   const mono_prompt_product_args& a = *args;
   if (int rc = product_shape(a.rows, a.n, a.k)) return rc;
   if (a.rows == 0) return mono::abi_ok();
-  const int64_t ws = mono_prompt_product_workspace(a.rows, a.n, a.k);
   if (int rc = need_stride(a.x_stride, a.k, 8, "x_stride")) return rc;
   if (int rc = need_stride(a.out_stride, a.n, 8, "out_stride")) return rc;
   if (int rc = need(a.x, "x", 16)) return rc;
   if (int rc = need(a.w, "w", 16)) return rc;
   if (int rc = need(a.s, "s", 4)) return rc;
   if (int rc = need(a.out, "out", 16)) return rc;
-  if (int rc = need_space(a.workspace, a.workspace_bytes, (size_t)ws)) return rc;
+  Product p{a.x, a.x_stride, {}, a.rows, static_cast<const uint8_t*>(a.w), a.s, a.n, a.k, a.out, a.out_stride, a.out_f32 != 0};
+  if (const size_t bytes = product_space(nullptr, p)) {
+    if (int rc = need_space(a.workspace, a.workspace_bytes, bytes)) return rc;
+    product_space(a.workspace, p);
+  }
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  Space sp{static_cast<char*>(a.workspace)};
-  const Rows x = sp.rows(a.rows, a.k);
-  if (hipError_t e = quant_rows(a.x, false, a.x_stride, a.rows, a.k, x, st)) return launched(e, "the rows' rounding");
-  if (a.rows > WIDE_ROWS)
-    return launched(wide_product(x, a.rows, a.w, a.s, a.n, a.k, a.out, a.out_f32 != 0, a.out_stride, st), "the product");
-  return launched(product(x, a.rows, a.w, a.s, a.n, a.k, a.out, a.out_f32 != 0, a.out_stride, st), "the product");
+  if (p.plan.kind == ProductPlan::FEW) return launched(few_product(p, st), "the product");
+  if (hipError_t e = quant_rows(p.x, false, p.x_stride, p.rows, p.k, p.q, st)) return launched(e, "the rows' rounding");
+  if (hipError_t e = p.plan.kind == ProductPlan::WIDE ? wide_product(p, st) : narrow_product(p, st)) return launched(e, "the product");
+  return launched(p.plan.splits > 1 ? join_product(p, st) : hipSuccess, "the sum of the product's parts");
 }
 
 extern "C" int mono_prompt_append(const mono_prompt_append_args* args, void* stream) {
@@ -169,17 +179,17 @@ extern "C" int mono_prompt_append(const mono_prompt_append_args* args, void* str
   if (a.tokens == 0 || a.requests == 0 || a.pt_stride == 0 || a.n_pages == 0 || a.max_pos == 0) return mono::abi_ok();
   const int each = a.f32 ? 4 : 8;  // a 16-byte load's elements
   if (int rc = need_stride(a.kv_stride, LATENT + PE, each, "kv_stride")) return rc;
-  if (int rc = need_stride(a.ik_stride, INDEX, 2, "ik_stride")) return rc;
+  if (int rc = need_stride(a.ik_stride, INDEX, each, "ik_stride")) return rc;
   if (int rc = need(a.kv_a, "kv_a", 16)) return rc;
-  if (int rc = need(a.ik, "ik", 8)) return rc;
+  if (int rc = need(a.ik, "ik", 16)) return rc;
   if (int rc = need(a.req, "req", 4)) return rc;
   if (int rc = need(a.pos, "pos", 4)) return rc;
   if (int rc = need(a.page_table, "page_table", 4)) return rc;
   if (int rc = need(a.g_kv, "g_kv", 16)) return rc;
-  if (int rc = need(a.g_ik, "g_ik", 8)) return rc;
-  if (int rc = need(a.b_ik, "b_ik", 8)) return rc;
-  if (int rc = need(a.rope_cos, "rope_cos", 4)) return rc;
-  if (int rc = need(a.rope_sin, "rope_sin", 4)) return rc;
+  if (int rc = need(a.g_ik, "g_ik", 16)) return rc;
+  if (int rc = need(a.b_ik, "b_ik", 16)) return rc;
+  if (int rc = need(a.rope_cos, "rope_cos", 16)) return rc;
+  if (int rc = need(a.rope_sin, "rope_sin", 16)) return rc;
   if (int rc = need(a.kv, "kv", 8)) return rc;
   if (a.kv_scale)
     if (int rc = need(a.kv_scale, "kv_scale", 4)) return rc;
@@ -219,7 +229,6 @@ extern "C" int mono_prompt_experts(const mono_prompt_experts_args* args, void* s
   if (int rc = need_space(a.workspace, a.workspace_bytes, experts_plan(a, nullptr, e))) return rc;
   experts_plan(a, a.workspace, e);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t places = e.picks + (e.shared ? e.tokens : 0);
   if (hipError_t r = sort_quant(a.x, a.x_stride, a.tokens, a.hidden, e.x, a.ids, a.picks, a.experts, e.shared, e.bm, e.sorted, st))
     return launched(r, "the tokens' sort");
   if (e.wide) {
@@ -227,7 +236,6 @@ extern "C" int mono_prompt_experts(const mono_prompt_experts_args* args, void* s
     if (hipError_t r = wide_experts_down(e, st)) return launched(r, "the experts' down products");
   } else {
     if (hipError_t r = experts_up(e, st)) return launched(r, "the experts' up products");
-    if (hipError_t r = quant_rows(e.mid, true, e.inter, places, e.inter, e.mid_q, st)) return launched(r, "the mids' rounding");
     if (hipError_t r = experts_down(e, st)) return launched(r, "the experts' down products");
   }
   return launched(experts_back(e, st), "the weighted sum");

@@ -59,13 +59,60 @@ struct Parts {
 hipError_t quant_rows(const void* x, bool f32, int64_t stride, int64_t rows, int k, const Rows& out, hipStream_t st);
 hipError_t sort_quant(const void* x, int64_t stride, int64_t tokens, int k, const Rows& out, const int* ids, int picks_each,
                       int experts, bool shared, int bm, const Sorted& sorted, hipStream_t st);
-hipError_t product(const Rows& x, int64_t rows, const void* w, const float* s, int n, int k, void* out, bool f32,
-                   int64_t out_stride, hipStream_t st);
+// How a product runs, by its sizes alone.
+//
+// FEW     at most 16 rows of FEW_BYTES codes: every workgroup rounds them for itself
+// NARROW  up to WIDE_ROWS rows: workgroups of 16 weight rows, 8 waves along K
+// WIDE    more: tiles of 256 weight rows x 64 or 128 rows, waves along the weight rows
+//
+// `splits` > 1: K is shared out over that many workgroups, whose f32 sums a second launch
+// adds in order. Where the tiles alone leave CUs without work, and each share keeps at
+// least 8 blocks of K.
+constexpr int FEW_BYTES = 32768;
+constexpr int WIDE_ROWS = 96;
+struct ProductPlan {
+  enum Kind { FEW, NARROW, WIDE } kind;
+  int splits;
+  int bm;  // rows of a tile
+};
+inline ProductPlan product_plan(int64_t rows, int n, int k) {
+  if (rows <= 16 && rows * k <= FEW_BYTES) return {ProductPlan::FEW, 1, 16};
+  const int kb = k / BLK;
+  constexpr int64_t FULL = 256;  // workgroups that leave no CU without one
+  int64_t tiles;
+  ProductPlan p;
+  if (rows <= WIDE_ROWS) {
+    p = {ProductPlan::NARROW, 1, 64};
+    tiles = n / 16 * ((rows + 63) / 64);
+  } else {
+    const int64_t wide = (n + 255) / 256;
+    p = {ProductPlan::WIDE, 1, (rows + 127) / 128 * wide < 256 ? 64 : 128};
+    tiles = (rows + p.bm - 1) / p.bm * wide;
+  }
+  const int64_t s = FULL / tiles < kb / 8 ? FULL / tiles : kb / 8;
+  if (p.bm == 64 && s > 1) p.splits = (int)s;
+  return p;
+}
 
-// Wide tiles (128 rows or more) where there are rows enough for them, narrow ones (64)
-// else.
-hipError_t wide_product(const Rows& x, int64_t rows, const void* w, const float* s, int n, int k, void* out, bool f32,
-                        int64_t out_stride, hipStream_t st);
+// A product's launch. part: f32 [splits, rows, n] where splits > 1.
+struct Product {
+  const void* x;
+  int64_t x_stride;
+  Rows q;  // the rows' codes (not FEW)
+  int64_t rows;
+  const uint8_t* w;
+  const float* s;
+  int n, k;
+  void* out;
+  int64_t out_stride;
+  bool f32;
+  float* part;
+  ProductPlan plan;
+};
+hipError_t few_product(const Product& a, hipStream_t st);
+hipError_t narrow_product(const Product& a, hipStream_t st);
+hipError_t wide_product(const Product& a, hipStream_t st);
+hipError_t join_product(const Product& a, hipStream_t st);
 
 struct Experts {
   Rows x, mid_q;

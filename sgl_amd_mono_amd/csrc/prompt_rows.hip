@@ -134,7 +134,30 @@ __global__ __launch_bounds__(128) void k_back(Experts a) {
       u32x4{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7])};
 }
 
+// The sums of a product whose K was shared out, in the shares' order. A thread adds 4 outputs.
+template <bool F32>
+__global__ __launch_bounds__(256) void k_join(const float* part, int splits, int64_t rows, int n, void* out, int64_t out_ld) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, each = n / 4;
+  if (i >= rows * each) return;
+  const int64_t row = i / each, c = 4 * (i % each);
+  f32x4 y = *reinterpret_cast<const f32x4*>(part + row * n + c);
+  for (int s = 1; s < splits; ++s) y += *reinterpret_cast<const f32x4*>(part + (s * rows + row) * n + c);
+  if (F32)
+    *reinterpret_cast<f32x4*>(static_cast<float*>(out) + row * out_ld + c) = y;
+  else
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + row * out_ld + c) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+}
+
 }  // namespace
+
+hipError_t join_product(const Product& a, hipStream_t st) {
+  const uint32_t grid = (uint32_t)((a.rows * (a.n / 4) + 255) / 256);
+  if (a.f32)
+    k_join<true><<<grid, 256, 0, st>>>(a.part, a.plan.splits, a.rows, a.n, a.out, a.out_stride);
+  else
+    k_join<false><<<grid, 256, 0, st>>>(a.part, a.plan.splits, a.rows, a.n, a.out, a.out_stride);
+  return hipGetLastError();
+}
 
 hipError_t quant_rows(const void* x, bool f32, int64_t stride, int64_t rows, int k, const Rows& out, hipStream_t st) {
   const uint32_t n = (uint32_t)(rows * (k / BLK)), grid = (n + T / 16 - 1) / (T / 16);

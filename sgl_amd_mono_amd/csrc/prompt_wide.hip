@@ -34,6 +34,8 @@ struct Wide {
   int mid_ld;
   Parts part;          // down
   int tiles_m, tiles_n;
+  float* split;        // dense, K shared out: f32 [splits, rows, n] instead of out
+  int splits;
   int groups;          // resident down: workgroups that share out a tile's weight columns
 };
 
@@ -60,13 +62,14 @@ struct WideTile {
   static constexpr int XD = MT / 4;  // groups of 16 rows of x that a wave brings
   const Wide& a;
   const int lane, wave;
+  int kb0 = 0, kbs;       // the tile's blocks of K: the first, how many
   const uint8_t* wp[NT];  // the weight tiles (uniform)
   const float* sp[2];     // scale rows: of weight tiles 0, 1 and 2, 3
   const uint8_t* xp[XD];  // the lane's rows of x for the DMA
   const float* xsp;       // the lane's row of the scales for the DMA
   f32x4 acc[NT][MT] = {};
 
-  MONO_DEV WideTile(const Wide& a_) : a(a_), lane(threadIdx.x % WAVE), wave(__builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)) {}
+  MONO_DEV WideTile(const Wide& a_) : a(a_), lane(threadIdx.x % WAVE), wave(__builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)), kbs(a_.kb) {}
 
   struct Ahead {
     i32x8 w[NT];
@@ -76,6 +79,7 @@ struct WideTile {
   // The loads of block kb in the order they go out: part 0 the rows' DMA and the scales, part
   // 1 + i weight tile i.
   MONO_DEV void issue(int kb, Stage<MT>& st, Ahead& n, int part) {
+    kb += kb0;
     if (part == 0) {
 #pragma unroll
       for (int h = 0; h < XD; ++h)
@@ -159,25 +163,25 @@ struct WideTile {
     Ahead a0, a1;
     issue(0, s0, a0);
     int kb = 0;
-    for (; kb + 1 < a.kb; kb += 2) {
+    for (; kb + 1 < kbs; kb += 2) {
       arrive<0>();
       compute(s0, a0, [&](int part) { issue(kb + 1, s1, a1, part); });
       arrive<0>();
-      compute(s1, a1, [&](int part) { issue(min(kb + 2, a.kb - 1), s0, a0, part); });
+      compute(s1, a1, [&](int part) { issue(min(kb + 2, kbs - 1), s0, a0, part); });
     }
     arrive<0>();
-    if (kb < a.kb) compute(s0, a0);
+    if (kb < kbs) compute(s0, a0);
   }
 
   // 64 rows: half the MFMA time a block to hide the same latency under, so two blocks ahead.
   MONO_DEV void run(Stage<MT>& s0, Stage<MT>& s1, Stage<MT>& s2) {
     constexpr int EACH = 2 * XD + 1 + 2 * NT;  // a stage's loads, the same for every wave
-    const int last = a.kb - 1;
+    const int last = kbs - 1;
     Ahead a0, a1, a2;
     issue(0, s0, a0);
     issue(min(1, last), s1, a1);
     int kb = 0;
-    for (; kb + 2 < a.kb; kb += 3) {
+    for (; kb + 2 < kbs; kb += 3) {
       arrive<EACH>();
       compute(s0, a0, [&](int part) { issue(min(kb + 2, last), s2, a2, part); });
       arrive<EACH>();
@@ -186,8 +190,8 @@ struct WideTile {
       compute(s2, a2, [&](int part) { issue(min(kb + 4, last), s1, a1, part); });
     }
     arrive<0>();
-    if (kb < a.kb) compute(s0, a0);
-    if (kb + 1 < a.kb) compute(s1, a1);
+    if (kb < kbs) compute(s0, a0);
+    if (kb + 1 < kbs) compute(s1, a1);
   }
 };
 
@@ -196,7 +200,7 @@ struct Place {
   const uint8_t* w;
   const float* s;
   int64_t first;
-  int count, tn;
+  int count, tn, split;
 };
 
 template <int MODE, int MT, class... Stages>
@@ -206,6 +210,10 @@ MONO_DEV void tile(const Wide& a, const Place& at, uint32_t (*top)[128], uint8_t
   const int count = at.count, tn = at.tn;
   WideTile<MODE, MT> W(a);
   const int lane = W.lane, wn = W.wave;
+  if (MODE != UP && MODE != DOWN && MT == 4) {
+    W.kb0 = at.split * a.kb / a.splits;
+    W.kbs = (at.split + 1) * a.kb / a.splits - W.kb0;
+  }
   // the wave's weight tiles: 64 neighbouring rows, or (up) 32 gate rows and their up rows
   int row[NT];
 #pragma unroll
@@ -271,6 +279,12 @@ MONO_DEV void tile(const Wide& a, const Place& at, uint32_t (*top)[128], uint8_t
     const f32x4 y[NT] = {W.acc[0][j], W.acc[1][j], W.acc[2][j], W.acc[3][j]};
     if (MODE == DOWN) {
       if (row[0] < a.n) store_part(buf, a.part, first + 16 * j, count - 16 * j, row[0], y);
+    } else if (MT == 4 && a.splits > 1) {
+      if (16 * j + lane % 16 < count)
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          if (row[i] < a.n)
+            *reinterpret_cast<f32x4*>(a.split + ((size_t)at.split * a.rows + first + 16 * j + lane % 16) * a.n + row[i] + 4 * g) = y[i];
     } else if (MODE == DENSE_BF16) {
       u32x2 h[NT];
 #pragma unroll
@@ -351,7 +365,7 @@ __global__ __launch_bounds__(T, 2) void k_down_resident(Wide a) {
   if (tm >= a.tiles_m) return;
   const Tile t = a.tiles[tm];
   if (t.count == 0) return;
-  const Place at{a.w + (size_t)t.expert * a.n * a.kb * BLK, a.s + (size_t)t.expert * (a.n / BLK) * a.kb, t.first, t.count, 0};
+  const Place at{a.w + (size_t)t.expert * a.n * a.kb * BLK, a.s + (size_t)t.expert * (a.n / BLK) * a.kb, t.first, t.count, 0, 0};
   uint8_t* buf = bufs[threadIdx.x / WAVE];
   if (t.count <= 64)
     resident_tile<KB, 4>(a, at, b % a.groups, buf, reinterpret_cast<Stage<4>(&)[KB]>(st));
@@ -370,8 +384,9 @@ __global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
   uint8_t* buf = bufs[MODE == UP || MODE == DENSE_F32 ? 0 : threadIdx.x / WAVE];
   // a block's XCD is its index modulo 8: each XCD takes neighbouring tiles, whose rows and
   // weights its L2 then holds once for all
-  const int per = gridDim.x / 8, b = (blockIdx.x % 8) * per + blockIdx.x / 8;
-  Place at{a.w, a.s, 0, 0, 0};
+  const int per = gridDim.x / 8;
+  int b = (blockIdx.x % 8) * per + blockIdx.x / 8;
+  Place at{a.w, a.s, 0, 0, 0, 0};
   if (MODE == UP || MODE == DOWN) {
     const int tm = b / a.tiles_n;
     if (tm >= a.tiles_m) return;
@@ -384,10 +399,12 @@ __global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
     at.s += (size_t)t.expert * ((a.n + BLK - 1) / BLK) * a.kb;
   } else {
     constexpr int GM = 8;  // row tiles side by side
+    const int tiles = a.tiles_m * a.tiles_n;
+    at.split = b / tiles;
+    if (at.split >= a.splits) return;
+    b -= at.split * tiles;
     const int group = b / (GM * a.tiles_n), in = b % (GM * a.tiles_n), high = min(GM, a.tiles_m - group * GM);
-    if (high <= 0) return;
     at.tn = in / high;
-    if (at.tn >= a.tiles_n) return;
     at.first = (int64_t)(group * GM + in % high) * (16 * MT);
     at.count = (int)min((int64_t)(16 * MT), a.rows - at.first);
   }
@@ -400,22 +417,23 @@ __global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
 }
 
 template <int MODE, int MT>
-hipError_t launch(Wide a, int64_t rows, hipStream_t st) {
-  if (rows) a.tiles_m = (int)((rows + 16 * MT - 1) / (16 * MT));
-  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+hipError_t launch(const Wide& a, int splits, hipStream_t st) {
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * splits;
   k_wide<MODE, MT><<<(uint32_t)((tiles + 7) / 8 * 8), T, 0, st>>>(a);
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t wide_product(const Rows& x, int64_t rows, const void* w, const float* s, int n, int k, void* out, bool f32,
-                        int64_t out_stride, hipStream_t st) {
-  Wide a{x.q, x.s, x.ld, static_cast<const uint8_t*>(w), s, n, k / BLK, rows, out, out_stride};
-  a.tiles_n = (n + BN - 1) / BN;
-  const bool low = (rows + 127) / 128 * a.tiles_n < 256;
-  if (f32) return launch<DENSE_F32, 4>(a, rows, st);
-  return low ? launch<DENSE_BF16, 4>(a, rows, st) : launch<DENSE_BF16, 8>(a, rows, st);
+hipError_t wide_product(const Product& p, hipStream_t st) {
+  Wide a{p.q.q, p.q.s, p.q.ld, p.w, p.s, p.n, p.k / BLK, p.rows, p.out, p.out_stride};
+  const bool low = p.f32 || p.plan.bm == 64;
+  a.tiles_n = (p.n + BN - 1) / BN;
+  a.tiles_m = (int)((p.rows + (low ? 63 : 127)) / (low ? 64 : 128));
+  a.split = p.part;
+  a.splits = p.plan.splits;
+  if (p.f32) return launch<DENSE_F32, 4>(a, a.splits, st);
+  return low ? launch<DENSE_BF16, 4>(a, a.splits, st) : launch<DENSE_BF16, 8>(a, 1, st);
 }
 
 hipError_t wide_experts_up(const Experts& e, hipStream_t st) {
@@ -423,7 +441,7 @@ hipError_t wide_experts_up(const Experts& e, hipStream_t st) {
          e.sorted.tiles, e.sorted.token, e.inter, e.mid_q.s, e.mid_q.ld};
   a.tiles_m = e.tiles;
   a.tiles_n = e.inter / BLK;
-  return launch<UP, 8>(a, 0, st);
+  return launch<UP, 8>(a, 1, st);
 }
 
 hipError_t wide_experts_down(const Experts& e, hipStream_t st) {
@@ -432,7 +450,7 @@ hipError_t wide_experts_down(const Experts& e, hipStream_t st) {
   a.part = e.part;
   a.tiles_m = e.tiles;
   a.tiles_n = (e.hidden + BN - 1) / BN;
-  if (a.kb > 4) return launch<DOWN, 8>(a, 0, st);
+  if (a.kb > 4) return launch<DOWN, 8>(a, 1, st);
   a.groups = min(a.tiles_n, 4);
   const uint32_t grid = (uint32_t)(((int64_t)a.tiles_m * a.groups + 7) / 8 * 8);
   if (a.kb > 2)

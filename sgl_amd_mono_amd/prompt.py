@@ -27,10 +27,16 @@ from .moe import FP8_TYPES
 from .runtime import need
 
 
+# The current stream's handle without a Stream object around it, which takes longer to make
+# than a short launch takes to enqueue.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _gpu(t: torch.Tensor, name: str) -> torch.device:
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name}: expected a tensor, got {type(t).__name__}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name}: expected a tensor on a GPU, got {t.device}")
     return t.device
 
@@ -41,29 +47,38 @@ def _rows(t: torch.Tensor, name: str, shape: tuple, dtype, dev: torch.device) ->
     there is no next)."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name}: expected a tensor, got {type(t).__name__}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
     if t.dtype != dtype:
         raise ValueError(f"{name}: expected dtype {dtype}, got {t.dtype}")
     if t.device != dev:
         raise ValueError(f"{name}: expected device {dev}, got {t.device}")
-    if shape[0] <= 1:
-        if shape[0] and t.stride(1) != 1:
+    rows, columns = shape
+    if rows <= 1:
+        if rows and columns > 1 and t.stride(1) != 1:
             raise ValueError(f"{name}: expected columns that lie together (strides {t.stride()})")
-        return -(-shape[1] // 8) * 8
-    if t.stride(1) != 1 or t.stride(0) < shape[1]:
-        raise ValueError(f"{name}: expected columns that lie together and rows apart (strides {t.stride()})")
-    return t.stride(0)
+        return -(-columns // 8) * 8
+    stride = t.stride()
+    if (stride[1] != 1 and columns > 1) or stride[0] < columns:
+        raise ValueError(f"{name}: expected columns that lie together and rows apart (strides {stride})")
+    return stride[0]
 
 
 def _enqueue(dev: torch.device, fn, args) -> None:
-    with torch.cuda.device(dev):
-        _lib.check(fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream))
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(C.byref(args), _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(C.byref(args), _raw_stream(dev.index))
+    if rc:
+        _lib.check(rc)
 
 
-def _workspace(args, nbytes: int, dev: torch.device) -> torch.Tensor:
+def _workspace(args, nbytes: int, dev: torch.device) -> torch.Tensor | None:
     if nbytes < 0:
         raise ValueError(_lib.lib().mono_last_error().decode(errors="replace"))
+    if nbytes == 0:
+        return None
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
     return ws

@@ -46,7 +46,10 @@ def _same(got, want, mag, f32, k):
 # ------------------------------------------------------------------- product
 @pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
 @pytest.mark.parametrize("m,n,k", [(1, 16, 128), (1, 2112, 7168), (3, 144, 384), (16, 128, 7168), (17, 272, 1024),
-                                   (63, 64, 256), (65, 2112, 512), (129, 400, 1152), (300, 1536, 640)])
+                                   (63, 64, 256), (65, 2112, 512), (129, 400, 1152), (300, 1536, 640),
+                                   # the borders of each way to run: few rows, K shared out, tiles of 64 and 128 rows
+                                   (16, 64, 2048), (17, 64, 2048), (16, 64, 2176), (4, 32, 8192), (5, 32, 8192), (45, 144, 7168),
+                                   (96, 16, 4096), (97, 16, 4096), (300, 528, 4096), (2050, 4112, 256)])
 def test_product(gpu_device, m, n, k, f32):
     w, s = _matrix(n, k, gpu_device, 1)
     x = workloads.rows_bf16(m, k, gpu_device, seed=2)
@@ -234,7 +237,10 @@ def _check_experts(c, got):
 
 
 @pytest.mark.parametrize("t,h,i,e,k", [(1, 256, 128, 4, 1), (1, 512, 256, 16, 8), (9, 384, 128, 5, 5), (40, 256, 384, 8, 2),
-                                       (130, 512, 128, 3, 2), (300, 256, 256, 33, 4), (700, 128, 128, 2, 1)])
+                                       (130, 512, 128, 3, 2), (300, 256, 256, 33, 4), (700, 128, 128, 2, 1),
+                                       # wide and narrow tiles over every number of mid blocks up to one too many for LDS
+                                       (200, 384, 384, 4, 2), (150, 128, 512, 5, 2), (150, 1152, 640, 3, 2), (30, 384, 512, 4, 3),
+                                       (30, 128, 640, 4, 3), (3, 640, 768, 9, 2)])
 def test_experts(gpu_device, t, h, i, e, k):
     c = _experts_case(gpu_device, t, h, i, e, k)
     _check_experts(c, prompt.experts(**c))

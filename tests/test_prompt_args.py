@@ -15,7 +15,7 @@ P = 1 << 20  # an aligned address that is nobody's
 
 
 def _product(**kw):
-    a = dict(x=P, x_stride=256, w=P, s=P, out=P, out_stride=64, out_f32=0, rows=4, n=64, k=256, workspace=P,
+    a = dict(x=P, x_stride=256, w=P, s=P, out=P, out_stride=64, out_f32=0, rows=40, n=64, k=256, workspace=P,
              workspace_bytes=1 << 20)
     a.update(kw)
     return _lib.lib().mono_prompt_product(C.byref(_lib.PromptProductArgs(**a)), None)
@@ -39,7 +39,9 @@ def test_product_of_no_rows_looks_at_nothing():
 
 def test_workspaces():
     h = _lib.lib()
-    assert h.mono_prompt_product_workspace(5, 64, 256) >= 5 * 256 + 5 * 2 * 4
+    assert h.mono_prompt_product_workspace(40, 64, 256) >= 40 * 256 + 40 * 2 * 4
+    assert h.mono_prompt_product_workspace(5, 64, 256) == 0  # few rows need none
+    assert h.mono_prompt_product_workspace(0, 64, 256) == 0
     assert h.mono_prompt_product_workspace(5, 60, 256) == -1 and b"n must" in h.mono_last_error()
     a = _lib.PromptExpertsArgs(tokens=10, picks=2, experts=4, shared=1, hidden=256, inter=128)
     assert h.mono_prompt_experts_workspace(C.byref(a)) > 0
