@@ -64,7 +64,7 @@ struct WideTile {
   const int lane, wave;
   int kb0 = 0, kbs;       // the tile's blocks of K: the first, how many
   const uint8_t* wp[NT];  // the weight tiles (uniform)
-  const float* sp[2];     // scale rows: of weight tiles 0, 1 and 2, 3
+  const float* sw[2];     // weight scales in LDS by block of K: of weight tiles 0, 1 and 2, 3
   const uint8_t* xp[XD];  // the lane's rows of x for the DMA
   const float* xsp;       // the lane's row of the scales for the DMA
   f32x4 acc[NT][MT] = {};
@@ -73,7 +73,6 @@ struct WideTile {
 
   struct Ahead {
     i32x8 w[NT];
-    float s[2];
   };
 
   // The loads of block kb in the order they go out: part 0 the rows' DMA and the scales, part
@@ -89,8 +88,6 @@ struct WideTile {
         dma4(xsp + (size_t)kb * a.xs_ld, st.s[wave]);
       else if (wave < MT / 4)
         dma4(xsp + (size_t)kb * a.xs_ld, &st.s[0][wave * WAVE]);
-      n.s[0] = ld_const_f32(sp[0] + kb);
-      n.s[1] = ld_const_f32(sp[1] + kb);
     } else if (part <= NT) {
       const uint8_t* at = wp[part - 1] + (size_t)kb * 2048;
       const i32x4 lo = *reinterpret_cast<const i32x4*>(at + 16 * (uint32_t)lane);
@@ -104,9 +101,11 @@ struct WideTile {
   }
 
   // One block's MFMAs, with `ahead(part)` (the loads of a later block) spread among them.
-  // FIRST: the sums begin with this block's.
+  // FIRST: the sums begin with this block's. (The weight scales come from LDS like the rows':
+  // a scalar load among the LDS reads would make each wait for a fragment one for all of
+  // them, since the two return in no common order.)
   template <bool FIRST = false, class F>
-  MONO_DEV void compute(const Stage<MT>& st, const Ahead& n, F ahead) {
+  MONO_DEV void compute(const Stage<MT>& st, const Ahead& n, int kb, F ahead) {
     const int r = lane % 16, g = lane / 16;
     const uint8_t* x = st.x + r * 64 + ((g ^ (r >> 1 & 3)) * 16);
     const float* xs = st.s[MT == 4 ? wave : 0] + r;
@@ -118,6 +117,7 @@ struct WideTile {
       sx[j % 2] = xs[16 * j];
     };
     load(0);
+    const float ws[2] = {sw[0][kb], sw[1][kb]};
     // each MFMA's partial is scaled while the two after it run: neither waits for the other
     constexpr int LAG = MT == 4 ? 2 : 1;  // (128 rows have no registers for two)
     f32x4 p[LAG + 1];
@@ -128,7 +128,7 @@ struct WideTile {
       if (t < MT * NT) {
         if (i == 0 && j + 1 < MT) load(j + 1);
         p[t % (LAG + 1)] = mfma_block<MODE == DENSE_F32>(n.w[i], xv[j % 2]);
-        if (i == 0) c[j % 2][0] = sx[j % 2] * n.s[0], c[j % 2][1] = sx[j % 2] * n.s[1];
+        if (i == 0) c[j % 2][0] = sx[j % 2] * ws[0], c[j % 2][1] = sx[j % 2] * ws[1];
         __builtin_amdgcn_sched_barrier(0);
       }
       if (v >= 0) {
@@ -145,8 +145,8 @@ struct WideTile {
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  MONO_DEV void compute(const Stage<MT>& st, const Ahead& n) {
-    compute(st, n, [](int) {});
+  MONO_DEV void compute(const Stage<MT>& st, const Ahead& n, int kb) {
+    compute(st, n, kb, [](int) {});
   }
 
   // The wave's loads but the last `LEFT` have come, and every wave's: a stage is whole.
@@ -165,12 +165,12 @@ struct WideTile {
     int kb = 0;
     for (; kb + 1 < kbs; kb += 2) {
       arrive<0>();
-      compute(s0, a0, [&](int part) { issue(kb + 1, s1, a1, part); });
+      compute(s0, a0, kb, [&](int part) { issue(kb + 1, s1, a1, part); });
       arrive<0>();
-      compute(s1, a1, [&](int part) { issue(min(kb + 2, kbs - 1), s0, a0, part); });
+      compute(s1, a1, kb + 1, [&](int part) { issue(min(kb + 2, kbs - 1), s0, a0, part); });
     }
     arrive<0>();
-    if (kb < kbs) compute(s0, a0);
+    if (kb < kbs) compute(s0, a0, kb);
   }
 
   // 64 rows: half the MFMA time a block to hide the same latency under, so two blocks ahead.
@@ -183,15 +183,15 @@ struct WideTile {
     int kb = 0;
     for (; kb + 2 < kbs; kb += 3) {
       arrive<EACH>();
-      compute(s0, a0, [&](int part) { issue(min(kb + 2, last), s2, a2, part); });
+      compute(s0, a0, kb, [&](int part) { issue(min(kb + 2, last), s2, a2, part); });
       arrive<EACH>();
-      compute(s1, a1, [&](int part) { issue(min(kb + 3, last), s0, a0, part); });
+      compute(s1, a1, kb + 1, [&](int part) { issue(min(kb + 3, last), s0, a0, part); });
       arrive<EACH>();
-      compute(s2, a2, [&](int part) { issue(min(kb + 4, last), s1, a1, part); });
+      compute(s2, a2, kb + 2, [&](int part) { issue(min(kb + 4, last), s1, a1, part); });
     }
     arrive<0>();
-    if (kb < kbs) compute(s0, a0);
-    if (kb + 1 < kbs) compute(s1, a1);
+    if (kb < kbs) compute(s0, a0, kb);
+    if (kb + 1 < kbs) compute(s1, a1, kb + 1);
   }
 };
 
@@ -204,7 +204,7 @@ struct Place {
 };
 
 template <int MODE, int MT, class... Stages>
-MONO_DEV void tile(const Wide& a, const Place& at, uint32_t (*top)[128], uint8_t* buf, Stages&... stages) {
+MONO_DEV void tile(const Wide& a, const Place& at, float (*sw)[MAX_DIM / BLK], uint32_t (*top)[128], uint8_t* buf, Stages&... stages) {
   constexpr int BM = 16 * MT;
   const int64_t first = at.first;
   const int count = at.count, tn = at.tn;
@@ -221,8 +221,15 @@ MONO_DEV void tile(const Wide& a, const Place& at, uint32_t (*top)[128], uint8_t
     row[i] = MODE == UP ? tn * (BN / 2) + wn * (TN / 2) + 16 * (i % 2) + (i / 2) * a.half : tn * BN + wn * TN + 16 * i;
     const int n = min(row[i], a.n - 16);  // past the matrix: its last rows again, not stored
     W.wp[i] = at.w + (size_t)n * a.kb * BLK;
-    if (i % 2 == 0) W.sp[i / 2] = at.s + (size_t)(n / BLK) * a.kb;
   }
+  // the tile's two rows of weight scales (gate and up; else of its two 128 weight rows)
+  for (int i = threadIdx.x; i < 2 * W.kbs; i += T) {
+    const int h = i >= W.kbs, kb = i - h * W.kbs;
+    const int n = MODE == UP ? tn * (BN / 2) + h * a.half : min(tn * BN + h * BLK, a.n - 1);
+    sw[h][kb] = at.s[(size_t)(n / BLK) * a.kb + W.kb0 + kb];
+  }
+  W.sw[0] = sw[MODE == UP ? 0 : wn / 2];
+  W.sw[1] = sw[MODE == UP ? 1 : wn / 2];
 #pragma unroll
   for (int h = 0; h < W.XD; ++h) {
     const int r = lane / 4;  // 16 rows x 64 bytes a DMA; the 16-byte pieces are swapped by row so that a
@@ -306,7 +313,7 @@ MONO_DEV void tile(const Wide& a, const Place& at, uint32_t (*top)[128], uint8_t
 // LDS whole and each wave goes through its weight columns, 64 at a time, without a barrier;
 // the next weights are on their way at every moment, also while sums are stored.
 template <int KB, int MT>
-MONO_DEV void resident_tile(const Wide& a, const Place& at, int group, uint8_t* buf, Stage<MT> (&st)[KB]) {
+MONO_DEV void resident_tile(const Wide& a, const Place& at, int group, float* sw, uint8_t* buf, Stage<MT> (&st)[KB]) {
   WideTile<DOWN, MT> W(a);
   const int lane = W.lane, r = lane / 4, last = a.kb - 1;
   using Ahead = typename WideTile<DOWN, MT>::Ahead;
@@ -315,15 +322,17 @@ MONO_DEV void resident_tile(const Wide& a, const Place& at, int group, uint8_t* 
     W.xp[h] = a.xq + (size_t)(at.first + min((W.XD * W.wave + h) * 16 + r, at.count - 1)) * a.kb * BLK +
               (((lane % 4) ^ (r >> 1 & 3)) * 16);
   W.xsp = a.xs + at.first + min((W.wave * WAVE + lane) % (16 * MT), at.count - 1);
-  W.sp[0] = W.sp[1] = at.s;
+  // the scales of the columns to come, [a turn's two 128 columns][KB]; past K's end zero
+  const int step = a.groups * BN;
+  for (int i = threadIdx.x; i < (a.n + step - 1) / step * 2 * KB; i += T) {
+    const int c = group * BN + i / (2 * KB) * step + i / KB % 2 * BLK, kb = i % KB;
+    sw[i] = c < a.n && kb <= last ? at.s[(size_t)(c / BLK) * a.kb + kb] : 0.f;
+  }
   Ahead n[2];
-  // block kb of the 64 columns from col on; past K's end (an odd number of blocks) the last one, scaled by zero
+  // block kb of the 64 columns from col on; past K's end (an odd number of blocks) the last one
   const auto weights = [&](int col, int kb, Ahead& to, int part) {
     const int c = min(col, a.n - PART), b = min(kb, last);
-    if (part == 0) {
-      const float v = ld_const_f32(at.s + (size_t)(c / BLK) * a.kb + b);
-      to.s[0] = to.s[1] = kb <= last ? v : 0.f;
-    } else if (part <= NT) {
+    if (part && part <= NT) {
       const uint8_t* p = at.w + (size_t)(c + 16 * (part - 1)) * a.kb * BLK + (size_t)b * 2048;
       const i32x4 lo = *reinterpret_cast<const i32x4*>(p + 16 * (uint32_t)lane);
       const i32x4 hi = *reinterpret_cast<const i32x4*>(p + 16 * (uint32_t)lane + 1024);
@@ -331,11 +340,11 @@ MONO_DEV void resident_tile(const Wide& a, const Place& at, int group, uint8_t* 
     }
   };
   int col = group * BN + W.wave * TN;
-  const int step = a.groups * BN;
+  W.sw[0] = W.sw[1] = sw + W.wave / 2 * KB;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) W.issue(min(kb, last), st[kb], n[0], 0);
 #pragma unroll
-  for (int part = 0; part <= NT; ++part) weights(col, 0, n[0], part);
+  for (int part = 1; part <= NT; ++part) weights(col, 0, n[0], part);
   W.template arrive<0>();
   for (; col < a.n; col += step) {
 #pragma unroll
@@ -344,15 +353,16 @@ MONO_DEV void resident_tile(const Wide& a, const Place& at, int group, uint8_t* 
         weights(kb + 1 < KB ? col : col + step, kb + 1 < KB ? kb + 1 : 0, n[(kb + 1) % 2], part);
       };
       if (kb == 0)
-        W.template compute<true>(st[kb], n[kb % 2], ahead);
+        W.template compute<true>(st[kb], n[kb % 2], kb, ahead);
       else
-        W.compute(st[kb], n[kb % 2], ahead);
+        W.compute(st[kb], n[kb % 2], kb, ahead);
     }
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       const f32x4 y[NT] = {W.acc[0][j], W.acc[1][j], W.acc[2][j], W.acc[3][j]};
       store_part(buf, a.part, at.first + 16 * j, at.count - 16 * j, col, y);
     }
+    W.sw[0] = W.sw[1] = W.sw[0] + 2 * KB;
   }
 }
 
@@ -360,6 +370,7 @@ template <int KB>
 __global__ __launch_bounds__(T, 2) void k_down_resident(Wide a) {
   static_assert(KB % 2 == 0, "the weights' two register sets alternate");
   __shared__ Stage<8> st[KB];
+  __shared__ float sw[MAX_DIM / BN / 4 * 2 * KB];  // (4 workgroups or more a tile wherever it has 4 turns' columns)
   __shared__ uint8_t bufs[WN][2048];
   const int per = gridDim.x / 8, b = (blockIdx.x % 8) * per + blockIdx.x / 8, tm = b / a.groups;
   if (tm >= a.tiles_m) return;
@@ -368,9 +379,9 @@ __global__ __launch_bounds__(T, 2) void k_down_resident(Wide a) {
   const Place at{a.w + (size_t)t.expert * a.n * a.kb * BLK, a.s + (size_t)t.expert * (a.n / BLK) * a.kb, t.first, t.count, 0, 0};
   uint8_t* buf = bufs[threadIdx.x / WAVE];
   if (t.count <= 64)
-    resident_tile<KB, 4>(a, at, b % a.groups, buf, reinterpret_cast<Stage<4>(&)[KB]>(st));
+    resident_tile<KB, 4>(a, at, b % a.groups, sw, buf, reinterpret_cast<Stage<4>(&)[KB]>(st));
   else
-    resident_tile<KB, 8>(a, at, b % a.groups, buf, st);
+    resident_tile<KB, 8>(a, at, b % a.groups, sw, buf, st);
 }
 
 template <int MODE, int MT>
@@ -379,6 +390,7 @@ __global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
   // another's DMA)
   __shared__ Stage<4> l0, l1, l2;
   __shared__ Stage<8> h0, h1;
+  __shared__ float sw[2][MAX_DIM / BLK];
   __shared__ uint32_t top[MODE == UP ? WN : 1][128];
   __shared__ uint8_t bufs[MODE == UP || MODE == DENSE_F32 ? 1 : WN][2048];
   uint8_t* buf = bufs[MODE == UP || MODE == DENSE_F32 ? 0 : threadIdx.x / WAVE];
@@ -409,11 +421,11 @@ __global__ __launch_bounds__(T, MODE == DENSE_F32 ? 1 : 2) void k_wide(Wide a) {
     at.count = (int)min((int64_t)(16 * MT), a.rows - at.first);
   }
   if constexpr (MT == 4)
-    tile<MODE, 4>(a, at, top, buf, l0, l1, l2);
+    tile<MODE, 4>(a, at, sw, top, buf, l0, l1, l2);
   else if ((MODE == UP || MODE == DOWN) && at.count <= 64)
-    tile<MODE, 4>(a, at, top, buf, l0, l1, l2);
+    tile<MODE, 4>(a, at, sw, top, buf, l0, l1, l2);
   else
-    tile<MODE, 8>(a, at, top, buf, h0, h1);
+    tile<MODE, 8>(a, at, sw, top, buf, h0, h1);
 }
 
 template <int MODE, int MT>
