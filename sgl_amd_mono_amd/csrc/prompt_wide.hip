@@ -126,7 +126,8 @@ struct WideTile {
     for (int t = 0; t < MT * NT + LAG; ++t) {
       const int i = t % NT, j = t / NT, v = t - LAG;
       if (t < MT * NT) {
-        if (i == 0 && j + 1 < MT) load(j + 1);
+        // (behind the fragment's first MFMA, whose wait for LDS then finds nothing younger to wait for)
+        if (i == 1 && j + 1 < MT) load(j + 1);
         p[t % (LAG + 1)] = mfma_block<MODE == DENSE_F32>(n.w[i], xv[j % 2]);
         if (i == 0) c[j % 2][0] = sx[j % 2] * ws[0], c[j % 2][1] = sx[j % 2] * ws[1];
         __builtin_amdgcn_sched_barrier(0);
