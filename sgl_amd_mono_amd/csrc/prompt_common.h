@@ -117,17 +117,23 @@ MONO_DEV uint32_t pack_halves(float a, float b) {
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
 }
 
+// The largest of four lane groups' values (lanes l, l ^ 16, l ^ 32, l ^ 48), in all of them.
+MONO_DEV uint32_t groups_umax(uint32_t v) {
+  const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(v, v, false, false));
+  v = max(a[0], a[1]);
+  const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(v, v, false, false));
+  return max(b[0], b[1]);
+}
+
 // A lane's 16 of one place's 64 columns (tiles of 16 weight rows i, columns 16 i + 4 g + e of
-// lane group g) as halves of a Parts block: the scale, and the values divided by it.
+// lane group g) as halves of a Parts block: the scale, and the values divided by it. (The
+// float maximum passes over a NaN, which stays one as a half.)
 MONO_DEV float part_block(const f32x4 (&y)[4], u32x2 (&h)[4]) {
-  uint32_t m = 0;
+  float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m = max(m, abs_bits(y[i][e]));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 16, WAVE));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 32, WAVE));
-  // 2^14 / 2^floor(log2 max); a block that is not finite keeps its values as they are
+  for (int i = 0; i < 4; ++i) top = fmaxf(fmaxf(top, fmaxf(fabsf(y[i][0]), fabsf(y[i][1]))), fmaxf(fabsf(y[i][2]), fabsf(y[i][3])));
+  const uint32_t m = groups_umax(__float_as_uint(top));
+  // 2^14 / 2^floor(log2 max); a block with an infinity keeps its values as they are
   const int e = m < 0x7f800000u ? max((int)(m >> 23), 27) : 127 + 14;
   const float inv = __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
 #pragma unroll

@@ -166,7 +166,7 @@ MONO_DEV void narrow_tile(const Narrow& a, f32x4* red, const uint8_t* w, const f
   const size_t at = (size_t)(first + m) * a.out_ld + n0 + 4 * (lane / 16);
   if (MODE == UP) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) y[0][r] = y[0][r] / (1.0f + expf(-y[0][r])) * y[NT - 1][r];
+    for (int r = 0; r < 4; ++r) y[0][r] = silu(y[0][r]) * y[NT - 1][r];
   }
   if (MODE != UP && a.splits > 1)
     *reinterpret_cast<f32x4*>(a.part + ((size_t)blockIdx.z * a.rows + first + m) * a.n + n0 + 4 * (lane / 16)) = y[0];

@@ -255,12 +255,10 @@ MONO_DEV void tile(const Wide& a, const Place& at, float (*sw)[MAX_DIM / BLK], u
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float gate = W.acc[i][j][e];
-          W.acc[i][j][e] = gate / (1.0f + expf(-gate)) * W.acc[i + 2][j][e];
+          W.acc[i][j][e] = silu(W.acc[i][j][e]) * W.acc[i + 2][j][e];
           m = max(m, abs_bits(W.acc[i][j][e]));
         }
-      m = max(m, (uint32_t)__shfl_xor((int)m, 16, WAVE));
-      m = max(m, (uint32_t)__shfl_xor((int)m, 32, WAVE));
+      m = groups_umax(m);
       if (g == 0) top[wn][16 * j + lane] = m;
     }
     __syncthreads();
