@@ -311,6 +311,10 @@ MONO_DEV void tile(const Wide& a, const Place& at, float (*sw)[MAX_DIM / BLK], u
 // The experts' down products where K is short (a few blocks of mids): the tile's rows stay in
 // LDS whole and each wave goes through its weight columns, 64 at a time, without a barrier;
 // the next weights are on their way at every moment, also while sums are stored.
+// 256 columns a turn, at most so many turns a workgroup (8192 tokens x 7168 columns: 2 turns 528
+// us, 4 496, 7 501, 14 554; 1500 tokens 225, 231, 247, 281).
+constexpr int TURNS = 4;
+
 template <int KB, int MT>
 MONO_DEV void resident_tile(const Wide& a, const Place& at, int group, float* sw, uint8_t* buf, Stage<MT> (&st)[KB]) {
   WideTile<DOWN, MT> W(a);
@@ -369,7 +373,7 @@ template <int KB>
 __global__ __launch_bounds__(T, 2) void k_down_resident(Wide a) {
   static_assert(KB % 2 == 0, "the weights' two register sets alternate");
   __shared__ Stage<8> st[KB];
-  __shared__ float sw[MAX_DIM / BN / 4 * 2 * KB];  // (4 workgroups or more a tile wherever it has 4 turns' columns)
+  __shared__ float sw[TURNS * 2 * KB];
   __shared__ uint8_t bufs[WN][2048];
   const int per = gridDim.x / 8, b = (blockIdx.x % 8) * per + blockIdx.x / 8, tm = b / a.groups;
   if (tm >= a.tiles_m) return;
@@ -462,7 +466,7 @@ hipError_t wide_experts_down(const Experts& e, hipStream_t st) {
   a.tiles_m = e.tiles;
   a.tiles_n = (e.hidden + BN - 1) / BN;
   if (a.kb > 4) return launch<DOWN, 8>(a, 1, st);
-  a.groups = min(a.tiles_n, 4);
+  a.groups = (a.tiles_n + TURNS - 1) / TURNS;
   const uint32_t grid = (uint32_t)(((int64_t)a.tiles_m * a.groups + 7) / 8 * 8);
   if (a.kb > 2)
     k_down_resident<4><<<grid, T, 0, st>>>(a);
