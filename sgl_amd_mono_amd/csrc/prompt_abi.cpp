@@ -81,7 +81,7 @@ int product_shape(int64_t rows, int32_t n, int32_t k) {
 // A product's plan over its workspace: the rows' codes and scales, and its parts.
 size_t product_space(void* ws, Product& p) {
   Space sp{static_cast<char*>(ws)};
-  p.plan = product_plan(p.rows, p.n, p.k);
+  p.plan = product_plan(p.rows, p.n, p.k, p.f32);
   if (p.plan.kind != ProductPlan::FEW) p.q = sp.rows(p.rows, p.k);
   if (p.plan.splits > 1) p.part = sp.take<float>((size_t)p.plan.splits * p.rows * p.n);
   return sp.off;
@@ -100,8 +100,10 @@ int experts_shape(const mono_prompt_experts_args& a) {
   return MONO_OK;
 }
 
-// Where the wide tiles take over: picks a routed expert gets on average.
-constexpr int WIDE_PICKS = 24;
+// Where the wide tiles take over: picks that a routed expert gets on average (256 experts
+// of 7168 x 512, 8 picks a token, narrow / wide us: 128 tokens 424 / 453, 256 tokens 514 /
+// 496, 512 tokens 652 / 558).
+constexpr int WIDE_PICKS = 7;
 
 // The call's plan over its workspace; `e.tiles` bounds the tile list.
 size_t experts_plan(const mono_prompt_experts_args& a, void* ws, Experts& e) {
@@ -143,7 +145,11 @@ extern "C" int64_t mono_prompt_product_workspace(int64_t rows, int32_t n, int32_
   Product p{};
   p.rows = rows, p.n = n, p.k = k;
   mono::abi_ok();
-  return rows ? (int64_t)product_space(nullptr, p) : 0;
+  if (!rows) return 0;
+  const size_t bf16 = product_space(nullptr, p);
+  p.f32 = true;
+  const size_t f32 = product_space(nullptr, p);
+  return (int64_t)(bf16 > f32 ? bf16 : f32);
 }
 
 extern "C" int mono_prompt_product(const mono_prompt_product_args* args, void* stream) {

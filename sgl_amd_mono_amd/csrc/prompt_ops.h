@@ -62,28 +62,35 @@ hipError_t sort_quant(const void* x, int64_t stride, int64_t tokens, int k, cons
 // How a product runs, by its sizes alone.
 //
 // FEW     at most 16 rows of FEW_BYTES codes: every workgroup rounds them for itself
-// NARROW  up to WIDE_ROWS rows: workgroups of 16 weight rows, 8 waves along K
+// NARROW  up to WIDE_ROWS rows (f32: NARROW_TILES_F32 workgroups): workgroups of 16 weight rows
+//         and up to 64 rows, 8 waves along K
 // WIDE    more: tiles of 256 weight rows x 64 or 128 rows, waves along the weight rows
+//
+// (narrow / wide, us a call in a graph, rows x 2112 x 7168: 17 rows 11.0 / 13.3, 24 12.3 / 13.5,
+// 33 19.0 / 14.2, 65 24.9 / 16.0; x 7168 x 4096: 17 11.4 / 13.2, 33 16.9 / 14.4. In f32, whose
+// wide tiles widen their codes in every wave: rows x 576 x 7168: 129 rows 16.6 / 19.6, 257
+// 23.1 / 21.1; x 2112: 45 18.6 / 19.1, 65 22.2 / 20.4; x 128: 1024 23.9 / 24.5.)
 //
 // `splits` > 1: K is shared out over that many workgroups, whose f32 sums a second launch
 // adds in order. Where the tiles alone leave CUs without work, and each share keeps at
 // least 8 blocks of K.
 constexpr int FEW_BYTES = 32768;
-constexpr int WIDE_ROWS = 96;
+constexpr int WIDE_ROWS = 32, NARROW_TILES_F32 = 128;
 struct ProductPlan {
   enum Kind { FEW, NARROW, WIDE } kind;
   int splits;
   int bm;  // rows of a tile
 };
-inline ProductPlan product_plan(int64_t rows, int n, int k) {
+inline ProductPlan product_plan(int64_t rows, int n, int k, bool f32) {
   if (rows <= 16 && rows * k <= FEW_BYTES) return {ProductPlan::FEW, 1, 16};
   const int kb = k / BLK;
   constexpr int64_t FULL = 256;  // workgroups that leave no CU without one
   int64_t tiles;
   ProductPlan p;
-  if (rows <= WIDE_ROWS) {
+  const int64_t narrow = n / 16 * ((rows + 63) / 64);
+  if (f32 ? narrow <= NARROW_TILES_F32 : rows <= WIDE_ROWS) {
     p = {ProductPlan::NARROW, 1, 64};
-    tiles = n / 16 * ((rows + 63) / 64);
+    tiles = narrow;
   } else {
     const int64_t wide = (n + 255) / 256;
     p = {ProductPlan::WIDE, 1, (rows + 127) / 128 * wide < 256 ? 64 : 128};
