@@ -102,14 +102,16 @@ int experts_shape(const mono_prompt_experts_args& a) {
 
 // Where the wide tiles take over: picks that a routed expert gets on average (256 experts
 // of 7168 x 512, 8 picks a token, narrow / wide us: 128 tokens 424 / 453, 256 tokens 514 /
-// 496, 512 tokens 652 / 558).
-constexpr int WIDE_PICKS = 7;
+// 496, 512 tokens 652 / 558). Never for a few tokens: the narrow up products widen their
+// codes to bf16, whose MFMA is exact where the FP8 one rounds, and a mid that falls over a
+// code's border shows most where few tokens share the error.
+constexpr int WIDE_PICKS = 7, FEW_TOKENS = 64;
 
 // The call's plan over its workspace; `e.tiles` bounds the tile list.
 size_t experts_plan(const mono_prompt_experts_args& a, void* ws, Experts& e) {
   Space sp{static_cast<char*>(ws)};
   const int64_t picks = a.tokens * a.picks, places = picks + (a.shared ? a.tokens : 0);
-  e.wide = picks > WIDE_PICKS * a.experts;
+  e.wide = a.tokens > FEW_TOKENS && picks > (int64_t)WIDE_PICKS * a.experts;
   e.bm = e.wide ? 128 : 64;
   e.tiles = (int)all_tiles(a.tokens, picks, a.experts, e.bm, a.shared);
   e.x = sp.rows(a.tokens, a.hidden);

@@ -149,7 +149,7 @@ MONO_DEV void narrow_tile(const Narrow& a, f32x4* red, const uint8_t* w, const f
     xsp[j] = a.xs + row;
   }
   f32x4 acc[NT][MT] = {};
-  accumulate<MODE == DENSE_F32, NT, MT>(wp, sp, xp, xsp, a.xs_ld, kb0, kb1, wave, acc);
+  accumulate<MODE != DENSE_BF16, NT, MT>(wp, sp, xp, xsp, a.xs_ld, kb0, kb1, wave, acc);
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
