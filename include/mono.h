@@ -489,7 +489,7 @@ typedef struct {
   int64_t x_stride;    /* a multiple of 8; x itself 16-byte aligned */
   const void* w;       /* e4m3 [n, k], (16, 16)-shuffled */
   const float* s;      /* f32 [ceil(n / 128), k / 128] */
-  void* out;           /* bf16 or f32 [rows, n], rows out_stride elements apart */
+  void* out;           /* bf16 or f32 [rows, n], rows out_stride elements apart; no element of x */
   int64_t out_stride;  /* a multiple of 8; out itself 16-byte aligned */
   int32_t out_f32;     /* 0: bf16 */
   int64_t rows;        /* 0..1048576 */
@@ -547,7 +547,8 @@ typedef struct {
   const float* s13;         /* f32 [E, 2 inter / 128, hidden / 128] */
   const void* w2;           /* e4m3 [E, hidden, inter], (16, 16)-shuffled */
   const float* s2;          /* f32 [E, hidden / 128, inter / 128] */
-  const void* residual;     /* optional bf16 [tokens, hidden] added to the sum */
+  const void* residual;     /* optional bf16 [tokens, hidden] added to the sum; out itself, or no
+                               element of it */
   int64_t residual_stride;  /* a multiple of 8 */
   void* out;                /* bf16 [tokens, hidden] */
   int64_t out_stride;       /* a multiple of 8 */

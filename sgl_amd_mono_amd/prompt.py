@@ -64,6 +64,19 @@ def _rows(t: torch.Tensor, name: str, shape: tuple, dtype, dev: torch.device) ->
     return stride[0]
 
 
+def _apart(a: torch.Tensor, a_stride: int, b: torch.Tensor, b_stride: int) -> bool:
+    """Whether two matrices of bytes-apart rows share no element: neither's memory reaches the
+    other's, or both are columns of one wider matrix, side by side."""
+    if not a.numel() or not b.numel():
+        return True
+    sa, sb = a_stride * a.element_size(), b_stride * b.element_size()
+    wa, wb = a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa + (a.shape[0] - 1) * sa + wa <= pb or pb + (b.shape[0] - 1) * sb + wb <= pa:
+        return True
+    return sa == sb and (pb - pa) % sa >= wa and (pb - pa) % sa + wb <= sa
+
+
 def _enqueue(dev: torch.device, fn, args) -> None:
     if torch.cuda.current_device() == dev.index:
         rc = fn(C.byref(args), _raw_stream(dev.index))
@@ -90,7 +103,7 @@ def product(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, out: torch.Tensor
     E4M3 in the (16, 16) layout with scales ``s`` f32 [ceil(N / 128), K / 128] -> [rows, N]
     in ``dtype`` (bf16 or f32; ``out``'s own where that is given). The rows are rounded to
     E4M3 with a scale for each 128 columns; a row that holds a NaN or an infinity has NaN
-    outputs. N % 16 == 0, K % 128 == 0."""
+    outputs. N % 16 == 0, K % 128 == 0. ``out`` must share no memory with ``x``."""
     dev = _gpu(x, "x")
     if x.dim() != 2 or not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise ValueError(f"x and w: expected [rows, K] and [N, K], got {tuple(x.shape)} and {tuple(getattr(w, 'shape', ()))}")
@@ -103,7 +116,11 @@ def product(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, out: torch.Tensor
         raise ValueError(f"out: expected dtype torch.bfloat16 or torch.float32, got {dtype}")
     if out is None:
         out = torch.empty(m, n, dtype=dtype, device=dev)
-    out_stride = _rows(out, "out", (m, n), dtype, dev)
+        out_stride = n
+    else:
+        out_stride = _rows(out, "out", (m, n), dtype, dev)
+        if not _apart(x, stride, out, out_stride):
+            raise ValueError("out: shares memory with x")
     args = _lib.PromptProductArgs(x=x.data_ptr(), x_stride=stride, w=w.data_ptr(), s=s.data_ptr(), out=out.data_ptr(),
                                   out_stride=out_stride, out_f32=dtype == torch.float32, rows=m, n=n, k=k)
     lib = _lib.lib()
@@ -130,8 +147,8 @@ def append(kv_a: torch.Tensor, ik: torch.Tensor, req: torch.Tensor, pos: torch.T
     ik_stride = _rows(ik, "ik", (t, INDEX_DIM), kv_a.dtype, dev)
     need(req, "req", (t,), torch.int32, dev)
     need(pos, "pos", (t,), torch.int32, dev)
-    if page_table.dim() != 2:
-        raise ValueError(f"page_table: expected [requests, pages], got {tuple(page_table.shape)}")
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+        raise ValueError(f"page_table: expected [requests, pages], got {tuple(getattr(page_table, 'shape', ()))}")
     need(page_table, "page_table", tuple(page_table.shape), torch.int32, dev)
     pages = caches.ikv.shape[0]
     need(caches.ikv, "ikv", (pages, 4, PAGE, 16), torch.uint8, dev)
@@ -142,8 +159,8 @@ def append(kv_a: torch.Tensor, ik: torch.Tensor, req: torch.Tensor, pos: torch.T
     need(g_kv, "g_kv", (KV_LORA,), torch.bfloat16, dev)
     need(g_ik, "g_ik", (INDEX_DIM,), torch.float32, dev)
     need(b_ik, "b_ik", (INDEX_DIM,), torch.float32, dev)
-    if rope_cos.dim() != 2 or rope_cos.shape[1] != PE_DIM // 2:
-        raise ValueError(f"rope_cos: expected [max_pos, {PE_DIM // 2}], got {tuple(rope_cos.shape)}")
+    if not isinstance(rope_cos, torch.Tensor) or rope_cos.dim() != 2 or rope_cos.shape[1] != PE_DIM // 2:
+        raise ValueError(f"rope_cos: expected [max_pos, {PE_DIM // 2}], got {tuple(getattr(rope_cos, 'shape', ()))}")
     need(rope_cos, "rope_cos", tuple(rope_cos.shape), torch.float32, dev)
     need(rope_sin, "rope_sin", tuple(rope_cos.shape), torch.float32, dev)
     args = _lib.PromptAppendArgs(
@@ -164,7 +181,7 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: torc
     f32 [tokens, picks] the router's answer (an id outside the routed experts is routed
     nowhere), the weights and scales those of ``moe.Fp8MoeWeights``. With ``shared`` the
     last expert is the shared one (every token, weight 1) and ids name the others. Rows of
-    ``x``, ``residual`` and ``out`` may lie apart; ``out`` may be ``residual``."""
+    ``x``, ``residual`` and ``out`` may lie apart; ``out`` may be ``residual`` or ``x`` itself."""
     dev = _gpu(x, "x")
     if x.dim() != 2 or not isinstance(ids, torch.Tensor) or ids.dim() != 2:
         raise ValueError(f"x and ids: expected [tokens, H] and [tokens, picks], got {tuple(x.shape)} and "
@@ -181,8 +198,12 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: torc
     need(s2, "s2", (e, h // 128, i // 128), torch.float32, dev)
     res_stride = h if residual is None else _rows(residual, "residual", (t, h), torch.bfloat16, dev)
     if out is None:
-        out = torch.empty(t, h, dtype=torch.bfloat16, device=dev)
-    out_stride = _rows(out, "out", (t, h), torch.bfloat16, dev)
+        out, out_stride = torch.empty(t, h, dtype=torch.bfloat16, device=dev), h
+    else:
+        out_stride = _rows(out, "out", (t, h), torch.bfloat16, dev)
+        same = residual is None or (out.data_ptr() == residual.data_ptr() and out_stride == res_stride)
+        if not same and not _apart(residual, res_stride, out, out_stride):
+            raise ValueError("out: shares memory with residual, and is not residual itself")
     args = _lib.PromptExpertsArgs(
         x=x.data_ptr(), x_stride=x_stride, ids=ids.data_ptr(), weights=weights.data_ptr(), w13=w13.data_ptr(),
         s13=s13.data_ptr(), w2=w2.data_ptr(), s2=s2.data_ptr(), residual=_lib.ptr(residual), residual_stride=res_stride,

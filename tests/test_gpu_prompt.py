@@ -102,6 +102,40 @@ def test_product_non_finite_and_extreme_rows(gpu_device, m):
     _same(got, want, mag, True, k)
 
 
+@pytest.mark.parametrize("m", [3, 30, 200])
+def test_product_nan_weights_stay_in_their_output(gpu_device, m):
+    n, k = 80, 1280
+    w, s = _matrix(n, k, gpu_device, 8)
+    x = workloads.rows_bf16(m, k, gpu_device, seed=9)
+    clean = prompt.product(x, w, s)
+    flat = w.view(torch.uint8).flatten()  # row 37, column 1279 in the (16, 16) layout
+    flat[((37 // 16 * (k // 32) + 1279 // 32) * 2 + 1279 % 32 // 16) * 256 + 37 % 16 * 16 + 1279 % 16] = 0x7F
+    got = prompt.product(x, w, s)
+    assert bool(got[:, 37].isnan().all())
+    keep = [c for c in range(n) if c != 37]
+    assert torch.equal(got[:, keep], clean[:, keep])
+
+
+@pytest.mark.parametrize("m,stride", [(5, 1 << 29), (40, 1 << 26), (300, 1 << 23)])
+def test_product_rows_far_apart(gpu_device, m, stride):
+    """Row offsets past 32 bits."""
+    n, k = 64, 256
+    w, s = _matrix(n, k, gpu_device, 10)
+    x = workloads.rows_bf16(m, k, gpu_device, seed=11)
+    far = torch.empty((m - 1) * stride + k, dtype=torch.bfloat16, device=gpu_device).as_strided((m, k), (stride, 1))
+    far.copy_(x)
+    assert torch.equal(prompt.product(far, w, s), prompt.product(x, w, s))
+
+
+def test_product_refuses_shared_memory(gpu_device):
+    w, s = _matrix(256, 256, gpu_device, 12)
+    x = workloads.rows_bf16(4, 512, gpu_device, seed=13)
+    want = prompt.product(x[:, :256].clone(), w, s)
+    with pytest.raises(ValueError, match="shares memory with x"):
+        prompt.product(x[:, :256], w, s, out=x[:, :256])
+    assert torch.equal(prompt.product(x[:, :256], w, s, out=x[:, 256:]), want)
+
+
 def test_product_of_no_rows(gpu_device):
     w, s = _matrix(64, 256, gpu_device, 7)
     assert prompt.product(torch.empty(0, 256, dtype=torch.bfloat16, device=gpu_device), w, s).shape == (0, 64)
@@ -201,6 +235,26 @@ def test_append_non_finite(gpu_device, raw):
     assert torch.equal(got.ikv[page, :, others], want.ikv[page, :, others])
 
 
+def test_append_far_into_a_long_cache(gpu_device):
+    """Slots whose rows lie past 2^31 bytes."""
+    c = _append_case(gpu_device, [(60, 9)], False, False)
+    want, _ = _append_both(c)
+    pages, near = 60000, c["page_table"][0].tolist()
+    far = dict(c, page_table=c["page_table"] + (pages - 8))
+    big = AttnCaches(ikv=torch.empty(pages, 4, 64, 16, dtype=torch.uint8, device=gpu_device),
+                     iks=torch.empty(pages, 4, 64, dtype=torch.uint8, device=gpu_device),
+                     kv=torch.empty(pages * 64, 576, dtype=torch.uint8, device=gpu_device),
+                     kv_scale=torch.empty(pages * 64, device=gpu_device))
+    prompt.append(**dict(far, caches=big))
+    for p in (60, 63, 64, 68):
+        a, b, t = near[p // 64], near[p // 64] + pages - 8, p % 64
+        assert torch.equal(big.kv[b * 64 + t].cpu(), want["kv"][a * 64 + t])
+        assert float(big.kv_scale[b * 64 + t]) == float(want["kv_scale"][a * 64 + t])
+        assert torch.equal(big.ikv[b, :, t].cpu(), want["ikv"][a, :, t])
+        at = t % 16 * 4 + t // 16
+        assert torch.equal(big.iks[b, :, at].cpu(), want["iks"][a, :, at])
+
+
 def test_append_of_nothing(gpu_device):
     c = _append_case(gpu_device, [(0, 3)], False, False)
     before = c["caches"].kv.clone()
@@ -280,6 +334,30 @@ def test_experts_strided_in_place(gpu_device):
     xw[:, 8:] = c["x"]
     got = prompt.experts(**dict(c, x=xw[:, 8:], residual=buf[:, 8:-32], out=buf[:, 8:-32]))
     assert torch.equal(got, want) and bool((buf[:, :8] == 0).all()) and bool((buf[:, -32:] == 0).all())
+
+
+def test_experts_out_over_x_and_residual(gpu_device):
+    c = _experts_case(gpu_device, 200, 256, 128, 8, 2)
+    want = prompt.experts(**c)
+    x = c["x"].clone()
+    assert torch.equal(prompt.experts(**dict(c, x=x, out=x)), want)
+    res = torch.cat([c["residual"], c["residual"][:1]])
+    with pytest.raises(ValueError, match="shares memory with residual"):
+        prompt.experts(**dict(c, residual=res[:-1], out=res[1:]))
+    assert torch.equal(prompt.experts(**dict(c, residual=res[:-1], out=res[:-1])), want)
+
+
+def test_experts_non_finite_tokens(gpu_device):
+    """A token's NaN or infinity is its own: the others' outputs keep their bits."""
+    for t in (20, 200):
+        c = _experts_case(gpu_device, t, 256, 128, 8, 2)
+        want = prompt.experts(**c)
+        x = c["x"].clone()
+        x[3, 7], x[5, 200] = float("nan"), float("inf")
+        got = prompt.experts(**dict(c, x=x))
+        assert bool(got[3].isnan().all()) and bool(got[5].isnan().all())
+        keep = [i for i in range(t) if i not in (3, 5)]
+        assert torch.equal(got[keep], want[keep])
 
 
 def test_experts_of_no_tokens(gpu_device):

@@ -106,6 +106,17 @@ def test_cpu_tensors_are_refused():
         prompt.append(x, x, s, s, s, AttnCaches(w, w, w, None), s, s, s, s, s)
 
 
+def test_shared_memory_is_told_apart():
+    wide = torch.zeros(6, 64, dtype=torch.bfloat16)
+    a, b = wide[:, :32], wide[:, 32:]
+    assert prompt._apart(a, 64, b, 64) and prompt._apart(b, 64, a, 64)
+    assert not prompt._apart(a, 64, wide[:, 24:48], 64) and not prompt._apart(wide[:, 24:48], 64, a, 64)
+    assert not prompt._apart(a, 64, a, 64)
+    assert prompt._apart(wide[:2], 64, wide[2:], 64) and not prompt._apart(wide[:3], 64, wide[2:], 64)
+    assert not prompt._apart(a, 64, wide.view(12, 32)[::2][:, :16], 32)  # other strides: only ranges are told apart
+    assert prompt._apart(a[:0], 64, a, 64)
+
+
 def test_the_restated_append_is_the_front_s_row():
     """The f64 restatement writes what the decode layer's oracle (f32) writes, on values
     where no code hangs on f32's last bits."""
