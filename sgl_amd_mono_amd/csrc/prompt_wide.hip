@@ -21,11 +21,12 @@
 // 1.9 (1.6) GHz. With every load a cache hit the first takes 208 us: what is left is the
 // vector memory path's 48 KB a tile and block, the barrier a block and the last round of
 // workgroups. Steps that brought it there, us: 64 x 64 a wave through narrow tiles 1932; this
-// split 340; MFMA ahead of the scaling, fragments a step ahead 245 (two workgroups a CU; 313
-// with their eight waves behind one barrier); loads spread among the MFMAs and LDS pieces
-// without bank conflicts 227; the fragment's reads behind an MFMA 214. Tried and left: tiles
-// of 256 x 256 in four waves of 452 registers 320 (the sums then lie where the vector unit
-// cannot add to them), half tiles for the last round 229.
+// split 340; MFMA ahead of the scaling, fragments a step ahead 245; loads spread among the
+// MFMAs and LDS pieces without bank conflicts 227; the fragment's reads behind an MFMA 214.
+// Tried and left: eight waves over 256 x 256 behind one barrier 251 (a third less from L2, and
+// no second workgroup to fill its waits); tiles of 256 x 256 in four waves of 452 registers 320
+// (the sums then lie where the vector unit cannot add to them); half tiles for the last round
+// 229.
 #include "prompt_common.h"
 
 namespace mono {
