@@ -492,7 +492,7 @@ typedef struct {
   void* out;           /* bf16 or f32 [rows, n], rows out_stride elements apart; no element of x */
   int64_t out_stride;  /* a multiple of 8; out itself 16-byte aligned */
   int32_t out_f32;     /* 0: bf16 */
-  int64_t rows;        /* 0..1048576 */
+  int64_t rows;        /* 0..1048576; rows x k below 2^35 */
   int32_t n, k;        /* multiples of 16 and of 128, up to 65536 */
   void* workspace;
   int64_t workspace_bytes;
@@ -552,11 +552,11 @@ typedef struct {
   int64_t residual_stride;  /* a multiple of 8 */
   void* out;                /* bf16 [tokens, hidden] */
   int64_t out_stride;       /* a multiple of 8 */
-  int64_t tokens;           /* tokens x (picks + 1) up to 1048576 */
+  int64_t tokens;           /* tokens x (picks + 1) up to 1048576, tokens x hidden below 2^35 */
   int32_t picks;            /* picks a token, 1..64 */
   int32_t experts;          /* routed experts, 1..1024 */
   int32_t shared;           /* 1: expert id `experts` is the shared one (weight 1, every token) */
-  int32_t hidden, inter;    /* multiples of 128 */
+  int32_t hidden, inter;    /* multiples of 128, up to 65536 and 32768 */
   void* workspace;
   int64_t workspace_bytes;
 } mono_prompt_experts_args;

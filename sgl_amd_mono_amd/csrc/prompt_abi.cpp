@@ -71,11 +71,16 @@ int need_space(const void* ws, int64_t bytes, size_t least) {
   return need(ws, "workspace", 256);
 }
 
+int need_elements(int64_t rows, int k, const char* names) {
+  if (rows * k > MAX_ELEMENTS) return refuse("%s must be at most %lld, got %lld x %d", names, (long long)MAX_ELEMENTS, (long long)rows, k);
+  return MONO_OK;
+}
+
 int product_shape(int64_t rows, int32_t n, int32_t k) {
   if (int rc = need_rows(rows, "rows")) return rc;
   if (n < 16 || n % 16 || n > MAX_DIM) return refuse("n must be a multiple of 16 in [16, %d], got %d", MAX_DIM, n);
   if (k < BLK || k % BLK || k > MAX_DIM) return refuse("k must be a multiple of %d in [%d, %d], got %d", BLK, BLK, MAX_DIM, k);
-  return MONO_OK;
+  return need_elements(rows, k, "rows x k");
 }
 
 // A product's plan over its workspace: the rows' codes and scales, and its parts.
@@ -97,7 +102,7 @@ int experts_shape(const mono_prompt_experts_args& a) {
     return refuse("hidden must be a multiple of %d in [%d, %d], got %d", BLK, BLK, MAX_DIM, a.hidden);
   if (a.inter < BLK || a.inter % BLK || a.inter > MAX_DIM / 2)
     return refuse("inter must be a multiple of %d in [%d, %d], got %d", BLK, BLK, MAX_DIM / 2, a.inter);
-  return MONO_OK;
+  return need_elements(a.tokens, a.hidden, "tokens x hidden");
 }
 
 // Where the wide tiles take over: picks that a routed expert gets on average (256 experts

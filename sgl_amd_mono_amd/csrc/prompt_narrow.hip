@@ -70,7 +70,7 @@ MONO_DEV void accumulate(const uint8_t* const (&wp)[NT], const float* const (&sp
         sx[u][j] = xsp[j][(size_t)b * xs_ld];
       }
     }
-    #pragma unroll
+#pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < NT; ++i)

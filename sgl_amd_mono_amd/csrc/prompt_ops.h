@@ -14,6 +14,7 @@ constexpr int BLK = 128;             // a scale's block of rows' and weights' co
 constexpr int MAX_EXPERTS = 1024;    // routed experts (a sort block each)
 constexpr int MAX_DIM = 1 << 16;     // columns and outputs of a product
 constexpr int64_t MAX_ROWS = 1 << 20;  // rows a call; picks of all rows of an experts call
+constexpr int64_t MAX_ELEMENTS = (1ll << 35) - 1;  // of the rows (a launch's threads, 16 a block, fit 32 bits)
 
 constexpr int LATENT = 512, PE = 64, INDEX = 128, PAGE = 64;
 

@@ -199,6 +199,7 @@ struct WideTile {
     const int last = kbs - 1;
     Ahead a0, a1, a2;
     issue(0, s0, a0);
+    __builtin_amdgcn_sched_barrier(0);  // (arrive counts loads: none of these goes out before the stage above)
     issue(min(1, last), s1, a1);
     int kb = 0;
     for (; kb + 2 < kbs; kb += 3) {

@@ -75,11 +75,12 @@ def test_product_of_small_integers_is_exact(gpu_device, m, n):
     assert torch.equal(got.cpu().double(), x.cpu().double() @ full.cpu().T)
 
 
-def test_product_strided_rows_and_out(gpu_device):
-    m, n, k = 77, 192, 384
+@pytest.mark.parametrize("m", [9, 30, 77, 200, 4500])
+def test_product_strided_rows_and_out(gpu_device, m):
+    n, k = 2112 if m > 4000 else 192, 384  # (4500 rows: tiles of 128)
     w, s = _matrix(n, k, gpu_device, 3)
     wide = workloads.rows_bf16(m, k + 64, gpu_device, seed=4)
-    buf = torch.full((m + 2, n + 48), 3.0, dtype=torch.bfloat16, device=gpu_device)
+    buf = torch.full((m + 2, n + 48), 3.0, dtype=torch.bfloat16, device=gpu_device)  # what lies around out stays
     got = prompt.product(wide[:, 64:], w, s, out=buf[1:-1, 16:-32])
     assert torch.equal(got, prompt.product(wide[:, 64:].contiguous(), w, s))
     assert bool((buf[0] == 3).all()) and bool((buf[-1] == 3).all())
@@ -323,6 +324,27 @@ def test_experts_odd_picks(gpu_device, t):
     c = dict(_experts_case(gpu_device, t, 256, 128, 8, 4, shared=False), residual=None)
     c["ids"][:] = 8
     assert bool((prompt.experts(**c) == 0).all())
+
+
+@pytest.mark.parametrize("counts", [(16, 17, 1, 30), (32, 33, 0, 64), (65, 1, 0, 62), (128, 129, 64, 65), (256, 0, 1, 257)])
+def test_experts_tile_borders(gpu_device, counts):
+    """Experts whose rows end on, before and behind a tile's last one, and experts without any."""
+    t = sum(counts)
+    c = _experts_case(gpu_device, t, 256, 128, len(counts), 1)
+    order = torch.randperm(t, generator=torch.Generator().manual_seed(t)).to(gpu_device)
+    c["ids"] = torch.cat([torch.full((n,), e) for e, n in enumerate(counts)]).int().to(gpu_device)[order][:, None].contiguous()
+    _check_experts(c, prompt.experts(**c))
+
+
+@pytest.mark.parametrize("t", [33, 500])
+def test_experts_ids_anywhere(gpu_device, t):
+    """Ids and weights that are contiguous and lie at any element (not 16-byte aligned)."""
+    c = _experts_case(gpu_device, t, 256, 128, 8, 3)
+    want = prompt.experts(**c)
+    for off in (1, 2, 3):
+        ids = torch.zeros(t * 3 + 4, dtype=torch.int32, device=gpu_device)[off:off + t * 3].view(t, 3)
+        wts = torch.zeros(t * 3 + 4, device=gpu_device)[off:off + t * 3].view(t, 3)
+        assert torch.equal(prompt.experts(**dict(c, ids=ids.copy_(c["ids"]), weights=wts.copy_(c["weights"]))), want)
 
 
 def test_experts_strided_in_place(gpu_device):

@@ -27,6 +27,7 @@ def _product(**kw):
     (dict(x=P + 8), "x must be 16-byte"), (dict(w=None), "w must"), (dict(s=None), "s must"), (dict(out=None), "out must"),
     (dict(x_stride=255), "x_stride"), (dict(x_stride=128), "x_stride"), (dict(out_stride=60), "out_stride"),
     (dict(workspace=None), "workspace"), (dict(workspace_bytes=100), "workspace must hold"), (dict(workspace=P + 16), "workspace"),
+    (dict(rows=1 << 20, k=1 << 15), "rows x k must be at most 34359738367"),
 ])  # fmt: skip
 def test_product_refusals(kw, what):
     with pytest.raises(ValueError, match=what):
@@ -83,6 +84,7 @@ def _experts(**kw):
     (dict(x_stride=250), "x_stride"), (dict(residual_stride=128), "residual_stride"), (dict(residual=P + 2), "residual"),
     (dict(ids=None), "ids"), (dict(weights=None), "weights"), (dict(w13=None), "w13"), (dict(s2=None), "s2"),
     (dict(out=P + 8), "out must"), (dict(workspace_bytes=0), "workspace"),
+    (dict(tokens=1 << 19, picks=1, hidden=1 << 16), "tokens x hidden"),
 ])  # fmt: skip
 def test_experts_refusals(kw, what):
     with pytest.raises(ValueError, match=what):
