@@ -49,7 +49,7 @@ def _same(got, want, mag, f32, k):
                                    (63, 64, 256), (65, 2112, 512), (129, 400, 1152), (300, 1536, 640),
                                    # the borders of each way to run: few rows, K shared out, tiles of 64 and 128 rows
                                    (16, 64, 2048), (17, 64, 2048), (16, 64, 2176), (4, 32, 8192), (5, 32, 8192), (45, 144, 7168),
-                                   (96, 16, 4096), (97, 16, 4096), (300, 528, 4096), (2050, 4112, 256)])
+                                   (96, 16, 4096), (97, 16, 4096), (300, 528, 4096), (2050, 4112, 256), (4100, 16, 128)])
 def test_product(gpu_device, m, n, k, f32):
     w, s = _matrix(n, k, gpu_device, 1)
     x = workloads.rows_bf16(m, k, gpu_device, seed=2)
@@ -295,7 +295,9 @@ def _check_experts(c, got):
                                        (130, 512, 128, 3, 2), (300, 256, 256, 33, 4), (700, 128, 128, 2, 1),
                                        # wide and narrow tiles over every number of mid blocks up to one too many for LDS
                                        (200, 384, 384, 4, 2), (150, 128, 512, 5, 2), (150, 1152, 640, 3, 2), (30, 384, 512, 4, 3),
-                                       (30, 128, 640, 4, 3), (3, 640, 768, 9, 2)])
+                                       (30, 128, 640, 4, 3), (3, 640, 768, 9, 2),
+                                       # as many experts and picks as a call takes, narrow and wide
+                                       (9, 128, 128, 1024, 64), (150, 128, 128, 1024, 64)])
 def test_experts(gpu_device, t, h, i, e, k):
     c = _experts_case(gpu_device, t, h, i, e, k)
     _check_experts(c, prompt.experts(**c))
