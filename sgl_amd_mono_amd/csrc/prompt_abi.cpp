@@ -106,11 +106,11 @@ int experts_shape(const mono_prompt_experts_args& a) {
 }
 
 // Where the wide tiles take over: picks that a routed expert gets on average (256 experts
-// of 7168 x 512, 8 picks a token, narrow / wide us: 128 tokens 424 / 453, 256 tokens 514 /
-// 496, 512 tokens 652 / 558). Never for a few tokens: the narrow up products widen their
+// of 7168 x 512, 8 picks a token, narrow / wide us: 128 tokens 391 / 433, 256 tokens 492 /
+// 496, 320 tokens 510 / 519, 384 tokens 554 / 538, 512 tokens 643 / 576). Never for a few tokens: the narrow up products widen their
 // codes to bf16, whose MFMA is exact where the FP8 one rounds, and a mid that falls over a
 // code's border shows most where few tokens share the error.
-constexpr int WIDE_PICKS = 7, FEW_TOKENS = 64;
+constexpr int WIDE_PICKS = 11, FEW_TOKENS = 64;
 
 // The call's plan over its workspace; `e.tiles` bounds the tile list.
 size_t experts_plan(const mono_prompt_experts_args& a, void* ws, Experts& e) {

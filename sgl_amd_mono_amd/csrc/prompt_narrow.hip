@@ -2,19 +2,20 @@
 // columns of sx[m, b] sw[n / 128, b] (xq[m, b] . wq[n, b]).
 //
 // The weights' bytes bound these: every one is read once for a few rows. A workgroup holds
-// 16 (or 16 gate and 16 up) weight rows and up to 64 rows of x; its 8 waves take the blocks
-// of K in turn, so that together they read 16 KB runs of each 16 weight rows, each
-// multiplies E4M3 codes on the MFMA and adds the f32 partial times sx sw to its sums, and
-// the waves' sums meet in LDS in wave order. The weights are the MFMA's A operand: a lane
-// then holds 4 consecutive outputs of one row, and one sx. The rows come from L2 straight
-// into registers: against the weights they are few.
+// 16 (or 16 gate and 16 up) weight rows and up to 64 rows of x; its 8 waves (4 for the
+// experts' up products) take the blocks of K in turn, so that together they read 16 KB runs
+// of each 16 weight rows, each multiplies E4M3 codes on the MFMA and adds the f32 partial
+// times sx sw to its sums, and the waves' sums meet in LDS in wave order. The weights are the
+// MFMA's A operand: a lane then holds 4 consecutive outputs of one row, and one sx. The rows
+// come from L2 straight into registers: against the weights they are few.
 //
-// Measured (256 experts of 7168 x 512, 8 picks a token): up products of 61 tokens 213 us, 7
-// TB/s; their down products 103 us, 7 TB/s (496 us with K shared out among the waves, which
-// leaves each wave half a block of its own). One token's up products take 17 us: 288
-// workgroups are one round over the CUs and an eighth of another. Tiles of 16 rows alone
-// need half the registers, and two workgroups a CU were slower from 2 tokens on (8 tokens
-// 137 against 128 us in all).
+// Measured (256 experts of 7168 x 512, 8 picks a token): up products of 61 tokens 197 us, 7.6
+// TB/s (8 waves, of which a CU's registers hold one workgroup, 213); their down products 103
+// us, 7 TB/s (496 us with K shared out among the waves, which leaves each wave half a block
+// of its own). One token's up products take 15 us, 4.4 TB/s (8 waves 17.5: its 288
+// workgroups were one round over the CUs and an eighth of another); in all 34 us a call for
+// 37, 8 tokens 122 for 128, 128 tokens 398 for 425. Tiles of 16 rows alone need half the
+// registers, and four workgroups a CU were slower from 3 tokens on (8 tokens 127).
 #include "prompt_common.h"
 
 namespace mono {
@@ -47,11 +48,11 @@ MONO_DEV i32x8 ld_pair(const uint8_t* p, size_t far) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// The wave's share of K (blocks kb0 + wave, + 8, .. below kb) of NT x MT tiles of 16 x 16.
-template <bool F32, int NT, int MT>
+// The wave's share of K (blocks kb0 + wave, + WV, .. below kb) of NT x MT tiles of 16 x 16.
+template <bool F32, int WV, int NT, int MT>
 MONO_DEV void accumulate(const uint8_t* const (&wp)[NT], const float* const (&sp)[NT], const uint8_t* const (&xp)[MT],
                          const float* const (&xsp)[MT], int xs_ld, int kb0, int kb, int wave, f32x4 (&acc)[NT][MT]) {
-  constexpr int U = MT == 4 ? 2 : 4;
+  constexpr int U = MT == 4 ? 2 : NT == 2 ? 3 : 4;
   for (int b0 = kb0 + wave; b0 < kb; b0 += WV * U) {
     i32x8 wv[U][NT], xv[U][MT];
     float sw[U][NT], sx[U][MT];
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(T) void k_few(const uint16_t* x, int64_t stride, in
     *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + at) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
 }
 
-template <int MODE, int NT, int MT>
+template <int MODE, int WV, int NT, int MT>
 MONO_DEV void narrow_tile(const Narrow& a, f32x4* red, const uint8_t* w, const float* s, int n0, int64_t first, int count,
                           int kb0, int kb1) {
   const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
@@ -158,7 +159,7 @@ MONO_DEV void narrow_tile(const Narrow& a, f32x4* red, const uint8_t* w, const f
     xsp[j] = a.xs + row;
   }
   f32x4 acc[NT][MT] = {};
-  accumulate<MODE != DENSE_BF16, NT, MT>(wp, sp, xp, xsp, a.xs_ld, kb0, kb1, wave, acc);
+  accumulate<MODE != DENSE_BF16, WV, NT, MT>(wp, sp, xp, xsp, a.xs_ld, kb0, kb1, wave, acc);
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -185,8 +186,8 @@ MONO_DEV void narrow_tile(const Narrow& a, f32x4* red, const uint8_t* w, const f
     *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = y[0];
 }
 
-template <int MODE>
-__global__ __launch_bounds__(T) void k_narrow(Narrow a) {
+template <int MODE, int WV>
+__global__ __launch_bounds__(WV * WAVE, 2) void k_narrow(Narrow a) {
   constexpr int NT = MODE == UP ? 2 : 1;
   __shared__ f32x4 red[WV * NT * 4 * WAVE];
   const int n0 = blockIdx.x * 16;
@@ -204,11 +205,11 @@ __global__ __launch_bounds__(T) void k_narrow(Narrow a) {
     s += (size_t)t.expert * ((a.n + BLK - 1) / BLK) * a.kb;
   }
   if (count <= 16)
-    narrow_tile<MODE, NT, 1>(a, red, w, s, n0, first, count, kb0, kb1);
+    narrow_tile<MODE, WV, NT, 1>(a, red, w, s, n0, first, count, kb0, kb1);
   else if (count <= 32)
-    narrow_tile<MODE, NT, 2>(a, red, w, s, n0, first, count, kb0, kb1);
+    narrow_tile<MODE, WV, NT, 2>(a, red, w, s, n0, first, count, kb0, kb1);
   else
-    narrow_tile<MODE, NT, 4>(a, red, w, s, n0, first, count, kb0, kb1);
+    narrow_tile<MODE, WV, NT, 4>(a, red, w, s, n0, first, count, kb0, kb1);
 }
 
 // The experts' down products: K is the mids' few blocks, so the waves share out the weight
@@ -315,16 +316,16 @@ hipError_t narrow_product(const Product& p, hipStream_t st) {
   Narrow a{p.q.q, p.q.s, p.q.ld, p.w, p.s, p.n, p.k / BLK, p.rows, p.out, p.out_stride, nullptr, nullptr, 0, p.part, p.plan.splits};
   const dim3 grid(p.n / 16, (uint32_t)((p.rows + BM - 1) / BM), p.plan.splits);
   if (p.f32)
-    k_narrow<DENSE_F32><<<grid, T, 0, st>>>(a);
+    k_narrow<DENSE_F32, WV><<<grid, T, 0, st>>>(a);
   else
-    k_narrow<DENSE_BF16><<<grid, T, 0, st>>>(a);
+    k_narrow<DENSE_BF16, WV><<<grid, T, 0, st>>>(a);
   return hipGetLastError();
 }
 
 hipError_t experts_up(const Experts& e, hipStream_t st) {
   Narrow a{e.x.q, e.x.s, e.x.ld, e.w13, e.s13, 2 * e.inter, e.hidden / BLK, 0, e.mid, e.inter,
            e.sorted.tiles, e.sorted.token, e.inter};
-  k_narrow<UP><<<dim3(e.inter / 16, e.tiles), T, 0, st>>>(a);
+  k_narrow<UP, 4><<<dim3(e.inter / 16, e.tiles), 4 * WAVE, 0, st>>>(a);
   return hipGetLastError();
 }
 

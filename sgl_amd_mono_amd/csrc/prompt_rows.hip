@@ -123,6 +123,8 @@ __global__ __launch_bounds__(128) void k_back(Experts a) {
   float y[8], v[U][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = 0.f;
+  u32x4 r = {0u, 0u, 0u, 0u};  // (on its way before the places are waited for)
+  if (a.residual) r = ld_u32x4(static_cast<const uint16_t*>(a.residual) + (int64_t)t * a.residual_stride + c);
   if (a.shared) load_part(a.part, a.picks + t, c, y);
   for (int j0 = 0; j0 < a.picks_each; j0 += U) {
     float w[U];
@@ -141,10 +143,12 @@ __global__ __launch_bounds__(128) void k_back(Experts a) {
       for (int i = 0; i < 8; ++i) y[i] = fmaf(w[u], v[u][i], y[i]);
   }
   if (a.residual) {
-    float r[8];
-    load8(static_cast<const uint16_t*>(a.residual) + (int64_t)t * a.residual_stride + c, r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] += r[i];
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = r[i];
+      y[2 * i] += bf16_lo(u);
+      y[2 * i + 1] += bf16_hi(u);
+    }
   }
   *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + (int64_t)t * a.out_stride + c) =
       u32x4{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7])};

@@ -297,7 +297,7 @@ def _check_experts(c, got):
                                        (200, 384, 384, 4, 2), (150, 128, 512, 5, 2), (150, 1152, 640, 3, 2), (30, 384, 512, 4, 3),
                                        (30, 128, 640, 4, 3), (3, 640, 768, 9, 2),
                                        # as many experts and picks as a call takes, narrow and wide
-                                       (9, 128, 128, 1024, 64), (150, 128, 128, 1024, 64)])
+                                       (9, 128, 128, 1024, 64), (150, 128, 128, 1024, 64), (200, 128, 128, 1024, 64)])
 def test_experts(gpu_device, t, h, i, e, k):
     c = _experts_case(gpu_device, t, h, i, e, k)
     _check_experts(c, prompt.experts(**c))
