@@ -126,15 +126,25 @@ MONO_DEV uint32_t groups_umax(uint32_t v) {
 }
 
 // A lane's 16 of one place's 64 columns (tiles of 16 weight rows i, columns 16 i + 4 g + e of
-// lane group g) as halves of a Parts block: the scale, and the values divided by it. (The
-// float maximum passes over a NaN, which stays one as a half.)
+// lane group g) as halves of a Parts block: the scale, and the values divided by it. The
+// scale is that of the largest finite value, so a sum past f32's range is an infinity in its
+// own column and costs the other 63 nothing. (The float maximum passes over a NaN, which
+// stays one as a half.)
 MONO_DEV float part_block(const f32x4 (&y)[4], u32x2 (&h)[4]) {
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) top = fmaxf(fmaxf(top, fmaxf(fabsf(y[i][0]), fabsf(y[i][1]))), fmaxf(fabsf(y[i][2]), fabsf(y[i][3])));
-  const uint32_t m = groups_umax(__float_as_uint(top));
-  // 2^14 / 2^floor(log2 max); a block with an infinity keeps its values as they are
-  const int e = m < 0x7f800000u ? max((int)(m >> 23), 27) : 127 + 14;
+  uint32_t m = groups_umax(__float_as_uint(top));
+  if (__any(m >= 0x7f800000u)) {  // rare: the whole wave again without the infinities
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = fmaxf(top, abs_bits(y[i][j]) < 0x7f800000u ? fabsf(y[i][j]) : 0.f);
+    m = groups_umax(__float_as_uint(top));
+  }
+  // 2^14 / 2^floor(log2 max)
+  const int e = max((int)(m >> 23), 27);
   const float inv = __uint_as_float((uint32_t)(127 + 14 + 127 - e) << 23);
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = u32x2{pack_halves(y[i][0] * inv, y[i][1] * inv), pack_halves(y[i][2] * inv, y[i][3] * inv)};

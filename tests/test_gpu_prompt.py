@@ -384,6 +384,25 @@ def test_experts_non_finite_tokens(gpu_device):
         assert torch.equal(got[keep], want[keep])
 
 
+@pytest.mark.parametrize("t,h,i", [(20, 256, 128), (200, 256, 128), (20, 384, 640), (200, 384, 640)])
+def test_experts_infinite_sum_leaves_its_neighbours(gpu_device, t, h, i):
+    """A down product past f32's range is an infinity in its own column: the other columns,
+    far above f16's largest value, keep the bits that they have where that column's weights
+    are zero (narrow and wide tiles, mids in LDS and not)."""
+    c = _experts_case(gpu_device, t, h, i, 8, 2)
+    c["s2"] *= 2.0**122
+    clean, col = {}, 70
+    for code, to in ((0x7E, c), (0x00, clean)):  # every weight of the column 448, or zero
+        w2 = c["w2"].view(torch.uint8).clone().view(9, h // 16, i // 32, 2, 16, 16)
+        w2[:, col // 16, :, :, col % 16] = code
+        to["w2"] = w2.view(9, h, i)
+    got, want = prompt.experts(**c), prompt.experts(**dict(c, **clean))
+    keep = [n for n in range(h) if n != col]
+    assert not bool(got[:, col].isfinite().all()) and bool(want.isfinite().all())
+    assert float(want.float().abs().max()) > 2.0**110
+    assert torch.equal(got[:, keep], want[:, keep])
+
+
 def test_experts_of_no_tokens(gpu_device):
     c = _experts_case(gpu_device, 4, 256, 128, 8, 2)
     for k in ("x", "ids", "weights", "residual"):
