@@ -58,12 +58,12 @@ MONO_DEV void accumulate(const uint8_t* const (&wp)[NT], const float* const (&sp
     float sw[U][NT], sx[U][MT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int b = b0 + WV * u < kb ? b0 + WV * u : b0;  // past the end: the first again, scaled by zero
-      const float on = b0 + WV * u < kb ? 1.f : 0.f;
+      const bool in = b0 + WV * u < kb;
+      const int b = in ? b0 + WV * u : b0;  // past the end: the first again, its scale zero (whatever its own is)
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         wv[u][i] = ld_pair(wp[i] + (size_t)b * 2048, 1024);
-        sw[u][i] = sp[i][b] * on;
+        sw[u][i] = in ? sp[i][b] : 0.f;
       }
 #pragma unroll
       for (int j = 0; j < MT; ++j) {

@@ -117,6 +117,22 @@ def test_product_nan_weights_stay_in_their_output(gpu_device, m):
     assert torch.equal(got[:, keep], clean[:, keep])
 
 
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("m,k", [(3, 1280), (30, 1280), (30, 2304), (200, 1280)])
+def test_product_infinite_weight_scale(gpu_device, m, k, f32):
+    """A weight block whose scale is infinite makes its outputs infinite, with the sign of the
+    block's own sum, whichever way the product runs."""
+    n = 80
+    w, s = _matrix(n, k, gpu_device, 14)
+    x = workloads.rows_bf16(m, k, gpu_device, seed=15)
+    first = ref.rounded(x[:, :128].cpu()) @ ref.weight(w.cpu(), s.cpu())[:, :128].T
+    s[0, 0] = float("inf")
+    got = prompt.product(x, w, s, dtype=torch.float32 if f32 else torch.bfloat16).cpu().double()
+    clear = first.abs() > 2.0**-14 * 8.0 * first.abs().max()  # its sign hangs on no rounding of the block's sum
+    assert bool(got.isinf().all()) and torch.equal(got.sign()[clear], first.sign()[clear])
+    assert float(clear.float().mean()) > 0.9
+
+
 @pytest.mark.parametrize("m,stride", [(5, 1 << 29), (40, 1 << 26), (300, 1 << 23)])
 def test_product_rows_far_apart(gpu_device, m, stride):
     """Row offsets past 32 bits."""
