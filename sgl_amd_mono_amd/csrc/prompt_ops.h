@@ -14,7 +14,7 @@ constexpr int BLK = 128;             // a scale's block of rows' and weights' co
 constexpr int MAX_EXPERTS = 1024;    // routed experts (a sort block each)
 constexpr int MAX_DIM = 1 << 16;     // columns and outputs of a product
 constexpr int64_t MAX_ROWS = 1 << 20;  // rows a call; picks of all rows of an experts call
-constexpr int64_t MAX_ELEMENTS = (1ll << 35) - 1;  // of the rows (a launch's threads, 16 a block, fit 32 bits)
+constexpr int64_t MAX_ELEMENTS = (1ll << 35) - 1;  // of the rows of a product or an experts call
 
 constexpr int LATENT = 512, PE = 64, INDEX = 128, PAGE = 64;
 
@@ -56,6 +56,13 @@ struct Parts {
   float* s;
   int ld;
 };
+
+// Blocks that one launch rounds at most: 16 threads each in workgroups of 1024, and one such
+// workgroup more for each expert that sorts beside them. A launch's threads are counted in 32
+// bits; more rows take another launch.
+constexpr int64_t ROUND_BLOCKS = 1 << 27;
+static_assert(ROUND_BLOCKS * 16 + MAX_EXPERTS * 1024 < 1ll << 32, "a rounding launch's threads");
+static_assert(ROUND_BLOCKS >= MAX_DIM / BLK, "a launch rounds at least a row");
 
 hipError_t quant_rows(const void* x, bool f32, int64_t stride, int64_t rows, int k, const Rows& out, hipStream_t st);
 hipError_t sort_quant(const void* x, int64_t stride, int64_t tokens, int k, const Rows& out, const int* ids, int picks_each,

@@ -180,20 +180,29 @@ hipError_t join_product(const Product& a, hipStream_t st) {
 }
 
 hipError_t quant_rows(const void* x, bool f32, int64_t stride, int64_t rows, int k, const Rows& out, hipStream_t st) {
-  const uint32_t n = (uint32_t)(rows * (k / BLK)), grid = (n + T / 16 - 1) / (T / 16);
-  if (f32)
-    k_quant_rows<<<grid, T, 0, st>>>(static_cast<const float*>(x), stride, n, k / BLK, out);
-  else
-    k_quant_rows<<<grid, T, 0, st>>>(static_cast<const uint16_t*>(x), stride, n, k / BLK, out);
-  return hipGetLastError();
+  const int kb = k / BLK;
+  const int64_t most = ROUND_BLOCKS / kb;
+  for (int64_t r = 0; r < rows; r += most) {
+    const uint32_t n = (uint32_t)((rows - r < most ? rows - r : most) * kb), grid = (n + T / 16 - 1) / (T / 16);
+    const Rows to{out.q + (size_t)r * k, out.s + r, out.ld};
+    if (f32)
+      k_quant_rows<<<grid, T, 0, st>>>(static_cast<const float*>(x) + r * stride, stride, n, kb, to);
+    else
+      k_quant_rows<<<grid, T, 0, st>>>(static_cast<const uint16_t*>(x) + r * stride, stride, n, kb, to);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t sort_quant(const void* x, int64_t stride, int64_t tokens, int k, const Rows& out, const int* ids, int picks_each,
                       int experts, bool shared, int bm, const Sorted& sorted, hipStream_t st) {
-  const uint32_t n = (uint32_t)(tokens * (k / BLK)), grid = experts + (n + T / 16 - 1) / (T / 16);
-  k_sort_quant<<<grid, T, 0, st>>>(static_cast<const uint16_t*>(x), stride, n, k / BLK, out, ids, (int)tokens, picks_each,
-                                   experts, shared, bm, sorted);
-  return hipGetLastError();
+  const int kb = k / BLK;
+  const int64_t most = ROUND_BLOCKS / kb, here = tokens < most ? tokens : most;
+  const uint32_t n = (uint32_t)(here * kb), grid = experts + (n + T / 16 - 1) / (T / 16);
+  const uint16_t* rows = static_cast<const uint16_t*>(x);
+  k_sort_quant<<<grid, T, 0, st>>>(rows, stride, n, kb, out, ids, (int)tokens, picks_each, experts, shared, bm, sorted);
+  if (hipError_t e = hipGetLastError()) return e;
+  return quant_rows(rows + here * stride, false, stride, tokens - here, k, Rows{out.q + (size_t)here * k, out.s + here, out.ld}, st);
 }
 
 hipError_t experts_back(const Experts& a, hipStream_t st) {

@@ -144,6 +144,21 @@ def test_product_rows_far_apart(gpu_device, m, stride):
     assert torch.equal(prompt.product(far, w, s), prompt.product(x, w, s))
 
 
+def test_product_of_the_most_elements(gpu_device):
+    """As many elements as a call takes: their rounding needs more threads than one launch has
+    (rows around the borders of its launches, 262656 rows each, against 64 bits)."""
+    n, m, k = 16, 525314, 65408
+    torch.cuda.empty_cache()
+    w, s = _matrix(n, k, gpu_device, 16)
+    x = torch.empty(m, k, dtype=torch.bfloat16, device=gpu_device)  # (what lies in the other rows is theirs)
+    at = [0, 1, 262655, 262656, 393985, 525311, 525312, 525313]
+    x[at] = workloads.rows_bf16(len(at), k, gpu_device, seed=17)
+    got = prompt.product(x, w, s)[at]
+    x = x[at].cpu()
+    torch.cuda.empty_cache()
+    _same(got, *ref.product(x, w.cpu(), s.cpu()), False, k)
+
+
 def test_product_refuses_shared_memory(gpu_device):
     w, s = _matrix(256, 256, gpu_device, 12)
     x = workloads.rows_bf16(4, 512, gpu_device, seed=13)
@@ -417,6 +432,21 @@ def test_experts_infinite_sum_leaves_its_neighbours(gpu_device, t, h, i):
     assert not bool(got[:, col].isfinite().all()) and bool(want.isfinite().all())
     assert float(want.float().abs().max()) > 2.0**110
     assert torch.equal(got[:, keep], want[:, keep])
+
+
+def test_experts_of_the_most_elements(gpu_device):
+    """As many elements as a call takes: rows past the rounding that is launched beside the
+    sort (262144 of them) against 64 bits."""
+    t, h, at = (1 << 19) - 1, 1 << 16, [0, 262143, 262144, 262145, 524286]
+    c = dict(_experts_case(gpu_device, len(at), h, 128, 2, 1, shared=False), residual=None)
+    torch.cuda.empty_cache()
+    x = torch.empty(t, h, dtype=torch.bfloat16, device=gpu_device)  # (what lies in the other rows is theirs)
+    ids, wts = torch.ones(t, 1, dtype=torch.int32, device=gpu_device), torch.ones(t, 1, device=gpu_device)
+    x[at], ids[at], wts[at] = c["x"], c["ids"], c["weights"]
+    got = prompt.experts(**dict(c, x=x, ids=ids, weights=wts, out=x))[at]
+    del x
+    torch.cuda.empty_cache()
+    _check_experts(dict(c, residual=torch.zeros_like(c["x"])), got)
 
 
 def test_experts_of_no_tokens(gpu_device):
