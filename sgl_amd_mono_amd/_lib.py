@@ -110,7 +110,8 @@ class PromptExpertsArgs(C.Structure):
     _fields_ = [("x", _VP), ("x_stride", _I64), ("ids", _VP), ("weights", _VP), ("w13", _VP), ("s13", _VP),
                 ("w2", _VP), ("s2", _VP), ("residual", _VP), ("residual_stride", _I64), ("out", _VP),
                 ("out_stride", _I64), ("tokens", _I64), ("picks", _I32), ("experts", _I32), ("shared", _I32),
-                ("hidden", _I32), ("inter", _I32), ("workspace", _VP), ("workspace_bytes", _I64)]
+                ("hidden", _I32), ("inter", _I32), ("batch_invariant", _I32), ("workspace", _VP),
+                ("workspace_bytes", _I64)]
 
 
 # the phase boundaries a one-launch layer stamps per workgroup (mono_layer_args.ticks)

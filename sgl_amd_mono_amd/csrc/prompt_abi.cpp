@@ -105,18 +105,32 @@ int experts_shape(const mono_prompt_experts_args& a) {
   return need_elements(a.tokens, a.hidden, "tokens x hidden");
 }
 
-// Where the wide tiles take over: picks that a routed expert gets on average (256 experts
-// of 7168 x 512, 8 picks a token, narrow / wide us: 128 tokens 391 / 433, 256 tokens 492 /
-// 496, 320 tokens 510 / 519, 384 tokens 554 / 538, 512 tokens 643 / 576). Never for a few tokens: the narrow up products widen their
-// codes to bf16, whose MFMA is exact where the FP8 one rounds, and a mid that falls over a
-// code's border shows most where few tokens share the error.
-constexpr int WIDE_PICKS = 11, FEW_TOKENS = 64;
+// Where the wide tiles take over, by time alone: above FEW_TOKENS tokens with more than
+// WIDE_PICKS picks a routed expert on average. Narrow / wide, us a call in a graph:
+//
+//   hidden x inter, experts, picks   64 tokens   96 tokens   128 tokens  256 tokens  512 tokens
+//   7168 x 512, 256, 8               425 / 452   462 / 509   463 / 495   504 / 544   599 / 571
+//   7168 x 1024, 64, 8               270 / 290   280 / 296   300 / 298   449 / 310   655 / 351
+//   7168 x 2048, 64, 8               523 / 520   541 / 532   574 / 537   827 / 554   1218 / 615
+//   7168 x 2048, 16, 4               176 / 180   205 / 192   249 / 194   379 / 213   584 / 281
+//   7168 x 512, 32, 8                103 / 101   124 / 127   147 / 132   211 / 139   329 / 179
+//   7168 x 512, 8, 4                  64 / 55     67 / 87     74 / 90    111 / 95    175 / 101
+//   2048 x 512, 16, 4                 40 / 37     43 / 54     44 / 56     55 / 56     70 / 59
+//   1024 x 128, 8, 2                  21 / 27     21 / 38     21 / 40     23 / 40     25 / 42
+//
+// The two differ in their up products' sums as well: the narrow ones widen the codes to bf16,
+// which costs nothing beside the weights' bytes and makes every product exact, the wide ones
+// take the FP8 MFMA's 1.4e-5, as the decode launch does. A mid that this carries over a code's
+// border moves by a code, so outputs are 0.0017 and 0.0020 of their norm from 64 bits. A
+// caller who wants a token's bits to be its own in any company asks for the narrow tiles (the
+// first geometry: 1500 tokens 1036 us for 685, 8192 tokens 4235 for 1595).
+constexpr int WIDE_PICKS = 11, FEW_TOKENS = 96;
 
 // The call's plan over its workspace; `e.tiles` bounds the tile list.
 size_t experts_plan(const mono_prompt_experts_args& a, void* ws, Experts& e) {
   Space sp{static_cast<char*>(ws)};
   const int64_t picks = a.tokens * a.picks, places = picks + (a.shared ? a.tokens : 0);
-  e.wide = a.tokens > FEW_TOKENS && picks > (int64_t)WIDE_PICKS * a.experts;
+  e.wide = !a.batch_invariant && a.tokens > FEW_TOKENS && picks > (int64_t)WIDE_PICKS * a.experts;
   e.bm = e.wide ? 128 : 64;
   e.tiles = (int)all_tiles(a.tokens, picks, a.experts, e.bm, a.shared);
   e.x = sp.rows(a.tokens, a.hidden);

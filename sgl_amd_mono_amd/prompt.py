@@ -186,13 +186,18 @@ def append(kv_a: torch.Tensor, ik: torch.Tensor, req: torch.Tensor, pos: torch.T
 
 def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: torch.Tensor, s13: torch.Tensor,
             w2: torch.Tensor, s2: torch.Tensor, residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
-            shared: bool = True) -> torch.Tensor:
+            shared: bool = True, batch_invariant: bool = False) -> torch.Tensor:
     """``residual[t] + shared(x[t]) + sum_j weights[t, j] * expert_ids[t, j](x[t])``, bf16
     [tokens, H]. ``x`` [tokens, H] bf16 are the normed rows, ``ids`` i32 and ``weights``
     f32 [tokens, picks] the router's answer (an id outside the routed experts is routed
     nowhere), the weights and scales those of ``moe.Fp8MoeWeights``. With ``shared`` the
     last expert is the shared one (every token, weight 1) and ids name the others. Rows of
-    ``x``, ``residual`` and ``out`` may lie apart; ``out`` may be ``residual`` or ``x`` itself."""
+    ``x``, ``residual`` and ``out`` may lie apart; ``out`` may be ``residual`` or ``x`` itself.
+
+    Wide calls (above 96 tokens with more than 11 picks a routed expert on average) sum their
+    up products on the FP8 MFMA, 1.4e-5 off for each 128 of them, narrower ones exactly but
+    for f32's rounding. With ``batch_invariant`` every call does as the narrower ones do: a
+    token's output then has the same bits whatever other tokens are in the call."""
     dev = _gpu(x, "x")
     if x.dim() != 2 or not isinstance(ids, torch.Tensor) or ids.dim() != 2:
         raise ValueError(f"x and ids: expected [tokens, H] and [tokens, picks], got {tuple(x.shape)} and "
@@ -219,7 +224,7 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: torc
         x=x.data_ptr(), x_stride=x_stride, ids=ids.data_ptr(), weights=weights.data_ptr(), w13=w13.data_ptr(),
         s13=s13.data_ptr(), w2=w2.data_ptr(), s2=s2.data_ptr(), residual=_lib.ptr(residual), residual_stride=res_stride,
         out=out.data_ptr(), out_stride=out_stride, tokens=t, picks=k, experts=e - bool(shared), shared=bool(shared),
-        hidden=h, inter=i,
+        hidden=h, inter=i, batch_invariant=bool(batch_invariant),
     )  # fmt: skip
     lib = _lib.lib()
     ws = _workspace(args, lib.mono_prompt_experts_workspace(C.byref(args)), dev)  # noqa: F841 (held over the call)

@@ -449,6 +449,24 @@ def test_experts_of_the_most_elements(gpu_device):
     _check_experts(dict(c, residual=torch.zeros_like(c["x"])), got)
 
 
+@pytest.mark.parametrize("h,i,e,k", [(256, 128, 8, 2), (1152, 384, 3, 2), (512, 640, 4, 3), (2432, 512, 6, 1)])
+def test_experts_batch_invariant(gpu_device, h, i, e, k):
+    """A token's output has the same bits alone, in the smallest and the widest company, and in
+    another place of the call; and it is right."""
+    c = dict(_experts_case(gpu_device, 600, h, i, e, k), batch_invariant=True)
+    c["ids"][5] = -1
+    rows = ("x", "ids", "weights", "residual")
+    want = prompt.experts(**c)
+    _check_experts({n: v for n, v in c.items() if n != "batch_invariant"}, want)
+    order = torch.randperm(600, generator=torch.Generator().manual_seed(h)).to(gpu_device)
+    assert torch.equal(prompt.experts(**dict(c, **{n: c[n][order] for n in rows})), want[order])
+    for first, n in [(0, 1), (7, 16), (3, 17), (100, 64), (100, 65), (90, 97), (1, 300)]:
+        part = {r: c[r][first:first + n].contiguous() for r in rows}
+        assert torch.equal(prompt.experts(**dict(c, **part)), want[first:first + n]), (first, n)
+        if n <= 96:  # calls this small sum so in any case
+            assert torch.equal(prompt.experts(**dict(c, batch_invariant=False, **part)), want[first:first + n])
+
+
 def test_experts_of_no_tokens(gpu_device):
     c = _experts_case(gpu_device, 4, 256, 128, 8, 2)
     for k in ("x", "ids", "weights", "residual"):
