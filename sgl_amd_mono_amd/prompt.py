@@ -1,10 +1,11 @@
 """The layer's work at prompt widths: any number of rows on the layer's own weights and
 caches, where the decode launches take a step of a few.
 
-* ``product``: rows times one FP8 matrix with a scale for each 128 x 128 block (the
-  projections that ``layer.ProjRuntime`` runs for a decode step)
+* ``product``: rows, rounded to E4M3, times one FP8 matrix with a scale for each 128 x 128
+  block: the projections' weights as they are. (``layer.ProjRuntime`` multiplies a decode
+  step's rows in bf16, unrounded: a projection of ``product`` is 2.6 % of its norm off that.)
 * ``append``: a prompt's keys into the MLA cache and the index plane (what the front
-  launch writes for a decode step's rows)
+  launch writes for a decode step's rows, from the same projections)
 * ``experts``: the routed and the shared FP8 experts (the products of
   ``moe.MoeRuntime.forward_fp8``, behind a router of the caller's)
 
@@ -113,7 +114,8 @@ def product(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, out: torch.Tensor
     """``x`` [rows, K] bf16 (rows may lie apart, each 16-byte aligned) times ``w`` [N, K]
     E4M3 in the (16, 16) layout with scales ``s`` f32 [ceil(N / 128), K / 128] -> [rows, N]
     in ``dtype`` (bf16 or f32; ``out``'s own where that is given). The rows are rounded to
-    E4M3 with a scale for each 128 columns; a row that holds a NaN or an infinity has NaN
+    E4M3 with a scale for each 128 columns, whatever ``dtype`` (the decode launches round
+    none of a projection's); a row that holds a NaN or an infinity has NaN
     outputs. N % 16 == 0, K % 128 == 0. ``out`` must share no memory with ``x``."""
     dev = _gpu(x, "x")
     if x.dim() != 2 or not isinstance(w, torch.Tensor) or w.dim() != 2:
