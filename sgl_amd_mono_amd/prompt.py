@@ -124,7 +124,10 @@ def product(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, out: torch.Tensor
     stride = _rows(x, "x", (m, k), torch.bfloat16, dev)
     need(w, "w", (n, k), FP8_TYPES, dev)
     need(s, "s", (-(-n // 128), k // 128), torch.float32, dev)
-    dtype = dtype if out is None else out.dtype
+    if out is not None:
+        if not isinstance(out, torch.Tensor):
+            raise ValueError(f"out: expected a tensor, got {type(out).__name__}")
+        dtype = out.dtype
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"out: expected dtype torch.bfloat16 or torch.float32, got {dtype}")
     if out is None:
@@ -163,6 +166,8 @@ def append(kv_a: torch.Tensor, ik: torch.Tensor, req: torch.Tensor, pos: torch.T
     if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
         raise ValueError(f"page_table: expected [requests, pages], got {tuple(getattr(page_table, 'shape', ()))}")
     need(page_table, "page_table", tuple(page_table.shape), torch.int32, dev)
+    if not isinstance(caches.ikv, torch.Tensor) or caches.ikv.dim() != 4:
+        raise ValueError(f"ikv: expected [pages, 4, {PAGE}, 16], got {tuple(getattr(caches.ikv, 'shape', ()))}")
     pages = caches.ikv.shape[0]
     need(caches.ikv, "ikv", (pages, 4, PAGE, 16), torch.uint8, dev)
     need(caches.iks, "iks", (pages, 4, PAGE), torch.uint8, dev)

@@ -108,6 +108,20 @@ def test_cpu_tensors_are_refused():
         prompt.append(x, x, s, s, s, AttnCaches(w, w, w, None), s, s, s, s, s)
 
 
+def test_what_is_no_tensor_is_refused_by_name(monkeypatch):
+    monkeypatch.setattr(prompt, "_gpu", lambda t, name: t.device)  # the checks alone, on CPU tensors
+    bf16, f32, i32 = (dict(dtype=d) for d in (torch.bfloat16, torch.float32, torch.int32))
+    x, w, s = torch.zeros(2, 128, **bf16), torch.zeros(16, 128, dtype=torch.uint8), torch.zeros(1, 1)
+    for out in ([0], 1.5, "out"):
+        with pytest.raises(ValueError, match="out: expected a tensor"):
+            prompt.product(x, w, s, out=out)
+    kv_a, ik, at, table = torch.zeros(2, 576, **bf16), torch.zeros(2, 128, **bf16), torch.zeros(2, **i32), torch.zeros(1, 1, **i32)
+    rest = (torch.zeros(512, **bf16), torch.zeros(128, **f32), torch.zeros(128, **f32), torch.zeros(9, 32), torch.zeros(9, 32))
+    for ikv in (None, [1], torch.tensor(3)):
+        with pytest.raises(ValueError, match="ikv: expected"):
+            prompt.append(kv_a, ik, at, at, table, AttnCaches(ikv, w, w, None), *rest)
+
+
 def test_shared_memory_is_told_apart():
     wide = torch.zeros(6, 64, dtype=torch.bfloat16)
     a, b = wide[:, :32], wide[:, 32:]
