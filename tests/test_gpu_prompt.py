@@ -61,6 +61,24 @@ def test_product(gpu_device, m, n, k, f32):
     _same(got, want, mag, f32, k)
 
 
+@pytest.mark.parametrize("m,n,k", [(5, 64, 2048), (16, 2112, 2048),  # few rows, rounded in the workgroup
+                                   (20, 256, 640), (100, 64, 640), (45, 128, 7168), (96, 16, 4096),  # narrow; K shared out
+                                   (300, 1536, 640), (1025, 528, 1024), (300, 528, 4096), (200, 2112, 7168)])  # wide; shared out
+def test_product_f32_sums(gpu_device, m, n, k):
+    """The sums of an f32 product are f32's. A running sum over kb blocks is rounded kb times,
+    2^-24 of what it then is: sqrt(kb / 2) 2^-24 of the result in the mean, as the parts of a
+    sum of independent terms grow; the block's scales, its product's four steps and eight
+    waves' sums are 10 roundings at most of all of it: at kb = 56 within 16 x 2^-24 = 9.5e-7
+    of the norm. The FP8 MFMA's own sums are 1.4e-5 off."""
+    w, s = _matrix(n, k, gpu_device, 18)
+    x = workloads.rows_bf16(m, k, gpu_device, seed=19)
+    got = prompt.product(x, w, s, dtype=torch.float32).cpu().double()
+    want, _ = ref.product(x.cpu(), w.cpu(), s.cpu())
+    off = float((got - want).norm() / want.norm())
+    print(f"{off:.2e}", flush=True)
+    assert off <= 16 * 2.0**-24
+
+
 @pytest.mark.parametrize("m", [1, 15, 64, 200, 257, 530, 1025])
 @pytest.mark.parametrize("n", [16, 208, 256, 528])
 def test_product_of_small_integers_is_exact(gpu_device, m, n):
@@ -341,6 +359,37 @@ def test_experts_without_shared_or_residual(gpu_device):
     got = prompt.experts(**dict(c, residual=None))
     c["residual"] = torch.zeros_like(c["x"])
     _check_experts(c, got)
+
+
+@pytest.mark.parametrize("t,h,i,e,k", [(150, 1152, 128, 3, 2), (130, 2048, 256, 2, 1), (150, 2432, 384, 3, 2), (300, 7168, 512, 4, 2)])
+def test_experts_wide_columns(gpu_device, t, h, i, e, k):
+    """Wide calls whose mids stay in LDS over more columns than one workgroup takes: even and
+    uneven turns of columns, the last past the matrix, tiles of more rows than 64 and of fewer."""
+    c = _experts_case(gpu_device, t, h, i, e, k)
+    few = torch.rand(t, generator=torch.Generator().manual_seed(t)).to(gpu_device) < 0.2
+    c["ids"][:, 0] = torch.where(few, e - 1, 0).int()  # the last expert gets some, the first most
+    if k > 1:
+        c["ids"][:, 1] = 1
+    _check_experts(c, prompt.experts(**c))
+
+
+@pytest.mark.parametrize("invariant", [False, True])
+def test_experts_narrow_up_products_are_exact(gpu_device, invariant):
+    """Beside its own rounding to bf16, an output of the narrow tiles is off by the parts' f16
+    (2^-11 / sqrt(3) = 0.00028 of the norm) and by mids over a border: one that is 1e-6 off (f32
+    sums, a few last bits of the SiLU) crosses with the probability 1e-6 / step and moves by a
+    step of at most 2^-3 of itself, sqrt(1e-6 x 2^-3) = 0.00036 of the norm; together 0.00046.
+    The FP8 MFMA's 1.4e-5 makes it 0.001."""
+    t = 300 if invariant else 64
+    c = dict(_experts_case(gpu_device, t, 1024, 512, 2, 1, shared=False), residual=None)
+    c["weights"][:] = 1.0
+    got = prompt.experts(**c, batch_invariant=invariant).cpu().double()
+    cpu = {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+    want, _, _ = ref.experts(cpu["x"], cpu["ids"], cpu["weights"], cpu["w13"], cpu["s13"], cpu["w2"], cpu["s2"], shared=False)
+    own = want.float().to(torch.bfloat16).double() - want
+    off = float(((got - want).square().sum() - own.square().sum()).clamp_min(0).sqrt() / want.norm())
+    print(f"{off:.2e}", flush=True)
+    assert off <= 0.00046
 
 
 @pytest.mark.parametrize("t", [6, 90, 400])
@@ -635,3 +684,30 @@ def test_experts_against_the_decode_launch(gpu_device):
     d = (got.double() - want.double())
     assert float(d.norm()) <= 2 * 0.031 * float(y.norm()) + 2.0**-7 * float(want.double().norm())
     assert bool((d.abs() <= 6 * 2 * 0.031 * y.square().mean().sqrt() + 2.0**-7 * want.double().abs()).all())
+
+
+def test_experts_on_the_decode_launch_s_rows(gpu_device):
+    """As above, on rows that both sides round to the same codes: in every 8 columns one of
+    size 2, three of size 1 and four of 1/2, whose mean square is 1, so that the launch's norm
+    leaves them (5e-7 off, which a code of 448 / 2^j does not hang on), and with experts whose
+    sum outweighs the residual. What is left is the module's head's: mids over a border, and
+    the outputs' rounding."""
+    dev = gpu_device
+    w = workloads.fp8_moe_weights(FP8_MOE, dev, seed=43)
+    w.g_post.fill_(1.0)
+    w.s2 *= 4096.0
+    g = torch.Generator(device=dev).manual_seed(44)
+    size = torch.tensor([2.0, 1.0, 1.0, 1.0, 0.5, 0.5, 0.5, 0.5], device=dev)
+    order = torch.rand(8, FP8_MOE.hidden // 8, 8, generator=g, device=dev).argsort(-1)
+    sign = torch.randint(0, 2, (8, FP8_MOE.hidden), generator=g, device=dev) * 2 - 1
+    a = (size[order].view(8, -1) * sign).to(torch.bfloat16)
+    rt = MoeRuntime(FP8_MOE, 8, device=dev)
+    want, dbg = rt.forward_fp8(a, w, debug=True)
+    torch.cuda.synchronize()
+    rt.check_errors()
+    rt.close()
+    got = prompt.experts(a, dbg["topk_ids"], dbg["topk_w"], w.w13, w.s13, w.w2, w.s2, residual=a)
+    d, y = got.double() - want.double(), dbg["y"].double()
+    print(f"{float(d.norm() / want.double().norm()):.2e}", flush=True)
+    assert float(y.norm()) > 4 * float(a.double().norm())
+    assert float(d.norm()) <= 0.0056 * float(y.norm()) + 2.0**-8 * float(want.double().norm())
