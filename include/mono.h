@@ -473,7 +473,9 @@ int mono_layer_set_launch_ordinal(mono_layer* layer, uint64_t ordinal);
  * These calls keep no state and own no memory: each takes a workspace of the caller's
  * (256-byte aligned, at least what the _workspace function says, its content undefined
  * before and after) that nothing else may use until the call's work has ended on its
- * stream. Calls with workspaces and outputs of their own may run at once. Every launch
+ * stream. (A product: k bytes and k / 32 a row, and f32 parts where its tiles are few. An
+ * experts call: some 2.06 hidden + 1.04 inter bytes, 4 inter more in narrow tiles, for each
+ * pick and each token's shared expert: 1.2 GB for 8192 tokens of 7168 with 8 picks.) Calls with workspaces and outputs of their own may run at once. Every launch
  * goes to the current device, which must be the one that holds the tensors. A call of no
  * rows launches nothing and looks at no pointer. Results do not depend on what else runs
  * and are the same bit for bit from call to call.

@@ -9,13 +9,16 @@
 // MFMA's A operand: a lane then holds 4 consecutive outputs of one row, and one sx. The rows
 // come from L2 straight into registers: against the weights they are few.
 //
-// Measured (256 experts of 7168 x 512, 8 picks a token): up products of 61 tokens 197 us, 7.6
-// TB/s (8 waves, of which a CU's registers hold one workgroup, 213); their down products 103
-// us, 7 TB/s (496 us with K shared out among the waves, which leaves each wave half a block
-// of its own). One token's up products take 15 us, 4.4 TB/s (8 waves 17.5: its 288
-// workgroups were one round over the CUs and an eighth of another); in all 34 us a call for
-// 37, 8 tokens 122 for 128, 128 tokens 398 for 425. Tiles of 16 rows alone need half the
-// registers, and four workgroups a CU were slower from 3 tokens on (8 tokens 127).
+// Measured (256 experts of 7168 x 512, 8 picks a token): up products of 61 tokens 196 us, 6.1
+// TB/s of the 162 experts that they pick, where a kernel that only reads has 6.4 (8 waves, of
+// which a CU's registers hold one workgroup, 213); their down products 104 us, 5.7 TB/s (496
+// us with K shared out among the waves, which leaves each wave half a block of its own). One
+// token's up products take 15 us, 4.5 TB/s (8 waves 17.5: its 288 workgroups were one round
+// over the CUs and an eighth of another); in all 34 us a call for 37, 8 tokens 122 for 128,
+// 128 tokens 398 for 425. Tiles of 16 rows alone need half the registers, and four workgroups
+// a CU were slower from 3 tokens on (8 tokens 127). Mids wider than LDS holds, rounded by a
+// launch of their own (5 us): down products of 64 tokens by 65 experts of 7168 x 1024 95 us,
+// of 7168 x 2048 189 us, 5 TB/s both; the up products 160 and 320 us, 6 TB/s.
 #include "prompt_common.h"
 
 namespace mono {
@@ -174,7 +177,7 @@ MONO_DEV void narrow_tile(const Narrow& a, f32x4* red, const uint8_t* w, const f
   const int m = 16 * wave + lane % 16;
   if (m >= count) return;
   const size_t at = (size_t)(first + m) * a.out_ld + n0 + 4 * (lane / 16);
-  if (MODE == UP) {
+  if (MODE == UP) {  // (the hardware's exponential and reciprocal: 1e-6 off for gates down to -16)
 #pragma unroll
     for (int r = 0; r < 4; ++r) y[0][r] = silu(y[0][r]) * y[NT - 1][r];
   }

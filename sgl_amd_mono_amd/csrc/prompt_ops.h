@@ -1,5 +1,5 @@
 // Host-side declarations of the prompt-width operators (internal to the library): FP8
-// block products, paged cache appends and routed experts over any number of rows.
+// block products, paged cache appends and routed experts over up to MAX_ROWS rows.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -48,8 +48,8 @@ inline int64_t all_tiles(int64_t tokens, int64_t picks, int experts, int bm, boo
 
 // The experts' outputs before their weighted sum, [places, ld]: f16 values and, for each 64
 // columns of a place, the power of two that they are multiplied by, which puts the largest
-// of them into [2^14, 2^15). 16 bits halve the bytes of the largest tensor of a call, and
-// against bf16's 2^-9 such a block's values are 2^-12 off.
+// of them into [2^14, 2^15). 16 bits halve the bytes of the largest tensor of a call; a value is
+// 2^-11 of itself off at most, an eighth of the output's own rounding to bf16 (2^-8).
 constexpr int PART = 64;
 struct Parts {
   uint16_t* v;

@@ -15,8 +15,11 @@
 // in registers: 4.2 PFLOP/s one MFMA later, 4.9 two later).
 //
 // Measured: 8192 x 7168 x 4096 209 us, 2.3 PFLOP/s (a library product of the same codes
-// with one scale a tensor: 200 us); 1500 x 2112 x 7168 34 us; the up products of 8192 tokens
-// x 9 experts of 7168 x 512 735 us, the down products 496. The MFMAs run for 57 % of the
+// with one scale a tensor: 195 us); 1500 x 2112 x 7168 34 us; the up products of 8192 tokens
+// x 9 experts of 7168 x 512 739 us, 1.5 PFLOP/s, the down products 519, 1.0. Mids wider than LDS
+// holds whole (1500 tokens x 9 of 65 experts): 7168 x 1024 up 353, down 206 us, 7168 x 2048
+// up 616, down 345, 1.0 to 1.3 PFLOP/s. f32 outputs, whose codes every wave widens: 1500 x 2112
+// x 7168 68 us, 8192 x 2112 x 7168 330, 0.7 PFLOP/s. The MFMAs run for 57 % of the
 // cycles of the first (45 % of the up products'), at a clock that the work's power holds at
 // 1.9 (1.6) GHz. With every load a cache hit the first takes 208 us: what is left is the
 // vector memory path's 48 KB a tile and block, the barrier a block and the last round of

@@ -1,5 +1,5 @@
-"""The layer's work at prompt widths: any number of rows on the layer's own weights and
-caches, where the decode launches take a step of a few.
+"""The layer's work at prompt widths: up to 1048576 rows a call on the layer's own weights
+and caches, where the decode launches take a step of a few.
 
 * ``product``: rows, rounded to E4M3, times one FP8 matrix with a scale for each 128 x 128
   block: the projections' weights as they are. (``layer.ProjRuntime`` multiplies a decode
@@ -13,6 +13,12 @@ The functions keep no state. They check the tensors, take their scratch from tor
 allocator and enqueue on the current stream of the tensors' device, so calls on several
 streams do not disturb each other, and a call may be captured in a graph. Operands made
 on another stream are the caller's to order, as for any torch operator.
+
+A call takes at most 1048576 rows (``experts``: tokens times (picks + 1), 116508 tokens at
+8 picks) and 2^35 elements of them. Scratch: a product K * (1 + 1/32) bytes a row, and f32
+parts where its tiles are few; ``experts`` mostly 2 * H bytes for each token's every pick
+(1.2 GB for 8192 tokens of 7168 with 8 picks and the shared expert), so a long prompt goes
+through it in pieces of some thousand tokens. A captured graph keeps its calls' scratch.
 """
 
 from __future__ import annotations
