@@ -49,7 +49,8 @@ inline int64_t all_tiles(int64_t tokens, int64_t picks, int experts, int bm, boo
 // The experts' outputs before their weighted sum, [places, ld]: f16 values and, for each 64
 // columns of a place, the power of two that they are multiplied by, which puts the largest
 // of them into [2^14, 2^15). 16 bits halve the bytes of the largest tensor of a call; a value is
-// 2^-11 of itself off at most, an eighth of the output's own rounding to bf16 (2^-8).
+// 2^-11 of itself off at most, an eighth of the output's own rounding to bf16 (2^-8); below 2^-29
+// of its block's largest value, 2^-39 of that.
 constexpr int PART = 64;
 struct Parts {
   uint16_t* v;

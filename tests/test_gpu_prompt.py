@@ -525,6 +525,67 @@ def test_experts_of_no_tokens(gpu_device):
     assert prompt.experts(**c).shape == (0, 256)
 
 
+# ------------------------------------------------ each way to run, as callers may
+WAYS = [(3, 272, 1024), (24, 272, 1024), (24, 64, 7168), (90, 2112, 256), (300, 528, 4096), (2050, 4112, 256)]
+
+
+@pytest.mark.parametrize("m,n,k", WAYS)
+def test_product_f32_strided_out(gpu_device, m, n, k):
+    w, s = _matrix(n, k, gpu_device, 61)
+    x = workloads.rows_bf16(m, k, gpu_device, seed=62)
+    buf = torch.full((m + 2, n + 24), 3.0, device=gpu_device)
+    got = prompt.product(x, w, s, out=buf[1:-1, 8:-16])
+    assert torch.equal(got, prompt.product(x, w, s, dtype=torch.float32))
+    assert bool((buf[0] == 3).all()) and bool((buf[-1] == 3).all())
+    assert bool((buf[:, :8] == 3).all()) and bool((buf[:, -16:] == 3).all())
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 16, 65536), (30, 32, 65536), (100, 16, 65536), (4200, 16, 65536), (1, 65536, 128),
+                                   (20, 65536, 128), (200, 65536, 256)])
+def test_product_widest(gpu_device, m, n, k):
+    """The largest K and N that a call takes, each way to run."""
+    w, s = _matrix(n, k, gpu_device, 63)
+    x = workloads.rows_bf16(m, k, gpu_device, seed=64)
+    at = torch.tensor(sorted({0, m // 2, m - 1}))
+    want, mag = ref.product(x[at].cpu(), w.cpu(), s.cpu())
+    for dtype in (torch.bfloat16, torch.float32):
+        _same(prompt.product(x, w, s, dtype=dtype)[at], want, mag, dtype == torch.float32, k)
+
+
+@pytest.mark.parametrize("t,h,i", [(3, 256, 32768), (120, 128, 32768), (5, 65536, 128), (120, 65536, 128)])
+def test_experts_widest(gpu_device, t, h, i):
+    c = _experts_case(gpu_device, t, h, i, 1, 1)
+    _check_experts(c, prompt.experts(**c))
+
+
+def test_graph_replays_of_each_way_to_run(gpu_device):
+    """Every way to run in one graph, replayed on new inputs with eager work between."""
+    dev = gpu_device
+    mats = [(_matrix(n, k, dev, 65), workloads.rows_bf16(m, k, dev, seed=66)) for m, n, k in WAYS]
+    moe = [_experts_case(dev, t, 256, i, 8, 4) for t, i in ((9, 128), (90, 640), (200, 128), (200, 640))]
+
+    def calls():
+        out = [prompt.product(x, *w, dtype=d) for w, x in mats for d in (torch.bfloat16, torch.float32)]
+        return out + [prompt.experts(**c, batch_invariant=b) for c in moe for b in (False, True)]
+
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = calls()
+    for step in range(4):
+        for _, x in mats:
+            x.copy_(workloads.rows_bf16(*x.shape, dev, seed=67 + step))
+        for c in moe:
+            c["x"].copy_(workloads.rows_bf16(*c["x"].shape, dev, seed=77 + step))
+            c["ids"].copy_(torch.randint(-1, 8, c["ids"].shape, device=dev).int())
+        graph.replay()
+        got = [o.clone() for o in outs]
+        want = calls()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---------------------------------------------------- streams, graphs, repeats
 def test_repeats_and_streams(gpu_device):
     """The same bits from call to call, and from two streams at once."""
