@@ -546,8 +546,8 @@ int mono_prompt_append(const mono_prompt_append_args* args, void* stream);
  * How the up products are summed goes by the sizes: up to 96 tokens, and up to 11 picks a
  * routed expert on average, exactly but for f32's rounding (outputs 0.0017 of their norm from
  * 64 bits, of which bf16 makes up nearly all); in wider calls on the FP8 MFMA, whose sums of
- * 128 products are 1.4e-5 off, as in mono_moe_fp8_forward (0.0020; a mid next to a border of
- * its code may take the neighbouring one). With batch_invariant the former holds at any
+ * 128 products are 1.4e-5 off, as in mono_moe_fp8_forward (0.0019 to 0.0022; a mid next to a
+ * border of its code may take the neighbouring one). With batch_invariant the former holds at any
  * width, and a token's output has the same bits whatever other tokens the call holds. */
 typedef struct {
   const void* x;            /* bf16 [tokens, hidden], the normed rows */

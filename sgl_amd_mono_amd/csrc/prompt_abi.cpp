@@ -121,7 +121,7 @@ int experts_shape(const mono_prompt_experts_args& a) {
 // The two differ in their up products' sums as well: the narrow ones widen the codes to bf16,
 // which costs nothing beside the weights' bytes and makes every product exact, the wide ones
 // take the FP8 MFMA's 1.4e-5, as the decode launch does. A mid that this carries over a code's
-// border moves by a code, so outputs are 0.0017 and 0.0020 of their norm from 64 bits. A
+// border moves by a code, so outputs are 0.0017 and 0.0019 to 0.0022 of their norm from 64 bits. A
 // caller who wants a token's bits to be its own in any company asks for the narrow tiles (the
 // first geometry: 1500 tokens 1036 us for 685, 8192 tokens 4235 for 1595).
 constexpr int WIDE_PICKS = 11, FEW_TOKENS = 96;
