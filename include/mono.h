@@ -538,6 +538,11 @@ typedef struct {
 
 int mono_prompt_append(const mono_prompt_append_args* args, void* stream);
 
+/* The same with token i's key rotated for pos[i] and written to the slot of position
+ * slot_pos[i] (NULL: pos): drafted tokens of a tree may share a position, but no slot. A token
+ * whose slot_pos is outside the page table is a pad too. */
+int mono_prompt_append_at(const mono_prompt_append_args* args, const int32_t* slot_pos, void* stream);
+
 /* out[t] = residual[t] + shared(x[t]) + sum_j weights[t, j] expert_(ids[t, j])(x[t]), with
  * expert(x) = w2 FP8(silu(gate) * up), (gate, up) = w13 FP8(x): the FP8 MoE of
  * mono_moe_fp8_forward behind a router and a norm of the caller's. A pick outside
@@ -577,6 +582,120 @@ typedef struct {
  * refused, see mono_last_error). */
 int64_t mono_prompt_experts_workspace(const mono_prompt_experts_args* args);
 int mono_prompt_experts(const mono_prompt_experts_args* args, void* stream);
+
+/* ------------------------------------- a prompt's own attention, and a drafted tree's
+ * Between mono_prompt_append and the rest of a layer: a prompt's tokens score the pages of
+ * their request by the index keys, select some, and attend to the latent rows that those hold;
+ * a tree of drafted tokens attends to its request's rows and to its own. */
+
+/* The index queries of tokens at pos[t], in the format that mono_front_forward hands to
+ * mono_attn_forward: of each of 64 heads' 128 dims bf16(x), RoPE on dims [0, 64), bf16,
+ * Hadamard, bf16 and FP4, each value formed in f64 between its roundings. A token whose
+ * position is outside [0, max_pos) is a pad: zeros. A head that is not finite has zero codes
+ * and scale bytes 255 (NaN). */
+typedef struct {
+  const void* x;          /* bf16 or f32 [tokens, 64 x 128], before RoPE */
+  int64_t x_stride;       /* elements from a row to the next; rows 16-byte aligned */
+  int32_t f32;            /* x: 0 bf16, 1 f32 */
+  int64_t tokens;         /* 0..1048576 */
+  const int32_t* pos;     /* [tokens] */
+  int32_t max_pos;
+  const float* rope_cos;  /* f32 [max_pos, 32], 16-byte aligned, as rope_sin */
+  const float* rope_sin;
+  void* iq;               /* u8 [tokens, 64, 64] E2M1 pairs, 16-byte aligned */
+  void* iqs;              /* u8 [tokens, 64, 4] E8M0 */
+} mono_prompt_query_args;
+
+int mono_prompt_query(const mono_prompt_query_args* args, void* stream);
+
+/* out[t, p] = the largest over the keys j of page p of token t's request at positions
+ * <= pos[t] of sum_h iw[t, h] max(0, q[t, h] . k[j]): mono_attn_forward's index scores, by
+ * page. -infinity where the token sees no key of the page (behind its position, a page outside
+ * the table or the pool, a pad: req outside [0, requests) or pos < 0); NaN where a key's is. */
+typedef struct {
+  const void* iq;            /* u8 [tokens, 64, 64], 16-byte aligned */
+  const void* iqs;           /* u8 [tokens, 64, 4] */
+  const void* iw;            /* bf16 [tokens, 64], 8-byte aligned */
+  int64_t tokens;            /* 0..1048576 */
+  const int32_t* req;        /* [tokens] row of page_table */
+  const int32_t* pos;        /* [tokens] */
+  const int32_t* page_table; /* [requests, pt_stride] */
+  int32_t requests, pt_stride, n_pages;
+  const void* ikv;           /* u8 [n_pages, 4, 64, 16], 16-byte aligned */
+  const void* iks;           /* u8 [n_pages, 4, 64] */
+  float* out;                /* f32 [tokens, columns] */
+  int32_t columns;           /* pages 0 .. columns - 1 are scored, 0..8192 */
+} mono_prompt_scores_args;
+
+int mono_prompt_scores(const mono_prompt_scores_args* args, void* stream);
+
+/* The `picks` pages that token t reads of those that it sees (0 .. pos[t] / 64, as far as there
+ * are columns): the first `first` and the last `last` of them, and of the others the ones with
+ * the highest scores, the lowest page first where scores are equal (+0 above -0, a NaN by its
+ * bits). Ascending, -1 behind; all -1 where pos < 0. */
+typedef struct {
+  const float* scores;  /* f32 [tokens, columns], rows stride elements apart */
+  int64_t stride;
+  int64_t tokens;       /* 0..1048576 */
+  int32_t columns;      /* 1..8192 */
+  const int32_t* pos;   /* [tokens] */
+  int32_t picks;        /* 1..8192 */
+  int32_t first, last;  /* together at most picks */
+  int32_t* pages;       /* [tokens, picks] */
+} mono_prompt_select_args;
+
+int mono_prompt_select(const mono_prompt_select_args* args, void* stream);
+
+/* Sparse MLA attention of token t over the keys at positions <= pos[t] of the pages that it
+ * lists: s_j = softmax_scale (q . c_j), p = softmax(s), out = sum_j p_j c_j[:512], with c_j =
+ * kv_scale[j] kv[j]. A page below 0, outside the table or the pool is none; one that is listed
+ * twice counts twice. A token that sees no key (a pad: req outside [0, requests) or pos < 0)
+ * has zeros. What lies in keys that are not seen does not matter. */
+typedef struct {
+  const void* q;             /* bf16 [tokens, heads, 576] (latent 512 | pe 64) */
+  int64_t tokens;            /* 0..1048576 */
+  int32_t heads;             /* 1..128 */
+  const int32_t* req;        /* [tokens] row of page_table */
+  const int32_t* pos;        /* [tokens] */
+  const int32_t* pages;      /* [tokens, picks] */
+  int32_t picks;             /* 0..8192 */
+  const int32_t* page_table; /* [requests, pt_stride] */
+  int32_t requests, pt_stride, n_pages;
+  const void* kv;            /* e4m3 [n_pages x 64, 576] */
+  const float* kv_scale;     /* f32 [n_pages x 64], or NULL: raw E4M3 rows */
+  float softmax_scale;
+  void* out;                 /* bf16 [tokens, heads, 512] (q, kv, kv_scale, out 16-byte aligned) */
+  void* workspace;
+  int64_t workspace_bytes;
+} mono_prompt_attention_args;
+
+/* Bytes of workspace (0: none; -1: refused, see mono_last_error). */
+int64_t mono_prompt_attention_workspace(int64_t tokens, int32_t heads, int32_t picks);
+int mono_prompt_attention(const mono_prompt_attention_args* args, void* stream);
+
+/* MLA attention of drafted tokens. Request r's nodes are rows starts[r] .. starts[r + 1] - 1 of
+ * q; its node i's key lies at position prefix[r] + i. Node n of it sees every key at positions
+ * below prefix[r], and key prefix[r] + j for each bit j of mask[n] (its ancestors and itself;
+ * any bits are good). Nodes of no request, and nodes that see nothing, have zeros. */
+typedef struct {
+  const void* q;             /* bf16 [nodes, heads, 576] */
+  int64_t nodes;             /* 0..1048576 */
+  int32_t heads;             /* 1..128 */
+  const int32_t* starts;     /* [requests + 1], ascending */
+  const int32_t* prefix;     /* [requests] */
+  const int64_t* mask;       /* [nodes] */
+  const int32_t* page_table; /* [requests, pt_stride] */
+  int32_t requests, pt_stride, n_pages;
+  const void* kv;            /* the rest as in mono_prompt_attention_args */
+  const float* kv_scale;
+  float softmax_scale;
+  void* out;                 /* bf16 [nodes, heads, 512] */
+  void* workspace;
+  int64_t workspace_bytes;
+} mono_prompt_tree_args;
+
+int64_t mono_prompt_tree_workspace(int64_t nodes, int32_t heads, int32_t pt_stride);
+int mono_prompt_tree(const mono_prompt_tree_args* args, void* stream);
 
 #ifdef __cplusplus
 }

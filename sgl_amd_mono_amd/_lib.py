@@ -114,6 +114,34 @@ class PromptExpertsArgs(C.Structure):
                 ("workspace_bytes", _I64)]
 
 
+class PromptQueryArgs(C.Structure):
+    _fields_ = [("x", _VP), ("x_stride", _I64), ("f32", _I32), ("tokens", _I64), ("pos", _VP), ("max_pos", _I32),
+                ("rope_cos", _VP), ("rope_sin", _VP), ("iq", _VP), ("iqs", _VP)]
+
+
+class PromptScoresArgs(C.Structure):
+    _fields_ = [("iq", _VP), ("iqs", _VP), ("iw", _VP), ("tokens", _I64), ("req", _VP), ("pos", _VP), ("page_table", _VP),
+                ("requests", _I32), ("pt_stride", _I32), ("n_pages", _I32), ("ikv", _VP), ("iks", _VP), ("out", _VP),
+                ("columns", _I32)]
+
+
+class PromptSelectArgs(C.Structure):
+    _fields_ = [("scores", _VP), ("stride", _I64), ("tokens", _I64), ("columns", _I32), ("pos", _VP), ("picks", _I32),
+                ("first", _I32), ("last", _I32), ("pages", _VP)]
+
+
+class PromptAttentionArgs(C.Structure):
+    _fields_ = [("q", _VP), ("tokens", _I64), ("heads", _I32), ("req", _VP), ("pos", _VP), ("pages", _VP), ("picks", _I32),
+                ("page_table", _VP), ("requests", _I32), ("pt_stride", _I32), ("n_pages", _I32), ("kv", _VP),
+                ("kv_scale", _VP), ("softmax_scale", _F32), ("out", _VP), ("workspace", _VP), ("workspace_bytes", _I64)]
+
+
+class PromptTreeArgs(C.Structure):
+    _fields_ = [("q", _VP), ("nodes", _I64), ("heads", _I32), ("starts", _VP), ("prefix", _VP), ("mask", _VP),
+                ("page_table", _VP), ("requests", _I32), ("pt_stride", _I32), ("n_pages", _I32), ("kv", _VP),
+                ("kv_scale", _VP), ("softmax_scale", _F32), ("out", _VP), ("workspace", _VP), ("workspace_bytes", _I64)]
+
+
 # the phase boundaries a one-launch layer stamps per workgroup (mono_layer_args.ticks)
 LAYER_TICKS = ("begin", "front", "attn", "back", "plan", "end", "a_seen", "norm", "router", "route", "quant")
 LAYER_TICK_WORDS = 16
@@ -165,6 +193,14 @@ SIGNATURES = {
     "mono_prompt_product_workspace": (_I64, [_I64, _I32, _I32]),
     "mono_prompt_product": (C.c_int, [C.POINTER(PromptProductArgs), _VP]),
     "mono_prompt_append": (C.c_int, [C.POINTER(PromptAppendArgs), _VP]),
+    "mono_prompt_append_at": (C.c_int, [C.POINTER(PromptAppendArgs), _VP, _VP]),
+    "mono_prompt_query": (C.c_int, [C.POINTER(PromptQueryArgs), _VP]),
+    "mono_prompt_scores": (C.c_int, [C.POINTER(PromptScoresArgs), _VP]),
+    "mono_prompt_select": (C.c_int, [C.POINTER(PromptSelectArgs), _VP]),
+    "mono_prompt_attention_workspace": (_I64, [_I64, _I32, _I32]),
+    "mono_prompt_attention": (C.c_int, [C.POINTER(PromptAttentionArgs), _VP]),
+    "mono_prompt_tree_workspace": (_I64, [_I64, _I32, _I32]),
+    "mono_prompt_tree": (C.c_int, [C.POINTER(PromptTreeArgs), _VP]),
     "mono_prompt_experts_workspace": (_I64, [C.POINTER(PromptExpertsArgs)]),
     "mono_prompt_experts": (C.c_int, [C.POINTER(PromptExpertsArgs), _VP]),
 }

@@ -1,75 +1,11 @@
 // The C entry points of the prompt-width operators: argument checks, the carving of the
 // caller's workspace, the launches. They keep no state: every call's scratch is the
 // workspace that the call is given.
-#include <hip/hip_runtime.h>
-
-#include <cstdarg>
-#include <cstdio>
-
-#include "abi_errors.h"
-#include "prompt_ops.h"
+#include "prompt_abi.h"
 
 namespace {
 
 using namespace mono::prompt;
-
-int refuse(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
-int refuse(const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  return mono::abi_fail(MONO_EINVAL, buf);
-}
-
-int launched(hipError_t e, const char* what) {
-  if (e == hipSuccess) return mono::abi_ok();
-  char buf[256];
-  snprintf(buf, sizeof buf, "launching %s: %s", what, hipGetErrorString(e));
-  return mono::abi_fail(MONO_EHIP, buf);
-}
-
-// a device pointer that the launches' vector loads and stores can use
-int need(const void* p, const char* name, size_t align) {
-  if (!p) return refuse("argument %s must be a device pointer, got NULL", name);
-  if (reinterpret_cast<uintptr_t>(p) % align) return refuse("argument %s must be %zu-byte aligned, got %p", name, align, p);
-  return MONO_OK;
-}
-
-int need_rows(int64_t rows, const char* name) {
-  if (rows < 0 || rows > MAX_ROWS) return refuse("%s must be in [0, %lld], got %lld", name, (long long)MAX_ROWS, (long long)rows);
-  return MONO_OK;
-}
-
-int need_stride(int64_t stride, int64_t least, int64_t multiple, const char* name) {
-  if (stride < least || stride % multiple)
-    return refuse("%s must be a multiple of %lld that is at least %lld, got %lld", name, (long long)multiple, (long long)least,
-                  (long long)stride);
-  return MONO_OK;
-}
-
-// Carves the caller's workspace into 256-byte aligned pieces; with no base it only adds
-// up what a call needs.
-struct Space {
-  char* base;
-  size_t off = 0;
-  template <class T>
-  T* take(size_t n) {
-    T* p = base ? reinterpret_cast<T*>(base + off) : nullptr;
-    off += (n * sizeof(T) + 255) & ~size_t(255);
-    return p;
-  }
-  Rows rows(int64_t n, int k) {
-    uint8_t* q = take<uint8_t>((size_t)n * k);
-    return Rows{q, take<float>((size_t)n * (k / BLK)), (int)n};
-  }
-};
-
-int need_space(const void* ws, int64_t bytes, size_t least) {
-  if (bytes < 0 || (size_t)bytes < least) return refuse("workspace must hold %zu bytes, got %lld", least, (long long)bytes);
-  return need(ws, "workspace", 256);
-}
 
 int need_elements(int64_t rows, int k, const char* names) {
   if (rows * k > MAX_ELEMENTS) return refuse("%s must be at most %lld, got %lld x %d", names, (long long)MAX_ELEMENTS, (long long)rows, k);
@@ -197,6 +133,10 @@ extern "C" int mono_prompt_product(const mono_prompt_product_args* args, void* s
 }
 
 extern "C" int mono_prompt_append(const mono_prompt_append_args* args, void* stream) {
+  return mono_prompt_append_at(args, nullptr, stream);
+}
+
+extern "C" int mono_prompt_append_at(const mono_prompt_append_args* args, const int32_t* slot_pos, void* stream) {
   if (!args) return refuse("mono_prompt_append: args is NULL");
   const mono_prompt_append_args& a = *args;
   if (int rc = need_rows(a.tokens, "tokens")) return rc;
@@ -222,7 +162,9 @@ extern "C" int mono_prompt_append(const mono_prompt_append_args* args, void* str
     if (int rc = need(a.kv_scale, "kv_scale", 4)) return rc;
   if (int rc = need(a.ikv, "ikv", 4)) return rc;
   if (int rc = need(a.iks, "iks", 1)) return rc;
-  return launched(append(a, static_cast<hipStream_t>(stream)), "the cache append");
+  if (slot_pos)
+    if (int rc = need(slot_pos, "slot_pos", 4)) return rc;
+  return launched(append(a, slot_pos, static_cast<hipStream_t>(stream)), "the cache append");
 }
 
 extern "C" int64_t mono_prompt_experts_workspace(const mono_prompt_experts_args* args) {

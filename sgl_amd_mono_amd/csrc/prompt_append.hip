@@ -16,8 +16,7 @@
 // Measured: 32768 bf16 tokens 21.9 us (one wave a token, with LDS permutes and library
 // square roots: 37), 3.5 TB/s of its 76 MB against the 4.9 of a large copy; the vector
 // unit's f64 and the memory are about even. 1 token 3.9 us.
-#include "prompt_common.h"
-#include "proj_common.h"
+#include "prompt_index.h"
 
 namespace mono {
 namespace prompt {
@@ -25,54 +24,6 @@ namespace {
 
 constexpr int T = 256;
 constexpr double EPS = 1e-6;
-
-// (every lane has a source here, so nothing needs the register's old value)
-template <int CTRL>
-MONO_DEV uint32_t dpp_all(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
-}
-template <int CTRL>
-MONO_DEV double dpp_d(double v) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint64_t r = (uint64_t)dpp_all<CTRL>((uint32_t)u) | (uint64_t)dpp_all<CTRL>((uint32_t)(u >> 32)) << 32;
-  return __builtin_bit_cast(double, r);
-}
-// the sum over each 16 lanes, the same in every one of them
-MONO_DEV double row_sum_d(double v) {
-  v += dpp_d<DPP_XOR1>(v);
-  v += dpp_d<DPP_XOR2>(v);
-  v += dpp_d<DPP_HALF_MIRROR>(v);
-  return v + dpp_d<DPP_MIRROR>(v);
-}
-// lane i's value of lane i ^ 4 in each 16 lanes: banks of 4 lanes rotated by one bank, the
-// odd ones forwards, the even ones backwards
-MONO_DEV uint32_t xor4_u(uint32_t v) {
-  const int up = (int)dpp_all<0x124>(v);  // row_ror:4: right for banks 1 and 3
-  return (uint32_t)__builtin_amdgcn_update_dpp(up, (int)v, 0x12c, 0xf, 0x5, false);  // row_ror:12 over banks 0 and 2
-}
-constexpr int DPP_XOR8 = 0x128;  // row_ror:8
-template <int X>
-MONO_DEV double row_xor_d(double v) {
-  if (X != 4) return dpp_d<X == 1 ? (int)DPP_XOR1 : X == 2 ? (int)DPP_XOR2 : DPP_XOR8>(v);
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  return __builtin_bit_cast(double, (uint64_t)xor4_u((uint32_t)u) | (uint64_t)xor4_u((uint32_t)(u >> 32)) << 32);
-}
-// A butterfly between lanes X apart: a + b in the lane with the bit clear, a - b in its partner.
-template <int X>
-MONO_DEV void lanes_butterfly(double (&y)[8], int sub) {
-  const double sign = sub & X ? -1.0 : 1.0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = fma(sign, y[i], row_xor_d<X>(y[i]));
-}
-MONO_DEV void lane_butterfly(double (&y)[8], int x) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (!(i & x)) {
-      const double a = y[i], b = y[i + x];
-      y[i] = a + b;
-      y[i + x] = a - b;
-    }
-}
 
 // 1 / sqrt(a), a > 0: the hardware's estimate (some 24 bits) and two Newton steps
 MONO_DEV double rsqrt_d(double a) {
@@ -82,59 +33,24 @@ MONO_DEV double rsqrt_d(double a) {
   return y;
 }
 
-// through f32, as torch casts (an opaque copy: the compiler would fuse the two roundings
-// into one, by a longer sequence)
-MONO_DEV float to_bf16(double v) {
-  float f = (float)v;
-  asm("" : "+v"(f));
-  return bf16_round(f);
-}
-
-// the larger of each magnitude's bits over the 16 lanes of a token, over 4 lanes of it
-MONO_DEV uint32_t quad_umax(uint32_t v) {
-  v = max(v, dpp_u<DPP_XOR1>(v));
-  return max(v, dpp_u<DPP_XOR2>(v));
-}
-
-MONO_DEV void load4(const uint16_t* p, float (&v)[4]) {
-  const u32x2 w = *reinterpret_cast<const u32x2*>(p);
-  const uint32_t a = w[0], b = w[1];
-  v[0] = bf16_lo(a), v[1] = bf16_hi(a), v[2] = bf16_lo(b), v[3] = bf16_hi(b);
-}
-MONO_DEV void load4(const float* p, float (&v)[4]) {
-  const f32x4 w = *reinterpret_cast<const f32x4*>(p);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = w[i];
-}
-
 // v / 2^(e - 127) within the E4M3 range; what is not finite stays so (its code is NaN)
 MONO_DEV float scaled_to_e4m3(float v, float inv) {
   const float q = v * inv;
   return abs_bits(v) < 0x7f800000u ? fminf(fmaxf(q, -FP8_MAX), FP8_MAX) : __uint_as_float(0x7fc00000u);
 }
 
-// Eight values of |q| <= 6 as E2M1 codes (the first in the low nibble), ties to even, no
-// negative zero: a sign bit stays where its code's magnitude is not zero.
-MONO_DEV uint32_t e2m1_pack8(const float (&q)[8]) {
-  uint32_t w = 0;
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[0], q[1], 1.0f, 0);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[2], q[3], 1.0f, 1);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[4], q[5], 1.0f, 2);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[6], q[7], 1.0f, 3);
-  return w & (((w & 0x77777777u) + 0x77777777u) | 0x77777777u);
-}
-
 template <class V>
-__global__ __launch_bounds__(T) void k_append(mono_prompt_append_args a) {
+__global__ __launch_bounds__(T) void k_append(mono_prompt_append_args a, const int32_t* slot_pos) {
   const int sub = threadIdx.x % 16;
   const int64_t i = (int64_t)blockIdx.x * (T / 16) + threadIdx.x / 16;
   // a lane group without a token to write computes the last token's and stores nothing
   const int64_t n = i < a.tokens ? i : a.tokens - 1;
-  int req = a.req[n], pos = a.pos[n];
-  bool live = i < a.tokens && req >= 0 && req < a.requests && pos >= 0 && pos < a.max_pos && pos / PAGE < a.pt_stride;
+  int req = a.req[n], pos = a.pos[n], at_pos = slot_pos ? slot_pos[n] : pos;
+  bool live = i < a.tokens && req >= 0 && req < a.requests && pos >= 0 && pos < a.max_pos && at_pos >= 0 && at_pos / PAGE < a.pt_stride;
   req = live ? req : 0;
   pos = live ? pos : 0;
-  const int page = a.page_table[(int64_t)req * a.pt_stride + pos / PAGE], t = pos % PAGE;
+  at_pos = live ? at_pos : 0;
+  const int page = a.page_table[(int64_t)req * a.pt_stride + at_pos / PAGE], t = at_pos % PAGE;
   live = live && page >= 0 && page < a.n_pages;
   if (!__any(live)) return;
   const V* kv = static_cast<const V*>(a.kv_a) + n * a.kv_stride;
@@ -234,40 +150,22 @@ __global__ __launch_bounds__(T) void k_append(mono_prompt_append_args a) {
     y[2 * v] = to_bf16(y0 * c - y1 * s);
     y[2 * v + 1] = to_bf16(y0 * s + y1 * c);
   }
-  lane_butterfly(y, 1);
-  lane_butterfly(y, 2);
-  lane_butterfly(y, 4);
-  lanes_butterfly<1>(y, sub);
-  lanes_butterfly<2>(y, sub);
-  lanes_butterfly<4>(y, sub);
-  lanes_butterfly<8>(y, sub);
-  uint32_t hm = 0;
-#pragma unroll
-  for (int v = 0; v < 8; ++v) {
-    k[v] = to_bf16(y[v] * 0.08838834764831844055);  // 128^-1/2
-    hm = max(hm, abs_bits(k[v]));
-  }
-  hm = quad_umax(hm);
-  const bool finite = hm < 0x7f800000u;
-  const uint32_t e8 = finite ? proj::code_ceil(proj::mul_rn(fmaxf(__uint_as_float(hm), 6.0f * 0x1p-126f), 1.0f / 6.0f)) : 255u;
-  const float ei = proj::pow2_of(254u - min(e8, 254u));
-#pragma unroll
-  for (int v = 0; v < 8; ++v) k[v] *= ei;
+  uint32_t e8;
+  const uint32_t codes = index_codes(y, sub, e8);
   if (!live) return;
-  // FP4 has no NaN: a block that is not finite gets the scale format's NaN
   const int64_t at = ((int64_t)page * 4 + sub / 4) * PAGE;
-  *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.ikv) + (at + t) * 16 + 4 * (sub % 4)) = finite ? e2m1_pack8(k) : 0u;
+  *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.ikv) + (at + t) * 16 + 4 * (sub % 4)) = codes;
   if (sub % 4 == 0) static_cast<uint8_t*>(a.iks)[at + t % 16 * 4 + t / 16] = (uint8_t)e8;
 }
 
 }  // namespace
 
-hipError_t append(const mono_prompt_append_args& a, hipStream_t st) {
+hipError_t append(const mono_prompt_append_args& a, const int32_t* slot_pos, hipStream_t st) {
   const uint32_t grid = (uint32_t)((a.tokens + T / 16 - 1) / (T / 16));
   if (a.f32)
-    k_append<float><<<grid, T, 0, st>>>(a);
+    k_append<float><<<grid, T, 0, st>>>(a, slot_pos);
   else
-    k_append<uint16_t><<<grid, T, 0, st>>>(a);
+    k_append<uint16_t><<<grid, T, 0, st>>>(a, slot_pos);
   return hipGetLastError();
 }
 

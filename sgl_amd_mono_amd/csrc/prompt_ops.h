@@ -16,7 +16,9 @@ constexpr int MAX_DIM = 1 << 16;     // columns and outputs of a product
 constexpr int64_t MAX_ROWS = 1 << 20;  // rows a call; picks of all rows of an experts call
 constexpr int64_t MAX_ELEMENTS = (1ll << 35) - 1;  // of the rows of a product or an experts call
 
-constexpr int LATENT = 512, PE = 64, INDEX = 128, PAGE = 64;
+constexpr int LATENT = 512, PE = 64, INDEX = 128, INDEX_HEADS = 64, PAGE = 64;
+constexpr int MAX_COLUMNS = 8192;  // pages that a call scores or selects from: 524288 keys
+constexpr int MAX_HEADS = 128;
 
 // Rows rounded to E4M3: codes [rows, k] and scales [k / 128, ld] (a block's scales of
 // consecutive rows lie together: a product's lanes hold one row each).
@@ -151,7 +153,46 @@ hipError_t wide_experts_up(const Experts& a, hipStream_t st);
 hipError_t wide_experts_down(const Experts& a, hipStream_t st);
 hipError_t experts_back(const Experts& a, hipStream_t st);
 
-hipError_t append(const mono_prompt_append_args& a, hipStream_t st);
+hipError_t append(const mono_prompt_append_args& a, const int32_t* slot_pos, hipStream_t st);
+hipError_t index_query(const mono_prompt_query_args& a, hipStream_t st);
+hipError_t page_scores(const mono_prompt_scores_args& a, hipStream_t st);
+hipError_t select_pages(const mono_prompt_select_args& a, hipStream_t st);
+
+// MLA attention over cache pages: of each token's list of pages (attention), or of all of its
+// request's (tree: `starts` is given, and tokens are nodes).
+struct Paged {
+  const void* q;  // bf16 [tokens, heads, 576]
+  int64_t tokens;
+  int heads;
+  const int32_t *req, *pos, *pages;
+  int picks;
+  const int32_t *starts, *prefix;
+  const int64_t* mask;
+  const int32_t* page_table;
+  int requests, pt_stride, n_pages;
+  const void* kv;
+  const float* kv_scale;
+  float scale_log2;  // the softmax scale x log2(e)
+  void* out;         // bf16 [tokens, heads, 512]
+  // how it is shared out: heads a workgroup, workgroups a token's heads, workgroups a token's
+  // pages, and all of them
+  int head_rows, head_tiles, splits;
+  int64_t work;
+  float *part, *part_m, *part_l;  // splits > 1: f32 [tokens, splits, heads, 512] and [.., heads] twice
+};
+
+// How the pages are shared out. Splits only where the tokens' heads alone would leave CUs
+// without work: two workgroups a CU, a page each at least.
+inline void paged_plan(Paged& a, int pages) {
+  a.head_rows = a.heads <= 16 ? 16 : 32;
+  a.head_tiles = (a.heads + a.head_rows - 1) / a.head_rows;
+  const int64_t whole = a.tokens * a.head_tiles, fit = 512 / whole;
+  a.splits = (int)(fit < pages ? fit : pages);
+  if (a.splits < 1) a.splits = 1;
+  a.work = whole * a.splits;
+}
+hipError_t paged_attention(const Paged& a, hipStream_t st);
+hipError_t join_attention(const Paged& a, hipStream_t st);
 
 }  // namespace prompt
 }  // namespace mono

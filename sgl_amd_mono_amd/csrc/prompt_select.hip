@@ -1,0 +1,130 @@
+// Which pages a token reads: the first and the last few that it sees, and of the others the
+// best-scored, exactly, a tie's lowest page first.
+//
+// A row's scores as whole numbers in the same order; the k-th largest is found bit by bit from
+// the top, and what is at or above it goes out in ascending order of pages. A row lies in
+// registers: of one wave, up to 512 columns, of a workgroup above.
+#include "prompt_common.h"
+
+namespace mono {
+namespace prompt {
+namespace {
+
+// larger key = larger value; +0 above -0, a NaN by its bits
+MONO_DEV uint32_t order_key(float f) {
+  const uint32_t b = __float_as_uint(f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// the sum over a row's waves
+template <int W>
+MONO_DEV int row_count(int n, int* lds, int wave) {
+  if (W == 1) return n;
+  __syncthreads();
+  if (threadIdx.x % WAVE == 0) lds[wave] = n;
+  __syncthreads();
+  n = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) n += lds[w];
+  return n;
+}
+
+// W waves a row, N values a lane: value i of lane l of wave w is column (w N + i) 64 + l.
+template <int W, int N>
+__global__ __launch_bounds__(256) void k_select(mono_prompt_select_args a) {
+  __shared__ int lds[4];
+  const int lane = threadIdx.x % WAVE, wv = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), w = wv % W;
+  const int64_t t = (int64_t)blockIdx.x * (4 / W) + wv / W;
+  if (t >= a.tokens) return;  // (W > 1: of the whole workgroup)
+  const int pos = __builtin_amdgcn_readfirstlane(a.pos[t]);
+  const int n = pos < 0 ? 0 : min(pos / PAGE + 1, a.columns);  // pages that the token sees
+  const int mine = pos < 0 ? -1 : min(pos / PAGE, a.columns - 1);
+  const float* row = a.scores + t * a.stride;
+  int32_t* out = a.pages + t * a.picks;
+  uint32_t key[N];
+  uint32_t always = 0;  // bit i: value i is taken whatever its score
+  int forced = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = (w * N + i) * WAVE + lane;
+    key[i] = order_key(row[min(c, a.columns - 1)]);
+    const bool f = c < n && (c < a.first || c > mine - a.last);
+    always |= f ? 1u << (i % 32) : 0u;
+    static_assert(N <= 32, "a bit each");
+    forced += __popcll(__ballot(f));
+  }
+  const auto open = [&](int i) { return (w * N + i) * WAVE + lane < n && !(always >> i & 1); };
+  forced = row_count<W>(forced, lds, w);
+  // picks left for the scores; an open key above `top` is taken, and of those equal to it the
+  // first `border`
+  const int need = a.picks - forced, rest = n - forced;
+  uint32_t top = 0;
+  int border = need > 0 ? INT32_MAX : 0;
+  if (need == 0) top = 0xffffffffu;
+  if (need > 0 && need < rest) {
+    const auto count = [&](auto at_least) {
+      int m = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) m += __popcll(__ballot(open(i) && at_least(key[i])));
+      return row_count<W>(m, lds, w);
+    };
+    int kept = rest;  // open keys that are at least `top`
+#pragma unroll 1
+    for (int bit = 31; bit >= 0 && kept != need; --bit) {
+      const uint32_t cand = top | 1u << bit;
+      const int m = count([&](uint32_t k) { return k >= cand; });
+      if (m >= need) top = cand, kept = m;
+    }
+    if (kept != need) border = need - count([&](uint32_t k) { return k > top; });
+  }
+  int ties_before = 0, taken_before = 0;
+  if (W > 1) {  // what the waves before this one take
+    int eq = 0, gt = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      eq += __popcll(__ballot(open(i) && key[i] == top));
+      gt += __popcll(__ballot((always >> i & 1) || (open(i) && key[i] > top)));
+    }
+    __syncthreads();
+    if (lane == 0) lds[w] = eq;
+    __syncthreads();
+    for (int v = 0; v < w; ++v) ties_before += lds[v];
+    __syncthreads();
+    if (lane == 0) lds[w] = gt;
+    __syncthreads();
+    for (int v = 0; v < w; ++v) taken_before += lds[v];
+    taken_before += min(ties_before, border);
+  }
+  int at = taken_before, ties = ties_before;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const bool eq = open(i) && key[i] == top;
+    const uint64_t eqs = __ballot(eq);
+    const bool tie = eq && ties + (int)__popcll(eqs & ((1ull << lane) - 1)) < border;
+    const bool take = (always >> i & 1) || (open(i) && key[i] > top) || tie;
+    const uint64_t taken = __ballot(take);
+    const int place = at + (int)__popcll(taken & ((1ull << lane) - 1));
+    if (take) out[place] = (w * N + i) * WAVE + lane;
+    at += __popcll(taken);
+    ties += __popcll(eqs);
+  }
+  if (w == W - 1)
+    for (int i = at + lane; i < a.picks; i += WAVE) out[i] = -1;
+}
+
+}  // namespace
+
+hipError_t select_pages(const mono_prompt_select_args& a, hipStream_t st) {
+  const auto launch = [&](auto kernel, int rows) {
+    kernel<<<(uint32_t)((a.tokens + rows - 1) / rows), 256, 0, st>>>(a);
+    return hipGetLastError();
+  };
+  if (a.columns <= 128) return launch(k_select<1, 2>, 4);
+  if (a.columns <= 256) return launch(k_select<1, 4>, 4);
+  if (a.columns <= 512) return launch(k_select<1, 8>, 4);
+  if (a.columns <= 2048) return launch(k_select<4, 8>, 1);
+  return launch(k_select<4, 32>, 1);  // 8192 columns: MAX_COLUMNS
+}
+
+}  // namespace prompt
+}  // namespace mono

@@ -8,6 +8,11 @@ and caches, where the decode launches take a step of a few.
   launch writes for a decode step's rows, from the same projections)
 * ``experts``: the routed and the shared FP8 experts (the products of
   ``moe.MoeRuntime.forward_fp8``, behind a router of the caller's)
+* ``index_query``, ``page_scores``, ``select_pages``, ``attention``: a prompt's own sparse
+  attention. Where a decode step's row selects its 2048 best keys one at a time, a prompt's
+  token selects pages of 64 keys by the best index score in each, and attends to their keys.
+* ``tree_attention``: attention of a tree of drafted tokens to its request's keys and to
+  those of the draft that each token's mask lets it see
 
 The functions keep no state. They check the tensors, take their scratch from torch's
 allocator and enqueue on the current stream of the tensors' device, so calls on several
@@ -28,10 +33,12 @@ import ctypes as C
 import torch
 
 from . import _lib
-from .attn import PAGE, AttnCaches
-from .layer import INDEX_DIM, KV_LORA, PE_DIM
+from .attn import PAGE, SOFTMAX_SCALE, TOPK, AttnCaches
+from .layer import INDEX_DIM, INDEX_HEADS, KV_LORA, PE_DIM
 from .moe import FP8_TYPES
 from .runtime import need as _need
+
+MAX_COLUMNS = 8192  # pages that a call scores, selects from or lists for a token: 524288 keys
 
 
 # The current stream's handle without a Stream object around it, which takes longer to make
@@ -153,14 +160,18 @@ def product(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, out: torch.Tensor
 
 def append(kv_a: torch.Tensor, ik: torch.Tensor, req: torch.Tensor, pos: torch.Tensor, page_table: torch.Tensor,
            caches: AttnCaches, g_kv: torch.Tensor, g_ik: torch.Tensor, b_ik: torch.Tensor, rope_cos: torch.Tensor,
-           rope_sin: torch.Tensor) -> None:
+           rope_sin: torch.Tensor, slot_pos: torch.Tensor | None = None) -> None:
     """Write the keys of ``tokens`` tokens into ``caches`` in place, as the front launch
     writes a decode step's: ``kv_a`` [tokens, 576] (latent 512 | k_pe 64) and ``ik``
     [tokens, 128], bf16 or f32 (both alike; rows may lie apart), are the projections before
     their norms and rotation. Token i is position ``pos[i]`` of request ``req[i]``, a row
     of ``page_table`` [requests, pages] (all i32). A token whose request, position (below
     the rows of ``rope_cos`` / ``rope_sin`` and what the page table covers) or page is out
-    of range is a pad and writes nothing; two tokens must not share a slot."""
+    of range is a pad and writes nothing; two tokens must not share a slot.
+
+    With ``slot_pos`` (i32 [tokens]) token i's key is rotated for ``pos[i]`` and written to the
+    slot of position ``slot_pos[i]``: the tokens of a drafted tree may share a position, but
+    each has a slot of its own (``tree_attention``)."""
     dev = _gpu(kv_a, "kv_a")
     if kv_a.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"kv_a: expected dtype torch.bfloat16 or torch.float32, got {kv_a.dtype}")
@@ -194,7 +205,12 @@ def append(kv_a: torch.Tensor, ik: torch.Tensor, req: torch.Tensor, pos: torch.T
         g_ik=g_ik.data_ptr(), b_ik=b_ik.data_ptr(), rope_cos=rope_cos.data_ptr(), rope_sin=rope_sin.data_ptr(),
         kv=caches.kv.data_ptr(), kv_scale=_lib.ptr(caches.kv_scale), ikv=caches.ikv.data_ptr(), iks=caches.iks.data_ptr(),
     )  # fmt: skip
-    _enqueue(dev, _lib.lib().mono_prompt_append, args)
+    if slot_pos is None:
+        _enqueue(dev, _lib.lib().mono_prompt_append, args)
+    else:
+        need(slot_pos, "slot_pos", (t,), torch.int32, dev)
+        at = slot_pos.data_ptr()
+        _enqueue(dev, lambda a, stream: _lib.lib().mono_prompt_append_at(a, at, stream), args)
 
 
 def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: torch.Tensor, s13: torch.Tensor,
@@ -242,4 +258,181 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: torc
     lib = _lib.lib()
     ws = _workspace(args, lib.mono_prompt_experts_workspace(C.byref(args)), dev)  # noqa: F841 (held over the call)
     _enqueue(dev, lib.mono_prompt_experts, args)
+    return out
+
+
+def index_query(x: torch.Tensor, pos: torch.Tensor, rope_cos: torch.Tensor,
+                rope_sin: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The FP4 index queries of tokens at ``pos`` (i32 [tokens]): ``x`` [tokens, 64 * 128] bf16
+    or f32 (rows may lie apart) is the projection before its rotation. Returns ``(iq, iqs)``, u8
+    [tokens, 64, 64] and [tokens, 64, 4], as ``attn.AttnStep`` and ``page_scores`` take them. A
+    token whose position has no row in ``rope_cos`` / ``rope_sin`` is a pad: zeros."""
+    dev = _gpu(x, "x")
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"x: expected dtype torch.bfloat16 or torch.float32, got {x.dtype}")
+    t = x.shape[0] if x.dim() == 2 else -1
+    stride = _rows(x, "x", (t, INDEX_HEADS * INDEX_DIM), x.dtype, dev)
+    need(pos, "pos", (t,), torch.int32, dev)
+    if not isinstance(rope_cos, torch.Tensor) or rope_cos.dim() != 2 or rope_cos.shape[1] != PE_DIM // 2:
+        raise ValueError(f"rope_cos: expected [max_pos, {PE_DIM // 2}], got {tuple(getattr(rope_cos, 'shape', ()))}")
+    need(rope_cos, "rope_cos", tuple(rope_cos.shape), torch.float32, dev)
+    need(rope_sin, "rope_sin", tuple(rope_cos.shape), torch.float32, dev)
+    iq = torch.empty(t, INDEX_HEADS, INDEX_DIM // 2, dtype=torch.uint8, device=dev)
+    iqs = torch.empty(t, INDEX_HEADS, INDEX_DIM // 32, dtype=torch.uint8, device=dev)
+    args = _lib.PromptQueryArgs(x=x.data_ptr(), x_stride=stride, f32=x.dtype == torch.float32, tokens=t, pos=pos.data_ptr(),
+                                max_pos=rope_cos.shape[0], rope_cos=rope_cos.data_ptr(), rope_sin=rope_sin.data_ptr(),
+                                iq=iq.data_ptr(), iqs=iqs.data_ptr())
+    _enqueue(dev, _lib.lib().mono_prompt_query, args)
+    return iq, iqs
+
+
+def _tokens_of(req: torch.Tensor, pos: torch.Tensor, page_table: torch.Tensor, t: int, dev: torch.device) -> None:
+    need(req, "req", (t,), torch.int32, dev)
+    need(pos, "pos", (t,), torch.int32, dev)
+    _table(page_table, dev)
+
+
+def _pages_number(v: int, name: str) -> None:
+    if not isinstance(v, int) or not 0 <= v <= MAX_COLUMNS:
+        raise ValueError(f"{name}: expected a number of pages in [0, {MAX_COLUMNS}], got {v!r}")
+
+
+def _table(page_table: torch.Tensor, dev: torch.device) -> None:
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+        raise ValueError(f"page_table: expected [requests, pages], got {tuple(getattr(page_table, 'shape', ()))}")
+    need(page_table, "page_table", tuple(page_table.shape), torch.int32, dev)
+
+
+def page_scores(iq: torch.Tensor, iqs: torch.Tensor, iw: torch.Tensor, req: torch.Tensor, pos: torch.Tensor,
+                page_table: torch.Tensor, caches: AttnCaches, columns: int | None = None) -> torch.Tensor:
+    """The best index score in each page that a token sees: f32 [tokens, columns], for pages 0
+    .. ``columns`` - 1 of its request (default: all that ``page_table`` [requests, pages] has;
+    at most 8192). ``iq`` / ``iqs`` are the tokens' index queries (``index_query``), ``iw`` bf16
+    [tokens, 64] their head weights; token i is position ``pos[i]`` of request ``req[i]`` (i32),
+    and a key's score the decode launches' index score. -infinity where the token sees no key
+    of the page, NaN where the score of one is."""
+    dev = _gpu(iq, "iq")
+    t = iq.shape[0] if iq.dim() == 3 else -1
+    need(iq, "iq", (t, INDEX_HEADS, INDEX_DIM // 2), torch.uint8, dev)
+    need(iqs, "iqs", (t, INDEX_HEADS, INDEX_DIM // 32), torch.uint8, dev)
+    need(iw, "iw", (t, INDEX_HEADS), torch.bfloat16, dev)
+    _tokens_of(req, pos, page_table, t, dev)
+    if not isinstance(caches.ikv, torch.Tensor) or caches.ikv.dim() != 4:
+        raise ValueError(f"ikv: expected [pages, 4, {PAGE}, 16], got {tuple(getattr(caches.ikv, 'shape', ()))}")
+    pages = caches.ikv.shape[0]
+    need(caches.ikv, "ikv", (pages, 4, PAGE, 16), torch.uint8, dev)
+    need(caches.iks, "iks", (pages, 4, PAGE), torch.uint8, dev)
+    columns = page_table.shape[1] if columns is None else columns
+    _pages_number(columns, "columns")
+    out = torch.empty(t, columns, dtype=torch.float32, device=dev)
+    args = _lib.PromptScoresArgs(
+        iq=iq.data_ptr(), iqs=iqs.data_ptr(), iw=iw.data_ptr(), tokens=t, req=req.data_ptr(), pos=pos.data_ptr(),
+        page_table=page_table.data_ptr(), requests=page_table.shape[0], pt_stride=page_table.shape[1], n_pages=pages,
+        ikv=caches.ikv.data_ptr(), iks=caches.iks.data_ptr(), out=out.data_ptr(), columns=columns,
+    )  # fmt: skip
+    _enqueue(dev, _lib.lib().mono_prompt_scores, args)
+    return out
+
+
+def select_pages(scores: torch.Tensor, pos: torch.Tensor, picks: int = TOPK // PAGE, first: int = 0, last: int = 1) -> torch.Tensor:
+    """The pages that each token reads, i32 [tokens, picks] ascending, -1 behind them: of the
+    pages 0 .. ``pos[i]`` // 64 of ``scores`` f32 [tokens, columns] (rows may lie apart) the
+    ``first`` first and the ``last`` last (the token's own page among them), and the best-scored
+    others, exactly, the lowest page of equal ones first (+0 above -0, a NaN by its bits). A token that
+    sees at most ``picks`` pages reads all of them (with the default 32, every key of up to
+    2048, as a decode step's row does). ``pos[i]`` < 0 is a pad: all -1."""
+    dev = _gpu(scores, "scores")
+    if scores.dim() != 2:
+        raise ValueError(f"scores: expected [tokens, columns], got {tuple(scores.shape)}")
+    for name, v in (("picks", picks), ("first", first), ("last", last)):
+        _pages_number(v, name)
+    t, columns = scores.shape
+    stride = max(_rows(scores, "scores", (t, columns), torch.float32, dev), columns)
+    need(pos, "pos", (t,), torch.int32, dev)
+    pages = torch.empty(t, picks, dtype=torch.int32, device=dev)
+    args = _lib.PromptSelectArgs(scores=scores.data_ptr(), stride=stride, tokens=t, columns=columns, pos=pos.data_ptr(),
+                                 picks=picks, first=first, last=last, pages=pages.data_ptr())
+    _enqueue(dev, _lib.lib().mono_prompt_select, args)
+    return pages
+
+
+def _latents(q: torch.Tensor, caches: AttnCaches, out: torch.Tensor | None, dev: torch.device) -> tuple[int, torch.Tensor]:
+    """The checks that both attentions share: the cache's pages and ``out``."""
+    if q.dim() != 3 or q.shape[2] != KV_LORA + PE_DIM:
+        raise ValueError(f"q: expected [tokens, heads, {KV_LORA + PE_DIM}], got {tuple(q.shape)}")
+    t, heads = q.shape[:2]
+    need(q, "q", (t, heads, KV_LORA + PE_DIM), torch.bfloat16, dev)
+    kv = caches.kv
+    if not isinstance(kv, torch.Tensor) or kv.dim() != 2 or kv.shape[0] % PAGE:
+        raise ValueError(f"kv: expected [pages * {PAGE}, {KV_LORA + PE_DIM}], got {tuple(getattr(kv, 'shape', ()))}")
+    slots = kv.shape[0]
+    need(kv, "kv", (slots, KV_LORA + PE_DIM), FP8_TYPES, dev)
+    if caches.kv_scale is not None:  # None: raw E4M3 rows (scale 1)
+        need(caches.kv_scale, "kv_scale", (slots,), torch.float32, dev)
+    if out is None:
+        out = torch.empty(t, heads, KV_LORA, dtype=torch.bfloat16, device=dev)
+    else:
+        need(out, "out", (t, heads, KV_LORA), torch.bfloat16, dev)
+        a, b = q.data_ptr(), out.data_ptr()
+        if a < b + 2 * out.numel() and b < a + 2 * q.numel():
+            raise ValueError("out: shares memory with q")
+    return slots // PAGE, out
+
+
+def attention(q: torch.Tensor, req: torch.Tensor, pos: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor,
+              caches: AttnCaches, softmax_scale: float = SOFTMAX_SCALE, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Sparse MLA attention of a prompt's tokens: ``q`` bf16 [tokens, heads, 576] (absorbed
+    latent query 512 | rotated query 64; up to 128 heads) over the cached rows of the pages that
+    each token lists in ``pages`` (i32 [tokens, picks]: ``select_pages``; numbers of pages of
+    its request, -1: none), as far as their positions are at most the token's own. Returns
+    [tokens, heads, 512] bf16, what the attention launch of a decode step hands on.
+
+    Token i is position ``pos[i]`` of request ``req[i]``, a row of ``page_table`` [requests,
+    pages] (all i32). A listed page outside the table or the pool is none, one that is listed
+    twice counts twice. A token that sees no key has zeros. Keys that a token does not see may
+    hold anything. ``out`` must share no memory with ``q``."""
+    dev = _gpu(q, "q")
+    n_pages, out = _latents(q, caches, out, dev)
+    t, heads = q.shape[:2]
+    _tokens_of(req, pos, page_table, t, dev)
+    if not isinstance(pages, torch.Tensor) or pages.dim() != 2:
+        raise ValueError(f"pages: expected [tokens, picks], got {tuple(getattr(pages, 'shape', ()))}")
+    picks = pages.shape[1]
+    need(pages, "pages", (t, picks), torch.int32, dev)
+    args = _lib.PromptAttentionArgs(
+        q=q.data_ptr(), tokens=t, heads=heads, req=req.data_ptr(), pos=pos.data_ptr(), pages=pages.data_ptr(), picks=picks,
+        page_table=page_table.data_ptr(), requests=page_table.shape[0], pt_stride=page_table.shape[1], n_pages=n_pages,
+        kv=caches.kv.data_ptr(), kv_scale=_lib.ptr(caches.kv_scale), softmax_scale=softmax_scale, out=out.data_ptr(),
+    )  # fmt: skip
+    lib = _lib.lib()
+    ws = _workspace(args, lib.mono_prompt_attention_workspace(t, heads, picks), dev)  # noqa: F841 (held over the call)
+    _enqueue(dev, lib.mono_prompt_attention, args)
+    return out
+
+
+def tree_attention(q: torch.Tensor, starts: torch.Tensor, prefix: torch.Tensor, mask: torch.Tensor, page_table: torch.Tensor,
+                   caches: AttnCaches, softmax_scale: float = SOFTMAX_SCALE, out: torch.Tensor | None = None) -> torch.Tensor:
+    """MLA attention of drafted tokens, a tree a request, over the whole cached prefix: ``q`` bf16
+    [nodes, heads, 576] as ``attention`` takes it -> [nodes, heads, 512] bf16. Request r (a row
+    of ``page_table``) has ``prefix[r]`` keys and the nodes ``starts[r]`` .. ``starts[r + 1]`` - 1
+    (i32 [requests] and [requests + 1]); the key of its node i lies at position ``prefix[r]`` + i
+    (``append`` with ``slot_pos``). A node sees the prefix and, for each bit j of its ``mask``
+    (i64 [nodes]: the node itself and its ancestors), the key at ``prefix[r]`` + j. A node of no
+    request, and one that sees nothing, has zeros. ``out`` must share no memory with ``q``."""
+    dev = _gpu(q, "q")
+    n_pages, out = _latents(q, caches, out, dev)
+    t, heads = q.shape[:2]
+    _table(page_table, dev)
+    requests, width = page_table.shape
+    need(starts, "starts", (requests + 1,), torch.int32, dev)
+    need(prefix, "prefix", (requests,), torch.int32, dev)
+    need(mask, "mask", (t,), torch.int64, dev)
+    args = _lib.PromptTreeArgs(
+        q=q.data_ptr(), nodes=t, heads=heads, starts=starts.data_ptr(), prefix=prefix.data_ptr(), mask=mask.data_ptr(),
+        page_table=page_table.data_ptr(), requests=requests, pt_stride=width, n_pages=n_pages, kv=caches.kv.data_ptr(),
+        kv_scale=_lib.ptr(caches.kv_scale), softmax_scale=softmax_scale, out=out.data_ptr(),
+    )  # fmt: skip
+    lib = _lib.lib()
+    ws = _workspace(args, lib.mono_prompt_tree_workspace(t, heads, width), dev)  # noqa: F841 (held over the call)
+    _enqueue(dev, lib.mono_prompt_tree, args)
     return out
