@@ -26,26 +26,29 @@ namespace {
 
 constexpr int T = 256, WAVES = 4, ROW = LATENT + PE, PAGE_BYTES = PAGE * ROW;
 constexpr int BLOCKS = ROW / 64, BLOCK_BYTES = PAGE * 64;  // a page's rows in blocks of 64 dims
-constexpr int DT = LATENT / WAVES / 16;                   // tiles of 16 dims a wave
-constexpr int AHEAD = 2;                                  // blocks read before they are used
+constexpr int DT = LATENT / WAVES / 32;                   // tiles of 32 dims a wave
+constexpr int HEADS = 32;                                 // columns of the values' MFMAs
 // NONE: no maximum yet, so low that any logit passes it (and finite: what is taken from it is a number)
-constexpr float NEG_INF = -__builtin_inff(), NONE = -1e38f, SLACK = 8.0f;
+constexpr float NEG_INF = -__builtin_inff(), NONE = -1e38f, EXP2_SLACK = 16.0f;
 
 // A page and its keys' scales.
 struct Stage {
   alignas(16) uint8_t kv[PAGE_BYTES];
   float scale[PAGE];
 };
-template <int MT>
+constexpr int P_PITCH = PAGE + 8;  // (8 heads' 16 bytes fall on distinct banks)
 struct Lds {
-  Stage stage[2];
-  alignas(16) uint16_t p[16 * MT][PAGE + 8];
-  float top[WAVES][16 * MT], sum[WAVES][16 * MT];
+  Stage stage[2];  // (at the start the second holds q's pieces, at the end both the outputs' rows)
+  alignas(16) uint16_t p[HEADS][P_PITCH];
+  float top[WAVES][HEADS];  // the waves' maxima, at the end their sums
+  float by[HEADS];          // what a head's sums are scaled by
+  uint32_t q_scale[HEADS];
   int over[WAVES];
   int slot[WAVE];       // a run of 64 pages of the list: where each lies in the pool
   uint64_t seen[WAVE];  // and which of its keys are seen
 };
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lvoid;
 typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
@@ -73,11 +76,35 @@ MONO_DEV void dma4(const float* base, uint32_t offset, void* to) {
 // 8 (l % 2) .. of row l / 2 and gets byte l of each of the 8 rows.
 MONO_DEV u32x2 lds_transposed(const uint8_t* p) { return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)p)); }
 
-MONO_DEV bf16x8 widen8(uint32_t lo, uint32_t hi) {
+// E4M3 x E4M3; the second operand's lanes have scales, byte B of `scale`
+template <int B>
+MONO_DEV f32x4 mfma_16(const i32x8& a, const i32x8& b, const f32x4& c, int scale) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 127, B, scale);
+}
+// C[32 x 32] += A[32 x 16] B[16 x 32] in bf16; lane l: row / column l % 32, k 8 (l / 32) .. + 7
+MONO_DEV f32x16 mfma_32(const bf16x8& a, const bf16x8& b, const f32x16& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+MONO_DEV bf16x8 widen8(const u32x2& w) {
   bf16x8 v;
-  widen4(lo, v, 0);
-  widen4(hi, v, 4);
+  widen4(w[0], v, 0);
+  widen4(w[1], v, 4);
   return v;
+}
+MONO_DEV i32x8 join(const u32x4& lo, const u32x4& hi) {
+  return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+
+// Four values of at most 448 x `unit` (a power of two) as two E4M3 pieces each: the nearest
+// multiple of `unit`, and what is left in multiples of `fine`.
+MONO_DEV void two_pieces(const float (&v)[4], float unit, float fine, uint32_t& hi, uint32_t& lo) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  i16x2 h = {0, 0}, l = {0, 0};
+  h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, v[0], v[1], unit, false);
+  h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, v[2], v[3], unit, true);
+  hi = __builtin_bit_cast(uint32_t, h);
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, unit, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, unit, true);
+  l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, v[0] - a[0], v[1] - a[1], fine, false);
+  l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, v[2] - b[0], v[3] - b[1], fine, true);
+  lo = __builtin_bit_cast(uint32_t, l);
 }
 
 // A page in LDS: block by block of 64 dims, in each the keys' 64 bytes as four units of 16,
@@ -174,7 +201,7 @@ MONO_DEV bool reads_of(const Paged& a, int64_t t, int split, Reads& rd) {
 
 template <int MT, bool TREE>
 __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
-  __shared__ Lds<MT> L;
+  __shared__ Lds L;
   const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   // the XCDs (workgroup b runs on XCD b mod 8) take neighbouring work each: neighbouring tokens
   // read many of the same pages, which one L2 then holds
@@ -188,14 +215,14 @@ __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
   Reads rd;
   const bool any = reads_of<TREE>(a, t, split, rd);
 
-  f32x4 o[DT][MT];
+  f32x16 o[DT];  // of lane l: dims 128 wave + 32 t + 8 (i / 4) + 4 (l / 32) + i % 4 of head l % 32
   float m_ref[MT], l_run[MT];
 #pragma unroll
-  for (int c = 0; c < MT; ++c) {
-    m_ref[c] = NONE, l_run[c] = 0.f;
+  for (int c = 0; c < MT; ++c) m_ref[c] = NONE, l_run[c] = 0.f;
 #pragma unroll
-    for (int b = 0; b < DT; ++b) o[b][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int b = 0; b < DT; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
   if (any) {
     int buf = 0;
     uint64_t live = 0;  // pages left of a run of 64 of the list
@@ -232,121 +259,161 @@ __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
     };
     int at = rd.lo;
     run_from(at);
-    bf16x8 q[MT][2 * BLOCKS];  // (behind the first page, which more steps led to)
+    // q's heads as two pieces (behind the first page, which more steps led to): wave w's eight
+    // heads, 8 lanes each, through LDS to all the waves
+    if (wave < 2 * MT) {
+      const uint32_t ln = lane_now(lane), head = 8 * wave + ln / 8;
+      const uint16_t* row = static_cast<const uint16_t*>(a.q) + (t * a.heads + min(h0 + (int)head, a.heads - 1)) * ROW + 8 * (ln % 8);
+      u32x4 v[BLOCKS];
+      uint32_t most = 0;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        v[b] = ld_u32x4(row + 64 * b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = max(most, max(v[b][i] & 0x7fffu, v[b][i] >> 16 & 0x7fffu));
+      }
+      most = max(most, dpp_u<DPP_XOR1>(most));
+      most = max(most, dpp_u<DPP_XOR2>(most));
+      most = max(most, dpp_u<DPP_HALF_MIRROR>(most));
+      // the power of two that puts the largest into (224, 448]
+      const uint32_t e = max((most >> 7) + ((most & 0x7fu) > 0x60u ? 1u : 0u), 16u);
+      const bool finite = most < 0x7f80u;
+      const float unit = __uint_as_float((finite ? e - 8u : 127u) << 23), fine = unit * 0.0625f;
+      // (q that is not finite: scales that are NaN, and so are its outputs)
+      if (ln % 8 == 0) L.q_scale[head] = finite ? (e - 8u) | (e - 12u) << 8 : 0xffffu;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        u32x2 piece[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float x[4] = {bf16_lo(v[b][2 * h]), bf16_hi(v[b][2 * h]), bf16_lo(v[b][2 * h + 1]), bf16_hi(v[b][2 * h + 1])};
+          uint32_t hi, lo;
+          two_pieces(x, unit, b < BLOCKS - 1 ? fine : unit, hi, lo);
+          piece[0][h] = hi, piece[1][h] = lo;
+        }
+        uint8_t* to = &L.stage[1].kv[head * ROW + 64 * b + 16 * unit_of(head, ln % 8 / 2) + 8 * (ln % 2)];
+        *reinterpret_cast<u32x2*>(to) = piece[0];
+        *reinterpret_cast<u32x2*>(to + 16 * MT * ROW) = piece[1];
+      }
+    }
+    static_assert(2 * HEADS * ROW <= PAGE_BYTES, "q's pieces fit a page's place");
+    if (MT == 1 && wave == 3)  // columns that are no heads
+      for (int u = lane; u < 16 * P_PITCH / 8; u += WAVE) reinterpret_cast<u32x4*>(L.p[16])[u] = u32x4{0u, 0u, 0u, 0u};
+    meet();
+    // lane (g, r): of head 16 c + r units g of the blocks of 64 dims, two blocks an MFMA; of the last
+    // block both pieces in one
+    i32x8 q[MT][BLOCKS];  // pieces of blocks 0 and 1, 2 and 3, ..; then the last
+    int q_scale = 0;
     {
       const uint32_t ln = lane_now(lane), r = ln % 16, g = ln / 16;
-      // q of heads 16 c + r: dims 64 b + 16 g + 8 h .. + 7 (the order in which a lane reads a row's units)
 #pragma unroll
       for (int c = 0; c < MT; ++c) {
-        const uint16_t* row = static_cast<const uint16_t*>(a.q) + (t * a.heads + min(h0 + 16 * c + (int)r, a.heads - 1)) * ROW + 16 * g;
+        const uint8_t* row = &L.stage[1].kv[(16 * c + r) * ROW + 16 * unit_of(r, g)];
+        const auto unit = [&](int piece, int b) { return *reinterpret_cast<const u32x4*>(row + piece * 16 * MT * ROW + 64 * b); };
 #pragma unroll
-        for (int k = 0; k < 2 * BLOCKS; ++k) q[c][k] = __builtin_bit_cast(bf16x8, ld_u32x4(row + 64 * (k / 2) + 8 * (k % 2)));
+        for (int k = 0; k < BLOCKS / 2; ++k)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) q[c][2 * k + h] = join(unit(h, 2 * k), unit(h, 2 * k + 1));
+        q[c][BLOCKS - 1] = join(unit(0, BLOCKS - 1), unit(1, BLOCKS - 1));
+        q_scale |= (int)(L.q_scale[16 * c + r] << 16 * c);
       }
     }
     for (;;) {
+      // of the page that comes first, which keys are seen; where the one after it lies
+      uint64_t mask = 0;
+      int64_t ahead = 0;
+      const auto seen_at = [&](uint64_t m) {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)m) |
+               (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(m >> 32)) << 32;
+      };
+      if (live) {
+        const uint64_t rest = live & (live - 1);
+        mask = seen_at(L.seen[__builtin_ctzll(live)]);
+        ahead = place_of(__builtin_ctzll(rest ? rest : live));
+      }
       while (live) {  // a page, while the next one of the run comes
         Stage &st = L.stage[buf], &next = L.stage[buf ^ 1];
-        const int i = __builtin_ctzll(live);
         live &= live - 1;
         meet_after_loads();  // the page has come, and every wave is done with the one before
-        const uint64_t seen_here = L.seen[i];
-        const uint64_t mask = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)seen_here) |
-                              (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(seen_here >> 32)) << 32;
-        const bool partial = mask != ~0ull;
+        const bool partial = mask != ~0ull, more = live != 0;
         if (partial) {  // what is not seen may hold anything, a NaN too: zeros instead
           const uint32_t ln = lane_now(lane);
-          if (!(mask >> (16 * wave + ln / 4) & 1))
+          if (!(mask >> (16 * wave + ln / 4) & 1)) {
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) *reinterpret_cast<u32x4*>(&st.kv[b * BLOCK_BYTES + 1024 * wave + 16 * ln]) = u32x4{0u, 0u, 0u, 0u};
+            if (ln % 4 == 0) st.scale[16 * wave + ln / 4] = 0.f;
+          }
           meet();
         }
-        const bool more = live != 0;
-        const int64_t ahead = place_of(more ? __builtin_ctzll(live) : i);
         if (more) bring_scales(ahead, next);
-
         f32x4 s[MT];
 #pragma unroll
         for (int c = 0; c < MT; ++c) s[c] = f32x4{0.f, 0.f, 0.f, 0.f};
         {
-          const uint32_t ln = lane_now(lane);
-          const uint32_t at_lane = lane_place();
+          const uint32_t ln = lane_now(lane), at_lane = lane_place();
           const uint8_t* key = &st.kv[(16 * wave + ln % 16) * 64 + 16 * unit_of(ln % 16, ln / 16)];
-          u32x4 w[AHEAD];  // (the order of reads, conversions and MFMAs is held: left alone, each read is waited for at once)
+          const auto unit = [&](int b) { return *reinterpret_cast<const u32x4*>(key + BLOCK_BYTES * b); };
 #pragma unroll
-          for (int b = 0; b < AHEAD; ++b) w[b] = *reinterpret_cast<const u32x4*>(key + BLOCK_BYTES * b);
-          __builtin_amdgcn_sched_barrier(0);
+          for (int k = 0; k < BLOCKS / 2 + 1; ++k) {
+            const i32x8 keys = k < BLOCKS / 2 ? join(unit(2 * k), unit(2 * k + 1)) : join(unit(2 * k), unit(2 * k));
+            if (k < BLOCKS / 2) {
 #pragma unroll
-          for (int b = 0; b < BLOCKS; ++b) {
-            const bf16x8 k0 = widen8(w[b % AHEAD][0], w[b % AHEAD][1]);
+              for (int c = 0; c < MT; ++c) s[c] = c ? mfma_16<2>(keys, q[c][2 * k], s[c], q_scale) : mfma_16<0>(keys, q[c][2 * k], s[c], q_scale);
+              bring(ahead, at_lane, next, 2 * k, more);  // (nine DMAs at once hold the wave up for 1000 cycles)
 #pragma unroll
-            for (int c = 0; c < MT; ++c) s[c] = mfma_bf16(k0, q[c][2 * b], s[c]);
-            __builtin_amdgcn_sched_barrier(0);
-            const bf16x8 k1 = widen8(w[b % AHEAD][2], w[b % AHEAD][3]);
-            if (b + AHEAD < BLOCKS) w[b % AHEAD] = *reinterpret_cast<const u32x4*>(key + BLOCK_BYTES * (b + AHEAD));
+              for (int c = 0; c < MT; ++c) s[c] = c ? mfma_16<3>(keys, q[c][2 * k + 1], s[c], q_scale) : mfma_16<1>(keys, q[c][2 * k + 1], s[c], q_scale);
+              bring(ahead, at_lane, next, 2 * k + 1, more);
+            } else {
 #pragma unroll
-            for (int c = 0; c < MT; ++c) s[c] = mfma_bf16(k1, q[c][2 * b + 1], s[c]);
-            bring(ahead, at_lane, next, b, more);  // (nine DMAs at once hold the wave up for 1000 cycles)
+              for (int c = 0; c < MT; ++c) s[c] = c ? mfma_16<2>(keys, q[c][2 * k], s[c], q_scale) : mfma_16<0>(keys, q[c][2 * k], s[c], q_scale);
+              bring(ahead, at_lane, next, 2 * k, more);
+            }
             __builtin_amdgcn_sched_barrier(0);
           }
         }
+#pragma unroll
+        for (int c = 0; c < MT; ++c) asm volatile("" : "+v"(s[c]));  // (formed here, not where they are used)
         // lane (g, r): keys 16 wave + 4 g + j of head 16 c + r
         const uint32_t first_key = 16 * wave + lane_now(lane) / 16 * 4;
         f32x4 ks = {1.f, 1.f, 1.f, 1.f}, by;
         if (a.kv_scale) ks = *reinterpret_cast<const f32x4*>(&st.scale[first_key]);
-        const uint32_t mine = partial ? (uint32_t)(mask >> first_key) : 15u;
-        if (partial)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) ks[j] = mine >> j & 1 ? ks[j] : 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) by[j] = ks[j] * a.scale_log2;
+        if (partial) {  // (a logit of minus infinity, whatever the scale's sign)
+          const uint32_t mine = (uint32_t)(mask >> first_key);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            by[j] = mine >> j & 1 ? by[j] : 1.f;
+#pragma unroll
+            for (int c = 0; c < MT; ++c) s[c][j] = mine >> j & 1 ? s[c][j] : NEG_INF;
+          }
+        }
         float ps[MT];
-        const auto weigh = [&]() {  // the probabilities to LDS, and whether one is over 2^SLACK
+        const auto weigh = [&]() {  // the probabilities to LDS, and whether one of the workgroup's is over EXP2_SLACK
           const uint32_t ln = lane_now(lane);
-          float top = NEG_INF;
+          uint16_t* to = &L.p[ln % 16][16 * wave + ln / 16 * 4];
+          float top = 0.f;
 #pragma unroll
           for (int c = 0; c < MT; ++c) {
             float y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = fmaf(s[c][j], by[j], -m_ref[c]);
-            if (partial)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) y[j] = mine >> j & 1 ? y[j] : NEG_INF;
-            top = fmaxf(fmaxf(top, fmaxf(y[0], y[1])), fmaxf(y[2], y[3]));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = __builtin_amdgcn_exp2f(y[j]);
+            for (int j = 0; j < 4; ++j) y[j] = __builtin_amdgcn_exp2f(fmaf(s[c][j], by[j], -m_ref[c]));
             ps[c] = (y[0] + y[1]) + (y[2] + y[3]);
-            *reinterpret_cast<u32x2*>(&L.p[16 * c + ln % 16][16 * wave + 4 * (ln / 16)]) =
-                u32x2{pack2(y[0] * ks[0], y[1] * ks[1]), pack2(y[2] * ks[2], y[3] * ks[3])};
+            top = fmaxf(fmaxf(top, fmaxf(y[0], y[1])), fmaxf(y[2], y[3]));
+            *reinterpret_cast<u32x2*>(to + c * 16 * P_PITCH) = u32x2{pack2(y[0] * ks[0], y[1] * ks[1]), pack2(y[2] * ks[2], y[3] * ks[3])};
+            __builtin_amdgcn_sched_barrier(0);
           }
-          return top > SLACK;
+          const bool over = __any(top > EXP2_SLACK);
+          if (lane == 0) L.over[wave] = over;
+          meet();
+          return __builtin_amdgcn_readfirstlane(L.over[0] | L.over[1] | L.over[2] | L.over[3]);
         };
-        const bool over = __any(weigh());
-        if (lane == 0) L.over[wave] = over;
-        meet();
-        const int any_over = L.over[0] | L.over[1] | L.over[2] | L.over[3];
-        // the values, transposed: dims 128 wave + 16 b .. of 32 keys a step; the first reads already here
-        constexpr int N = PAGE / 32 * DT, VAHEAD = 4;
-        u32x2 vw[VAHEAD];
-        const auto value_place = [&]() {
-          const uint32_t ln = lane_now(lane);
-          return &st.kv[2 * wave * BLOCK_BYTES + (8 * (ln / 16) + ln % 16 / 2) * 64 + 8 * (ln % 2)];
-        };
-        const auto read = [&](const uint8_t* keys, uint32_t swap, int i) {
-          vw[i % VAHEAD] = lds_transposed(keys + i / DT * 2048 + i % DT / 4 * BLOCK_BYTES + 16 * (swap ^ i % 4));
-        };
-        const auto first_reads = [&]() {
-          const uint8_t* keys = value_place();
-          const uint32_t swap = unit_of(lane_now(lane) % 16 / 2, 0);
-#pragma unroll
-          for (int i = 0; i < VAHEAD; ++i) read(keys, swap, i);
-        };
-        first_reads();
-        if (__builtin_amdgcn_readfirstlane(any_over)) {
+        if (weigh()) {
 #pragma unroll
           for (int c = 0; c < MT; ++c) {
             float m = NONE;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) m = fmaxf(m, mine >> j & 1 ? s[c][j] * by[j] : NONE);
+            for (int j = 0; j < 4; ++j) m = fmaxf(m, s[c][j] * by[j]);
             m = groups_max(m);
             if (lane_now(lane) < 16) L.top[wave][16 * c + lane_now(lane)] = m;
           }
@@ -359,35 +426,49 @@ __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
             const float by = __builtin_amdgcn_exp2f(m_ref[c] - m);
             m_ref[c] = m;
             l_run[c] *= by;
-#pragma unroll
-            for (int b = 0; b < DT; ++b)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) o[b][c][j] *= by;
+            if (wave == 0 && lane_now(lane) < 16) L.by[16 * c + lane_now(lane)] = by;
           }
           weigh();
-          meet();
-          first_reads();  // (again: held across this path they would spill)
+          const float by = L.by[lane_now(lane) % HEADS];
+#pragma unroll
+          for (int b = 0; b < DT; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[b][i] *= by;
         }
 #pragma unroll
         for (int c = 0; c < MT; ++c) l_run[c] += ps[c];
 
+        // the values, transposed and widened: 32 dims x 16 keys against 16 keys x 32 heads
         {
-          const uint8_t* keys = value_place();
-          const uint32_t ln = lane_now(lane), swap = unit_of(ln % 16 / 2, 0);
-          bf16x8 pk[MT];
+          const uint32_t ln = lane_now(lane), half = ln / 32;
+          const uint16_t* pr = &L.p[ln % 32][8 * half];
+          // lane l reads bytes of key 16 k + 8 half + l % 16 / 2 and gets one dim of the eight keys
+          const uint8_t* keys = &st.kv[2 * wave * BLOCK_BYTES + (8 * half + ln % 16 / 2) * 64 + 8 * (ln % 2)];
+          const uint32_t swap = unit_of(ln % 16 / 2, ln / 16 % 2);
+          constexpr int N = PAGE / 16 * DT, VAHEAD = 4;  // (tile i % DT of keys 16 (i / DT) ..)
+          u32x2 w[VAHEAD];
+          bf16x8 pk[2];
+          const auto read = [&](int i) {
+            w[i % VAHEAD] = lds_transposed(keys + i % DT / 2 * BLOCK_BYTES + 16 * (swap ^ 2 * (i % 2)) + 1024 * (i / DT));
+          };
+          const auto read_p = [&](int k) { pk[k % 2] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(pr + 16 * k)); };
+          read_p(0);
+#pragma unroll
+          for (int i = 0; i < VAHEAD; ++i) read(i);
+          const uint64_t rest = live & (live - 1);
+          const int next_i = more ? __builtin_ctzll(live) : 0, after_i = __builtin_ctzll(rest ? rest : more ? live : 1);
+          const uint64_t next_seen = L.seen[next_i];
+          const int after_slot = L.slot[after_i];
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            if (i % DT == 0) {
-#pragma unroll
-              for (int c = 0; c < MT; ++c)
-                pk[c] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(&L.p[16 * c + ln % 16][32 * (i / DT) + 8 * (ln / 16)]));
-            }
-            const bf16x8 v = widen8(vw[i % VAHEAD][0], vw[i % VAHEAD][1]);
-            if (i + VAHEAD < N) read(keys, swap, i + VAHEAD);
-#pragma unroll
-            for (int c = 0; c < MT; ++c) o[i % DT][c] = mfma_bf16(v, pk[c], o[i % DT][c]);
+            if (i % DT == 0 && i + DT < N) read_p(i / DT + 1);
+            const bf16x8 v = widen8(w[i % VAHEAD]);
+            if (i + VAHEAD < N) read(i + VAHEAD);
+            o[i % DT] = mfma_32(v, pk[i / DT % 2], o[i % DT]);
             __builtin_amdgcn_sched_barrier(0);
           }
+          mask = seen_at(next_seen);
+          ahead = (int64_t)__builtin_amdgcn_readfirstlane(after_slot) * PAGE;
         }
         buf ^= 1;
       }
@@ -397,53 +478,50 @@ __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
     }
   }
 
-  const int tid = wave * WAVE + (int)lane_now(lane), g = tid % WAVE / 16, r = tid % 16;
   // the heads' sums: over the lane groups, then the waves
-  float l[MT];
+  const int tid = wave * WAVE + (int)lane_now(lane), ln = tid % WAVE, heads = min(16 * MT, a.heads - h0);
   __syncthreads();  // (the last page's readers)
 #pragma unroll
   for (int c = 0; c < MT; ++c) {
-    l[c] = groups_sum(l_run[c]);
-    if (g == 0) L.sum[wave][16 * c + r] = l[c];
+    const float l = groups_sum(l_run[c]);
+    if (ln < 16) L.top[wave][16 * c + ln] = l;
+    if (wave == 0 && ln < 16) L.by[16 * c + ln] = m_ref[c];
   }
   __syncthreads();
-#pragma unroll
-  for (int c = 0; c < MT; ++c) {
-    l[c] = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) l[c] += L.sum[w][16 * c + r];
-  }
-  const int heads = min(16 * MT, a.heads - h0);
+  const auto sum_of = [&](int head) { return (L.top[0][head] + L.top[1][head]) + (L.top[2][head] + L.top[3][head]); };
+  // the outputs through LDS, so that rows go out whole
+  const int head = ln % HEADS, dim0 = 128 * wave + 4 * (ln / HEADS);
   if (a.splits > 1) {
     const int64_t first = (t * a.splits + split) * a.heads + h0;  // this split's rows of the parts
-    if (wave == 0 && g == 0)
-#pragma unroll
-      for (int c = 0; c < MT; ++c)
-        if (16 * c + r < heads) {
-          a.part_m[first + 16 * c + r] = l[c] == 0.f ? NEG_INF : m_ref[c];
-          a.part_l[first + 16 * c + r] = l[c];
-        }
+    if (tid < heads) {
+      const float l = sum_of(tid);
+      a.part_m[first + tid] = l == 0.f ? NEG_INF : L.by[tid];
+      a.part_l[first + tid] = l;
+    }
     if (!any) return;
-#pragma unroll
-    for (int c = 0; c < MT; ++c)
-      if (16 * c + r < heads)
-#pragma unroll
-        for (int b = 0; b < DT; ++b)
-          *reinterpret_cast<f32x4*>(a.part + (first + 16 * c + r) * LATENT + 16 * (DT * wave + b) + 4 * g) = o[b][c];
-    return;
-  }
-  // through LDS, so that rows go out whole
-  uint16_t* stage = reinterpret_cast<uint16_t*>(L.stage[0].kv);
-  constexpr int PITCH = LATENT + 8;
-  static_assert(16 * MT * PITCH * 2 <= PAGE_BYTES, "the outputs fit a page's place");
-#pragma unroll
-  for (int c = 0; c < MT; ++c) {
-    const float by = l[c] == 0.f ? 0.f : 1.0f / l[c];
+    float* stage = reinterpret_cast<float*>(&L.stage);
+    constexpr int PITCH = LATENT + 4;
+    static_assert(HEADS * PITCH * 4 <= sizeof L.stage, "the parts fit the pages' places");
 #pragma unroll
     for (int b = 0; b < DT; ++b)
-      *reinterpret_cast<u32x2*>(stage + (16 * c + r) * PITCH + 16 * (DT * wave + b) + 4 * g) =
-          u32x2{pack_bf16x2(o[b][c][0] * by, o[b][c][1] * by), pack_bf16x2(o[b][c][2] * by, o[b][c][3] * by)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(stage + head * PITCH + dim0 + 32 * b + 8 * i) = f32x4{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]};
+    __syncthreads();
+    float* part = a.part + first * LATENT;
+    for (int u = tid; u < heads * (LATENT / 4); u += T)
+      *reinterpret_cast<f32x4*>(part + 4 * u) = *reinterpret_cast<const f32x4*>(stage + u / (LATENT / 4) * PITCH + u % (LATENT / 4) * 4);
+    return;
   }
+  uint16_t* stage = reinterpret_cast<uint16_t*>(&L.stage);
+  constexpr int PITCH = LATENT + 8;
+  const float l = sum_of(head < 16 * MT ? head : 0), inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+  for (int b = 0; b < DT; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<u32x2*>(stage + head * PITCH + dim0 + 32 * b + 8 * i) =
+          u32x2{pack2(o[b][4 * i] * inv, o[b][4 * i + 1] * inv), pack2(o[b][4 * i + 2] * inv, o[b][4 * i + 3] * inv)};
   __syncthreads();
   uint16_t* out = static_cast<uint16_t*>(a.out) + (t * a.heads + h0) * LATENT;
   for (int u = tid; u < heads * (LATENT / 8); u += T)
