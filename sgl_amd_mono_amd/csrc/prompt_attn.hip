@@ -152,7 +152,7 @@ MONO_DEV float groups_sum(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// What a workgroup reads: a token's pages [lo, hi) of its list (attention) or of its request's
+// What a workgroup reads: pages [lo, hi) of a token's list (attention) or of its request's
 // (tree), and which keys of each are seen.
 struct Reads {
   const int32_t* table;  // the request's row of the page table
@@ -170,51 +170,110 @@ MONO_DEV uint64_t seen_of(const Reads& rd, int page, bool tree) {
   return m;
 }
 
+// A workgroup's task: a token (node), heads 16 MT ht .., chunk `chunk` of `chunks` of its pages, whose
+// parts are rows of part `part` (chunks > 1).
+struct Task {
+  int64_t t;
+  int ht, chunk, chunks;
+  int64_t part;
+  bool any;  // it has pages
+};
+
+MONO_DEV void node_reads(const Paged& a, int64_t t, int req, Reads& rd) {
+  rd.table = a.page_table + (int64_t)req * a.pt_stride;
+  rd.end = max(a.prefix[req], 0);
+  rd.draft = (uint64_t)a.mask[t];
+}
+
+// Request r's nodes and pages (the last one or two hold the draft's keys).
+MONO_DEV void request_of(const Paged& a, int r, int64_t& first, int& n, int& pages) {
+  first = min((int64_t)max(a.starts[r], 0), a.tokens);
+  n = (int)max(min((int64_t)a.starts[r + 1], a.tokens) - first, (int64_t)0);
+  pages = n ? (int)min((int64_t)min(a.pt_stride, 1 << 20), ((int64_t)max(a.prefix[r], 0) + PAGE - 1) / PAGE + 1) : 0;
+}
+
+// Trees of few nodes: each node's pages in chunks of `each`, a request's nodes side by side over
+// the same chunk. As many pages a chunk as make one round of tasks of them, each node's last chunk
+// being a short one.
+MONO_DEV int chunk_pages(const Paged& a, int lane) {
+  int total = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += WAVE) {
+    int64_t first;
+    int n = 0, pages = 0;
+    if (r0 + lane < a.requests) request_of(a, r0 + lane, first, n, pages);
+    total += wave_sum_i(n * pages);
+  }
+  const int tasks = a.tasks - (int)a.tokens * a.head_tiles;
+  return max((int)(((int64_t)total * a.head_tiles + tasks - 1) / tasks), 1);
+}
+
+// Task `id` of them; false behind the last.
+MONO_DEV bool planned_task(const Paged& a, int lane, int each, int id, Task& k, Reads& rd) {
+  k.ht = id % a.head_tiles;
+  id /= a.head_tiles;
+  int part = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += WAVE) {
+    int64_t first = 0;
+    int n = 0, pages = 0;
+    if (r0 + lane < a.requests) request_of(a, r0 + lane, first, n, pages);
+    const int chunks = (pages + each - 1) / each, tasks = n * chunks, parts = chunks > 1 ? tasks : 0;
+    const int upto = wave_incl_scan(tasks), parts_upto = wave_incl_scan(parts);
+    const uint64_t here = __ballot(upto > id);
+    if (here) {
+      const int l = __builtin_ctzll(here);
+      const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      const int nodes = of(n), at = id - (of(upto) - of(tasks)), node = at % nodes;
+      k.chunk = at / nodes;
+      k.chunks = of(chunks);
+      k.part = part + of(parts_upto) - of(parts) + node * k.chunks + k.chunk;
+      k.t = (int64_t)of((int)first) + node;
+      node_reads(a, k.t, r0 + l, rd);
+      rd.lo = k.chunk * each;
+      rd.hi = min(rd.lo + each, of(pages));
+      k.any = true;
+      return k.part < a.parts;  // (starts that do not ascend: nothing is written behind the parts)
+    }
+    id -= __builtin_amdgcn_readlane(upto, WAVE - 1);
+    part += __builtin_amdgcn_readlane(parts_upto, WAVE - 1);
+  }
+  return false;
+}
+
 template <bool TREE>
-MONO_DEV bool reads_of(const Paged& a, int64_t t, int split, Reads& rd) {
+MONO_DEV void task_of(const Paged& a, int lane, int64_t id, Task& k, Reads& rd) {
+  k.ht = (int)(id % a.head_tiles);
+  const int64_t rest = id / a.head_tiles;
+  k.t = rest / a.splits, k.chunk = (int)(rest % a.splits), k.chunks = a.splits;
+  k.part = rest;
+  k.any = false;
   int pages;
   if (TREE) {
     // the request whose nodes hold t: as many starts as are at most t
-    const int lane = threadIdx.x % WAVE;
-    int req = -1, at = 0;
-    for (int r0 = 0; r0 <= a.requests; r0 += WAVE) at += __popcll(__ballot(r0 + lane <= a.requests && a.starts[min(r0 + lane, a.requests)] <= t));
-    req = at - 1;
-    if (req < 0 || req >= a.requests) return false;
-    rd.table = a.page_table + (int64_t)req * a.pt_stride;
-    rd.end = max(a.prefix[req], 0);
-    rd.draft = (uint64_t)a.mask[t];
+    int at = 0;
+    for (int r0 = 0; r0 <= a.requests; r0 += WAVE) at += __popcll(__ballot(r0 + lane <= a.requests && a.starts[min(r0 + lane, a.requests)] <= k.t));
+    if (at < 1 || at > a.requests) return;
+    node_reads(a, k.t, at - 1, rd);
     const int drafted = rd.draft ? 64 - __builtin_clzll(rd.draft) : 0;
     pages = (int)min((int64_t)a.pt_stride, (rd.end + drafted + PAGE - 1) / PAGE);
   } else {
-    const int req = a.req[t], pos = a.pos[t];
-    if (req < 0 || req >= a.requests || pos < 0) return false;
+    const int req = a.req[k.t], pos = a.pos[k.t];
+    if (req < 0 || req >= a.requests || pos < 0) return;
     rd.table = a.page_table + (int64_t)req * a.pt_stride;
-    rd.list = a.pages + t * a.picks;
+    rd.list = a.pages + k.t * a.picks;
     rd.end = (int64_t)pos + 1;
     rd.draft = 0;
     pages = a.picks;
   }
-  rd.lo = (int)((int64_t)pages * split / a.splits);
-  rd.hi = (int)((int64_t)pages * (split + 1) / a.splits);
-  return rd.lo < rd.hi;
+  rd.lo = (int)((int64_t)pages * k.chunk / k.chunks);
+  rd.hi = (int)((int64_t)pages * (k.chunk + 1) / k.chunks);
+  k.any = rd.lo < rd.hi;
 }
 
 template <int MT, bool TREE>
-__global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
-  __shared__ Lds L;
-  const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  // the XCDs (workgroup b runs on XCD b mod 8) take neighbouring work each: neighbouring tokens
-  // read many of the same pages, which one L2 then holds
-  const int64_t each = (a.work + 7) / 8, id = blockIdx.x % 8 * each + blockIdx.x / 8;
-  if (blockIdx.x / 8 >= each || id >= a.work) return;
-  const int ht = (int)(id % a.head_tiles);
-  const int64_t rest = id / a.head_tiles;
-  // attention: a token's splits side by side; tree: a split's nodes
-  const int64_t t = TREE ? rest % a.tokens : rest / a.splits;
-  const int split = (int)(TREE ? rest / a.tokens : rest % a.splits), h0 = ht * 16 * MT;
-  Reads rd;
-  const bool any = reads_of<TREE>(a, t, split, rd);
-
+MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& task, const Reads& rd) {
+  const int64_t t = task.t;
+  const int h0 = task.ht * 16 * MT;
+  const bool any = task.any;
   f32x16 o[DT];  // of lane l: dims 128 wave + 32 t + 8 (i / 4) + 4 (l / 32) + i % 4 of head l % 32
   float m_ref[MT], l_run[MT];
 #pragma unroll
@@ -491,8 +550,8 @@ __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
   const auto sum_of = [&](int head) { return (L.top[0][head] + L.top[1][head]) + (L.top[2][head] + L.top[3][head]); };
   // the outputs through LDS, so that rows go out whole
   const int head = ln % HEADS, dim0 = 128 * wave + 4 * (ln / HEADS);
-  if (a.splits > 1) {
-    const int64_t first = (t * a.splits + split) * a.heads + h0;  // this split's rows of the parts
+  if (task.chunks > 1) {
+    const int64_t first = task.part * a.heads + h0;  // this chunk's rows of the parts
     if (tid < heads) {
       const float l = sum_of(tid);
       a.part_m[first + tid] = l == 0.f ? NEG_INF : L.by[tid];
@@ -528,74 +587,114 @@ __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
     *reinterpret_cast<u32x4*>(out + 8 * u) = *reinterpret_cast<const u32x4*>(stage + u / (LATENT / 8) * PITCH + u % (LATENT / 8) * 8);
 }
 
-// A head's parts as one, each scaled to the largest of their maxima. A wave takes every fourth
+template <int MT, bool TREE, bool PLANNED>
+__global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
+  __shared__ Lds L;
+  const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  // the XCDs (workgroup b runs on XCD b mod 8) take neighbouring work each: neighbouring tokens
+  // read many of the same pages, which one L2 then holds
+  const int64_t each = (a.work + 7) / 8, id = blockIdx.x % 8 * each + blockIdx.x / 8;
+  Task task;
+  Reads rd;
+  if (!PLANNED) {
+    if (blockIdx.x / 8 >= each || id >= a.work) return;
+    task_of<TREE>(a, lane, id, task, rd);
+    attend<MT, TREE>(a, L, lane, wave, task, rd);
+    return;
+  }
+  for (int64_t t = (int64_t)blockIdx.x * T + threadIdx.x; t < a.tokens; t += (int64_t)gridDim.x * T)
+    if (t < a.starts[0] || t >= a.starts[a.requests]) a.plan[t] = NodePlan{0, 0};  // nodes of no request
+  const int pages = chunk_pages(a, lane);
+  if (!planned_task(a, lane, pages, (int)id, task, rd)) return;
+  if (threadIdx.x == 0 && task.ht == 0 && task.chunk == 0) a.plan[task.t] = NodePlan{task.chunks, (int)task.part};
+  attend<MT, TREE>(a, L, lane, wave, task, rd);
+}
+
+// A head's parts as one, each scaled to the largest of their maxima. Wave w of W takes every W-th
 // part, eight of them in flight; the waves' sums meet in LDS.
 constexpr int MAX_SPLITS = 512, JOIN_AHEAD = 8;
-__global__ __launch_bounds__(T) void k_join(Paged a) {
-  __shared__ float by[MAX_SPLITS + JOIN_AHEAD * WAVES];
-  __shared__ alignas(16) float sums[WAVES][LATENT];
+template <int W>
+__global__ __launch_bounds__(W * WAVE) void k_join(Paged a) {
+  __shared__ float by[MAX_SPLITS + JOIN_AHEAD * W];
+  __shared__ alignas(16) float sums[W][LATENT];
   const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int64_t t = blockIdx.x / a.heads;
   const int h = blockIdx.x % a.heads;
-  const int64_t step = a.heads, first = t * a.splits * step + h;
+  int splits = a.splits;
+  int64_t part = t * a.splits;
+  if (a.plan) {
+    const NodePlan p = a.plan[t];
+    splits = p.chunks, part = p.part;
+    if (splits == 1) return;  // it was written whole
+    if (splits < 0 || splits > MAX_SPLITS || part < 0 || part + splits > a.parts) splits = 0;  // (starts that do not ascend)
+  }
+  const int64_t step = a.heads, first = part * step + h;
   float m = NEG_INF, l = 0.f;
-  for (int s = lane; s < a.splits; s += WAVE) m = fmaxf(m, a.part_m[first + s * step]);
+  for (int s = lane; s < splits; s += WAVE) m = fmaxf(m, a.part_m[first + s * step]);
   m = wave_max(m);
-  for (int s = lane; s < a.splits; s += WAVE) {
+  for (int s = lane; s < splits; s += WAVE) {
     const float ps = a.part_l[first + s * step], w = __builtin_amdgcn_exp2f(a.part_m[first + s * step] - m);
     l += ps == 0.f ? 0.f : ps * w;
     if (wave == 0) by[s] = ps == 0.f ? -1.f : w;  // -1: it saw nothing and wrote nothing
   }
-  if (wave == 0 && lane < JOIN_AHEAD * WAVES) by[a.splits + lane] = -1.f;
+  if (wave == 0)
+    for (int i = lane; i < JOIN_AHEAD * W; i += WAVE) by[splits + i] = -1.f;
   l = wave_sum(l);
   __syncthreads();
   float o[8] = {};
-  for (int s0 = wave; s0 < a.splits; s0 += JOIN_AHEAD * WAVES) {
+  for (int s0 = wave; s0 < splits; s0 += JOIN_AHEAD * W) {
     f32x4 v[JOIN_AHEAD][2];
 #pragma unroll
     for (int i = 0; i < JOIN_AHEAD; ++i) {
-      const float* row = a.part + (first + min(s0 + i * WAVES, a.splits - 1) * step) * LATENT + 8 * lane;
+      const float* row = a.part + (first + min(s0 + i * W, splits - 1) * step) * LATENT + 4 * lane;
       v[i][0] = *reinterpret_cast<const f32x4*>(row);
-      v[i][1] = *reinterpret_cast<const f32x4*>(row + 4);
+      v[i][1] = *reinterpret_cast<const f32x4*>(row + LATENT / 2);
     }
 #pragma unroll
     for (int i = 0; i < JOIN_AHEAD; ++i) {
-      const float w = by[s0 + i * WAVES];
+      const float w = by[s0 + i * W];
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] = w == -1.f ? o[j] : fmaf(v[i][j / 4][j % 4], w, o[j]);
     }
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j) *reinterpret_cast<f32x4*>(&sums[wave][8 * lane + 4 * j]) = f32x4{o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]};
+  for (int j = 0; j < 2; ++j)
+    *reinterpret_cast<f32x4*>(&sums[wave][LATENT / 2 * j + 4 * lane]) = f32x4{o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]};
   __syncthreads();
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  float r[2];
+  uint32_t* out = static_cast<uint32_t*>(a.out) + (t * a.heads + h) * (LATENT / 2);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    r[j] = 0.f;
+  for (int u = tid; u < LATENT / 2; u += W * WAVE) {
+    float r[2] = {0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) r[j] += sums[w][2 * tid + j];
+    for (int w = 0; w < W; ++w) r[0] += sums[w][2 * u], r[1] += sums[w][2 * u + 1];
+    out[u] = pack2(r[0] * inv, r[1] * inv);
   }
-  reinterpret_cast<uint32_t*>(a.out)[((t * a.heads + h) * LATENT) / 2 + tid] = pack_bf16x2(r[0] * inv, r[1] * inv);
 }
 
 }  // namespace
 
 hipError_t paged_attention(const Paged& a, hipStream_t st) {
-  const uint32_t grid = (uint32_t)((a.work + 7) / 8 * 8);
-  const bool tree = a.starts != nullptr;
-  if (a.head_rows == 16) {
-    if (tree) k_pages<1, true><<<grid, T, 0, st>>>(a);
-    else k_pages<1, false><<<grid, T, 0, st>>>(a);
-  } else {
-    if (tree) k_pages<2, true><<<grid, T, 0, st>>>(a);
-    else k_pages<2, false><<<grid, T, 0, st>>>(a);
-  }
-  return hipGetLastError();
+  const uint32_t grid = (uint32_t)(a.plan ? a.tasks : (a.work + 7) / 8 * 8);
+  const auto launch = [&](auto kernel) {
+    kernel<<<grid, T, 0, st>>>(a);
+    return hipGetLastError();
+  };
+  if (!a.starts) return launch(a.head_rows == 16 ? k_pages<1, false, false> : k_pages<2, false, false>);
+  if (a.plan) return launch(a.head_rows == 16 ? k_pages<1, true, true> : k_pages<2, true, true>);
+  return launch(a.head_rows == 16 ? k_pages<1, true, false> : k_pages<2, true, false>);
 }
 
 hipError_t join_attention(const Paged& a, hipStream_t st) {
-  k_join<<<(uint32_t)(a.tokens * a.heads), T, 0, st>>>(a);
+  const uint32_t grid = (uint32_t)(a.tokens * a.heads);
+  // waves a head by how many parts it has, at most or on average: each wave has eight rows on their way
+  const int64_t parts = a.plan ? a.tasks / (a.tokens * a.head_tiles) : a.splits;
+  if (parts <= 8)
+    k_join<1><<<grid, WAVE, 0, st>>>(a);
+  else if (parts <= 32)
+    k_join<4><<<grid, 4 * WAVE, 0, st>>>(a);
+  else
+    k_join<8><<<grid, 8 * WAVE, 0, st>>>(a);
   return hipGetLastError();
 }
 

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "mono.h"
 
 namespace mono {
@@ -175,21 +177,38 @@ struct Paged {
   float scale_log2;  // the softmax scale x log2(e)
   void* out;         // bf16 [tokens, heads, 512]
   // how it is shared out: heads a workgroup, workgroups a token's heads, workgroups a token's
-  // pages, and all of them
+  // pages (not planned trees), and all of them
   int head_rows, head_tiles, splits;
   int64_t work;
-  float *part, *part_m, *part_l;  // splits > 1: f32 [tokens, splits, heads, 512] and [.., heads] twice
+  // trees of few nodes, planned on the device: workgroups, and what each node's chunks are
+  int tasks;
+  struct NodePlan* plan;  // [tokens]
+  int64_t parts;
+  float *part, *part_m, *part_l;  // pages shared out: f32 [parts, heads, 512] and [.., heads] twice
+};
+struct NodePlan {
+  int chunks, part;  // its chunks of pages (0: a node of no request), the first one's part
 };
 
-// How the pages are shared out. Splits only where the tokens' heads alone would leave CUs
-// without work: two workgroups a CU, a page each at least.
+// How the pages are shared out. Only where the tokens' heads alone would leave CUs without
+// work: two workgroups a CU, a page each at least. A tree's pages are known on the device only;
+// up to PLANNED nodes' heads its workgroups plan there, with a second chunk or more for the nodes
+// that have more than their share of pages (their parts: at most two for each workgroup).
+constexpr int FULL = 512, PLANNED = FULL / 2;
 inline void paged_plan(Paged& a, int pages) {
   a.head_rows = a.heads <= 16 ? 16 : 32;
   a.head_tiles = (a.heads + a.head_rows - 1) / a.head_rows;
-  const int64_t whole = a.tokens * a.head_tiles, fit = 512 / whole;
-  a.splits = (int)(fit < pages ? fit : pages);
-  if (a.splits < 1) a.splits = 1;
+  const int64_t whole = a.tokens * a.head_tiles;
+  a.splits = 1;
+  a.work = whole;
+  if (a.starts) {
+    if (whole <= PLANNED && pages > 1) a.tasks = FULL, a.work = FULL, a.parts = std::min<int64_t>(2 * FULL, a.tokens * pages);
+    return;
+  }
+  const int64_t fit = FULL / whole;
+  a.splits = (int)std::max<int64_t>(std::min<int64_t>(fit, pages), 1);
   a.work = whole * a.splits;
+  if (a.splits > 1) a.parts = a.tokens * a.splits;
 }
 hipError_t paged_attention(const Paged& a, hipStream_t st);
 hipError_t join_attention(const Paged& a, hipStream_t st);

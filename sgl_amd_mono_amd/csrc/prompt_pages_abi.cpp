@@ -37,17 +37,19 @@ int tree_shape(int64_t nodes, int32_t heads, int32_t pt_stride) {
 size_t paged_space(void* ws, int pages, Paged& p) {
   Space sp{static_cast<char*>(ws)};
   paged_plan(p, pages);
-  if (p.splits == 1) return 0;
-  const size_t rows = (size_t)p.tokens * p.splits * p.heads;
+  if (!p.parts) return 0;
+  const size_t rows = (size_t)p.parts * p.heads;
   p.part = sp.take<float>(rows * LATENT);
   p.part_m = sp.take<float>(rows);
   p.part_l = sp.take<float>(rows);
+  if (p.tasks) p.plan = sp.take<NodePlan>(p.tokens);
   return sp.off;
 }
 
-int64_t paged_workspace(int64_t tokens, int32_t heads, int pages) {
+int64_t paged_workspace(int64_t tokens, int32_t heads, int pages, bool tree) {
   Paged p{};
-  p.tokens = tokens, p.heads = heads;
+  const int32_t some = 0;
+  p.tokens = tokens, p.heads = heads, p.starts = tree ? &some : nullptr;
   mono::abi_ok();
   return tokens ? (int64_t)paged_space(nullptr, pages, p) : 0;
 }
@@ -69,7 +71,7 @@ int run_paged(Paged& p, int pages, float scale, void* ws, int64_t ws_bytes, void
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (hipError_t e = paged_attention(p, st)) return launched(e, "the attention over pages");
-  return launched(p.splits > 1 ? join_attention(p, st) : hipSuccess, "the join of the attention's parts");
+  return launched(p.parts ? join_attention(p, st) : hipSuccess, "the join of the attention's parts");
 }
 
 }  // namespace
@@ -131,7 +133,7 @@ extern "C" int mono_prompt_select(const mono_prompt_select_args* args, void* str
 
 extern "C" int64_t mono_prompt_attention_workspace(int64_t tokens, int32_t heads, int32_t picks) {
   if (attention_shape(tokens, heads, picks)) return -1;
-  return paged_workspace(tokens, heads, picks);
+  return paged_workspace(tokens, heads, picks, false);
 }
 
 extern "C" int mono_prompt_attention(const mono_prompt_attention_args* args, void* stream) {
@@ -154,7 +156,7 @@ extern "C" int mono_prompt_attention(const mono_prompt_attention_args* args, voi
 
 extern "C" int64_t mono_prompt_tree_workspace(int64_t nodes, int32_t heads, int32_t pt_stride) {
   if (tree_shape(nodes, heads, pt_stride)) return -1;
-  return paged_workspace(nodes, heads, pt_stride);
+  return paged_workspace(nodes, heads, pt_stride, true);
 }
 
 extern "C" int mono_prompt_tree(const mono_prompt_tree_args* args, void* stream) {
