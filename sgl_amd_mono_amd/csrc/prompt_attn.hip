@@ -192,19 +192,35 @@ MONO_DEV void request_of(const Paged& a, int r, int64_t& first, int& n, int& pag
   pages = n ? (int)min((int64_t)min(a.pt_stride, 1 << 20), ((int64_t)max(a.prefix[r], 0) + PAGE - 1) / PAGE + 1) : 0;
 }
 
-// Trees of few nodes: each node's pages in chunks of `each`, a request's nodes side by side over
-// the same chunk. As many pages a chunk as make one round of tasks of them, each node's last chunk
-// being a short one.
-MONO_DEV int chunk_pages(const Paged& a, int lane) {
-  int total = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += WAVE) {
-    int64_t first;
-    int n = 0, pages = 0;
-    if (r0 + lane < a.requests) request_of(a, r0 + lane, first, n, pages);
-    total += wave_sum_i(n * pages);
+// Trees of few nodes: each node's pages in chunks of so many, a request's nodes side by side over
+// the same chunk: the fewest pages a chunk that make at most `most` tasks, between their share of
+// all pages and that of all pages beside a short chunk a node. Two workgroups a CU, but one where
+// that leaves it a few pages only: fewer parts to write and join are then worth more. `tasks`
+// comes to be how many there are.
+constexpr int FEW_PAGES = 8;
+MONO_DEV int chunk_pages(const Paged& a, int lane, int& tasks) {
+  const auto over = [&](auto of) {  // the requests' sum
+    int total = 0;
+    for (int r0 = 0; r0 < a.requests; r0 += WAVE) {
+      int64_t first;
+      int n = 0, pages = 0;
+      if (r0 + lane < a.requests) request_of(a, r0 + lane, first, n, pages);
+      total += wave_sum_i(n * of(pages));
+    }
+    return total * a.head_tiles;
+  };
+  const auto share = [](int n, int by) { return max((n + by - 1) / by, 1); };
+  const int total = over([](int pages) { return pages; }), least = (int)a.tokens * a.head_tiles;
+  const int most = total <= FULL / 2 * FEW_PAGES && least <= FULL / 4 ? FULL / 2 : FULL;
+  int lo = share(total, most), hi = share(total, most - least);
+  const auto made = [&](int each) { return over([&](int pages) { return (pages + each - 1) / each; }); };
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (made(mid) <= most) hi = mid;
+    else lo = mid + 1;
   }
-  const int tasks = a.tasks - (int)a.tokens * a.head_tiles;
-  return max((int)(((int64_t)total * a.head_tiles + tasks - 1) / tasks), 1);
+  tasks = min(made(hi), FULL);  // (more only by starts that do not ascend)
+  return hi;
 }
 
 // Task `id` of them; false behind the last.
@@ -591,35 +607,40 @@ template <int MT, bool TREE, bool PLANNED>
 __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
   __shared__ Lds L;
   const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  int tasks = (int)a.work, pages = 0;
+  if (PLANNED) {
+    for (int64_t t = (int64_t)blockIdx.x * T + threadIdx.x; t < a.tokens; t += (int64_t)gridDim.x * T)
+      if (t < a.starts[0] || t >= a.starts[a.requests]) a.plan[t] = NodePlan{0, 0};  // nodes of no request
+    pages = chunk_pages(a, lane, tasks);
+  }
   // the XCDs (workgroup b runs on XCD b mod 8) take neighbouring work each: neighbouring tokens
   // read many of the same pages, which one L2 then holds
-  const int64_t each = (a.work + 7) / 8, id = blockIdx.x % 8 * each + blockIdx.x / 8;
+  const int each = (tasks + 7) / 8, id = (int)(blockIdx.x % 8) * each + (int)(blockIdx.x / 8);
+  if ((int)(blockIdx.x / 8) >= each || id >= tasks) return;
   Task task;
   Reads rd;
-  if (!PLANNED) {
-    if (blockIdx.x / 8 >= each || id >= a.work) return;
+  if (!PLANNED)
     task_of<TREE>(a, lane, id, task, rd);
-    attend<MT, TREE>(a, L, lane, wave, task, rd);
-    return;
+  else {
+    if (!planned_task(a, lane, pages, id, task, rd)) return;
+    if (threadIdx.x == 0 && task.ht == 0 && task.chunk == 0) a.plan[task.t] = NodePlan{task.chunks, (int)task.part};
   }
-  for (int64_t t = (int64_t)blockIdx.x * T + threadIdx.x; t < a.tokens; t += (int64_t)gridDim.x * T)
-    if (t < a.starts[0] || t >= a.starts[a.requests]) a.plan[t] = NodePlan{0, 0};  // nodes of no request
-  const int pages = chunk_pages(a, lane);
-  if (!planned_task(a, lane, pages, (int)id, task, rd)) return;
-  if (threadIdx.x == 0 && task.ht == 0 && task.chunk == 0) a.plan[task.t] = NodePlan{task.chunks, (int)task.part};
   attend<MT, TREE>(a, L, lane, wave, task, rd);
 }
 
-// A head's parts as one, each scaled to the largest of their maxima. Wave w of W takes every W-th
-// part, eight of them in flight; the waves' sums meet in LDS.
+// A head's parts as one, each scaled to the largest of their maxima. A workgroup takes 512 / S of
+// its dims, wave w of W every W-th part, eight of them in flight; the waves' sums meet in LDS.
 constexpr int MAX_SPLITS = 512, JOIN_AHEAD = 8;
-template <int W>
+template <int W, int S>
 __global__ __launch_bounds__(W * WAVE) void k_join(Paged a) {
   __shared__ float by[MAX_SPLITS + JOIN_AHEAD * W];
-  __shared__ alignas(16) float sums[W][LATENT];
+  constexpr int N = LATENT / S, V = N / WAVE;  // dims: of the workgroup, of a lane
+  typedef float Vec __attribute__((ext_vector_type(V < 4 ? V : 4)));
+  constexpr int VECS = V < 4 ? 1 : V / 4, EACH = V / VECS;
+  __shared__ alignas(16) float sums[W][N];
   const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-  const int64_t t = blockIdx.x / a.heads;
-  const int h = blockIdx.x % a.heads;
+  const int slice = blockIdx.x % S, h = blockIdx.x / S % a.heads;
+  const int64_t t = blockIdx.x / S / a.heads;
   int splits = a.splits;
   int64_t part = t * a.splits;
   if (a.plan) {
@@ -641,30 +662,28 @@ __global__ __launch_bounds__(W * WAVE) void k_join(Paged a) {
     for (int i = lane; i < JOIN_AHEAD * W; i += WAVE) by[splits + i] = -1.f;
   l = wave_sum(l);
   __syncthreads();
-  float o[8] = {};
+  float o[V] = {};
   for (int s0 = wave; s0 < splits; s0 += JOIN_AHEAD * W) {
-    f32x4 v[JOIN_AHEAD][2];
+    Vec v[JOIN_AHEAD][VECS];
 #pragma unroll
     for (int i = 0; i < JOIN_AHEAD; ++i) {
-      const float* row = a.part + (first + min(s0 + i * W, splits - 1) * step) * LATENT + 4 * lane;
-      v[i][0] = *reinterpret_cast<const f32x4*>(row);
-      v[i][1] = *reinterpret_cast<const f32x4*>(row + LATENT / 2);
+      const float* row = a.part + (first + min(s0 + i * W, splits - 1) * step) * LATENT + N * slice + EACH * lane;
+#pragma unroll
+      for (int j = 0; j < VECS; ++j) v[i][j] = *reinterpret_cast<const Vec*>(row + N / VECS * j);
     }
 #pragma unroll
     for (int i = 0; i < JOIN_AHEAD; ++i) {
       const float w = by[s0 + i * W];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = w == -1.f ? o[j] : fmaf(v[i][j / 4][j % 4], w, o[j]);
+      for (int j = 0; j < V; ++j) o[j] = w == -1.f ? o[j] : fmaf(v[i][j / EACH][j % EACH], w, o[j]);
     }
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
-    *reinterpret_cast<f32x4*>(&sums[wave][LATENT / 2 * j + 4 * lane]) = f32x4{o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]};
+  for (int j = 0; j < V; ++j) sums[wave][N / VECS * (j / EACH) + EACH * lane + j % EACH] = o[j];
   __syncthreads();
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  uint32_t* out = static_cast<uint32_t*>(a.out) + (t * a.heads + h) * (LATENT / 2);
-#pragma unroll
-  for (int u = tid; u < LATENT / 2; u += W * WAVE) {
+  uint32_t* out = static_cast<uint32_t*>(a.out) + (t * a.heads + h) * (LATENT / 2) + N / 2 * slice;
+  for (int u = tid; u < N / 2; u += W * WAVE) {
     float r[2] = {0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < W; ++w) r[0] += sums[w][2 * u], r[1] += sums[w][2 * u + 1];
@@ -675,9 +694,8 @@ __global__ __launch_bounds__(W * WAVE) void k_join(Paged a) {
 }  // namespace
 
 hipError_t paged_attention(const Paged& a, hipStream_t st) {
-  const uint32_t grid = (uint32_t)(a.plan ? a.tasks : (a.work + 7) / 8 * 8);
   const auto launch = [&](auto kernel) {
-    kernel<<<grid, T, 0, st>>>(a);
+    kernel<<<(uint32_t)((a.work + 7) / 8 * 8), T, 0, st>>>(a);
     return hipGetLastError();
   };
   if (!a.starts) return launch(a.head_rows == 16 ? k_pages<1, false, false> : k_pages<2, false, false>);
@@ -686,15 +704,11 @@ hipError_t paged_attention(const Paged& a, hipStream_t st) {
 }
 
 hipError_t join_attention(const Paged& a, hipStream_t st) {
-  const uint32_t grid = (uint32_t)(a.tokens * a.heads);
-  // waves a head by how many parts it has, at most or on average: each wave has eight rows on their way
-  const int64_t parts = a.plan ? a.tasks / (a.tokens * a.head_tiles) : a.splits;
-  if (parts <= 8)
-    k_join<1><<<grid, WAVE, 0, st>>>(a);
-  else if (parts <= 32)
-    k_join<4><<<grid, 4 * WAVE, 0, st>>>(a);
+  const int64_t heads = a.tokens * a.heads;
+  if (heads <= 256)
+    k_join<4, 4><<<(uint32_t)(4 * heads), 4 * WAVE, 0, st>>>(a);
   else
-    k_join<8><<<grid, 8 * WAVE, 0, st>>>(a);
+    k_join<1, 1><<<(uint32_t)heads, WAVE, 0, st>>>(a);
   return hipGetLastError();
 }
 

@@ -202,7 +202,7 @@ inline void paged_plan(Paged& a, int pages) {
   a.splits = 1;
   a.work = whole;
   if (a.starts) {
-    if (whole <= PLANNED && pages > 1) a.tasks = FULL, a.work = FULL, a.parts = std::min<int64_t>(2 * FULL, a.tokens * pages);
+    if (whole <= PLANNED && pages > 1) a.tasks = a.work = FULL, a.parts = std::min<int64_t>(FULL / a.head_tiles, a.tokens * pages);
     return;
   }
   const int64_t fit = FULL / whole;
