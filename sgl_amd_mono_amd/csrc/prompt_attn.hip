@@ -198,7 +198,7 @@ MONO_DEV void request_of(const Paged& a, int r, int64_t& first, int& n, int& pag
 // that leaves it a few pages only: fewer parts to write and join are then worth more. `tasks`
 // comes to be how many there are.
 constexpr int FEW_PAGES = 8;
-MONO_DEV int chunk_pages(const Paged& a, int lane, int& tasks) {
+MONO_DEV int chunk_pages(const Paged& a, int lane, int64_t& tasks) {
   const auto over = [&](auto of) {  // the requests' sum
     int total = 0;
     for (int r0 = 0; r0 < a.requests; r0 += WAVE) {
@@ -603,26 +603,37 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
     *reinterpret_cast<u32x4*>(out + 8 * u) = *reinterpret_cast<const u32x4*>(stage + u / (LATENT / 8) * PITCH + u % (LATENT / 8) * 8);
 }
 
+// Which task workgroup b takes; it runs on XCD b mod 8. Neighbouring tasks read many of the same
+// pages, which one L2 then holds, so an XCD takes BLOCK of them in a row; and all XCDs go through
+// the tokens together and from the last one down, since a prompt's later tokens have more pages:
+// the short tasks are left for the end (600 tokens from position 0: an eighth of the tokens for each
+// XCD 52 us, single tokens 40, fours 39.5, fours from the last 29, sixty-fours from the last 41; 4096
+// tokens of 5 requests 410, 310, 303, 298, 307).
+constexpr int BLOCK = 4;
+MONO_DEV int64_t task_id(uint32_t b, int64_t tasks) {
+  const uint32_t i = b / 8;
+  return tasks - 1 - ((int64_t)(i / BLOCK * 8 + b % 8) * BLOCK + i % BLOCK);
+}
+
 template <int MT, bool TREE, bool PLANNED>
 __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
   __shared__ Lds L;
   const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  int tasks = (int)a.work, pages = 0;
+  int64_t tasks = a.work;
+  int pages = 0;
   if (PLANNED) {
     for (int64_t t = (int64_t)blockIdx.x * T + threadIdx.x; t < a.tokens; t += (int64_t)gridDim.x * T)
       if (t < a.starts[0] || t >= a.starts[a.requests]) a.plan[t] = NodePlan{0, 0};  // nodes of no request
     pages = chunk_pages(a, lane, tasks);
   }
-  // the XCDs (workgroup b runs on XCD b mod 8) take neighbouring work each: neighbouring tokens
-  // read many of the same pages, which one L2 then holds
-  const int each = (tasks + 7) / 8, id = (int)(blockIdx.x % 8) * each + (int)(blockIdx.x / 8);
-  if ((int)(blockIdx.x / 8) >= each || id >= tasks) return;
+  const int64_t id = task_id(blockIdx.x, tasks);
+  if (id < 0) return;
   Task task;
   Reads rd;
   if (!PLANNED)
     task_of<TREE>(a, lane, id, task, rd);
   else {
-    if (!planned_task(a, lane, pages, id, task, rd)) return;
+    if (!planned_task(a, lane, pages, (int)id, task, rd)) return;
     if (threadIdx.x == 0 && task.ht == 0 && task.chunk == 0) a.plan[task.t] = NodePlan{task.chunks, (int)task.part};
   }
   attend<MT, TREE>(a, L, lane, wave, task, rd);
@@ -695,7 +706,7 @@ __global__ __launch_bounds__(W * WAVE) void k_join(Paged a) {
 
 hipError_t paged_attention(const Paged& a, hipStream_t st) {
   const auto launch = [&](auto kernel) {
-    kernel<<<(uint32_t)((a.work + 7) / 8 * 8), T, 0, st>>>(a);
+    kernel<<<(uint32_t)((a.work + 8 * BLOCK - 1) / (8 * BLOCK) * (8 * BLOCK)), T, 0, st>>>(a);
     return hipGetLastError();
   };
   if (!a.starts) return launch(a.head_rows == 16 ? k_pages<1, false, false> : k_pages<2, false, false>);
