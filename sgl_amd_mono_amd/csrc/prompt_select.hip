@@ -29,6 +29,18 @@ MONO_DEV int row_count(int n, int* lds, int wave) {
   return n;
 }
 
+// the largest of a row's waves
+template <int W>
+MONO_DEV uint32_t row_max(uint32_t v, int* lds, int wave) {
+  if (W == 1) return v;
+  __syncthreads();
+  if (threadIdx.x % WAVE == 0) lds[wave] = (int)v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) v = max(v, (uint32_t)lds[w]);
+  return v;
+}
+
 // W waves a row, N values a lane: value i of lane l of wave w is column (w N + i) 64 + l.
 template <int W, int N>
 __global__ __launch_bounds__(256) void k_select(mono_prompt_select_args a) {
@@ -47,11 +59,12 @@ __global__ __launch_bounds__(256) void k_select(mono_prompt_select_args a) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int c = (w * N + i) * WAVE + lane;
-    key[i] = order_key(row[min(c, a.columns - 1)]);
+    const uint32_t k = order_key(row[min(c, a.columns - 1)]);
     const bool f = c < n && (c < a.first || c > mine - a.last);
     always |= f ? 1u << (i % 32) : 0u;
     static_assert(N <= 32, "a bit each");
     forced += __popcll(__ballot(f));
+    key[i] = c < n && !f ? k : 0u;  // (only what is open is above 0)
   }
   const auto open = [&](int i) { return (w * N + i) * WAVE + lane < n && !(always >> i & 1); };
   forced = row_count<W>(forced, lds, w);
@@ -65,15 +78,23 @@ __global__ __launch_bounds__(256) void k_select(mono_prompt_select_args a) {
     const auto count = [&](auto at_least) {
       int m = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) m += __popcll(__ballot(open(i) && at_least(key[i])));
+      for (int i = 0; i < N; ++i) m += __popcll(__ballot(at_least(key[i])));
       return row_count<W>(m, lds, w);
     };
-    int kept = rest;  // open keys that are at least `top`
+    // Bounds of the k-th largest: the largest key above; below, as many keys as there are lanes
+    // with one, each lane's largest, are at least the smallest of those.
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) most = max(most, key[i]);
+    uint32_t hi = row_max<W>(wave_umax(most), lds, w);
+    top = row_max<W>(need <= WAVE ? ~wave_umax(~most) : 0u, lds, w);
+    int kept = 0;  // keys that are at least `top` (0: not counted)
 #pragma unroll 1
-    for (int bit = 31; bit >= 0 && kept != need; --bit) {
-      const uint32_t cand = top | 1u << bit;
-      const int m = count([&](uint32_t k) { return k >= cand; });
-      if (m >= need) top = cand, kept = m;
+    while (top < hi && kept != need) {
+      const uint32_t mid = top + (hi - top + 1) / 2;
+      const int m = count([&](uint32_t k) { return k >= mid; });
+      if (m >= need) top = mid, kept = m;
+      else hi = mid - 1;
     }
     if (kept != need) border = need - count([&](uint32_t k) { return k > top; });
   }
@@ -83,7 +104,7 @@ __global__ __launch_bounds__(256) void k_select(mono_prompt_select_args a) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       eq += __popcll(__ballot(open(i) && key[i] == top));
-      gt += __popcll(__ballot((always >> i & 1) || (open(i) && key[i] > top)));
+      gt += __popcll(__ballot((always >> i & 1) || (key[i] > top)));
     }
     __syncthreads();
     if (lane == 0) lds[w] = eq;
@@ -101,7 +122,7 @@ __global__ __launch_bounds__(256) void k_select(mono_prompt_select_args a) {
     const bool eq = open(i) && key[i] == top;
     const uint64_t eqs = __ballot(eq);
     const bool tie = eq && ties + (int)__popcll(eqs & ((1ull << lane) - 1)) < border;
-    const bool take = (always >> i & 1) || (open(i) && key[i] > top) || tie;
+    const bool take = (always >> i & 1) || (key[i] > top) || tie;
     const uint64_t taken = __ballot(take);
     const int place = at + (int)__popcll(taken & ((1ull << lane) - 1));
     if (take) out[place] = (w * N + i) * WAVE + lane;
