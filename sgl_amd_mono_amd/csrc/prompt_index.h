@@ -40,11 +40,11 @@ MONO_DEV double row_xor_d(double v) {
   return __builtin_bit_cast(double, (uint64_t)xor4_u((uint32_t)u) | (uint64_t)xor4_u((uint32_t)(u >> 32)) << 32);
 }
 // A butterfly between lanes X apart: a + b in the lane with the bit clear, a - b in its partner.
-template <int X>
-MONO_DEV void lanes_butterfly(double (&y)[8], int sub) {
+template <int X, int N>
+MONO_DEV void lanes_butterfly(double (&y)[N], int sub) {
   const double sign = sub & X ? -1.0 : 1.0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = fma(sign, y[i], row_xor_d<X>(y[i]));
+  for (int i = 0; i < N; ++i) y[i] = fma(sign, y[i], row_xor_d<X>(y[i]));
 }
 MONO_DEV void lane_butterfly(double (&y)[8], int x) {
 #pragma unroll
@@ -64,6 +64,12 @@ MONO_DEV float to_bf16(double v) {
   return bf16_round(f);
 }
 
+MONO_DEV uint32_t pack_bf16(double a, double b) {
+  float x = (float)a, y = (float)b;
+  asm("" : "+v"(x), "+v"(y));
+  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)x, (__bf16)y});
+}
+
 // the larger of each magnitude's bits over the 16 lanes of a token, over 4 lanes of it
 MONO_DEV uint32_t quad_umax(uint32_t v) {
   v = max(v, dpp_u<DPP_XOR1>(v));
@@ -81,15 +87,24 @@ MONO_DEV void load4(const float* p, float (&v)[4]) {
   for (int i = 0; i < 4; ++i) v[i] = w[i];
 }
 
+// Eight E2M1 codes without negative zeros: a sign bit stays where its code's magnitude is not zero.
+MONO_DEV uint32_t no_negative_zero(uint32_t w) { return w & (((w & 0x77777777u) + 0x77777777u) | 0x77777777u); }
+
 // Eight values of |q| <= 6 as E2M1 codes (the first in the low nibble), ties to even, no
-// negative zero: a sign bit stays where its code's magnitude is not zero.
+// negative zero.
 MONO_DEV uint32_t e2m1_pack8(const float (&q)[8]) {
   uint32_t w = 0;
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[0], q[1], 1.0f, 0);
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[2], q[3], 1.0f, 1);
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[4], q[5], 1.0f, 2);
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[6], q[7], 1.0f, 3);
-  return w & (((w & 0x77777777u) + 0x77777777u) | 0x77777777u);
+  return no_negative_zero(w);
+}
+
+// The code of the scale of a block whose largest magnitude has the f32 bits hm: the smallest power of
+// two that it divided by is at most 6; NaN's, 255, where it is not finite.
+MONO_DEV uint32_t block_code(uint32_t hm) {
+  return hm < 0x7f800000u ? proj::code_ceil(proj::mul_rn(fmaxf(__uint_as_float(hm), 6.0f * 0x1p-126f), 1.0f / 6.0f)) : 255u;
 }
 
 // The codes of a vector whose rotated values (dims 8 sub .. + 7, bf16 values) are y: Hadamard,
@@ -111,12 +126,11 @@ MONO_DEV uint32_t index_codes(double (&y)[8], int sub, uint32_t& e8) {
     hm = max(hm, abs_bits(k[v]));
   }
   hm = quad_umax(hm);
-  const bool finite = hm < 0x7f800000u;
-  e8 = finite ? proj::code_ceil(proj::mul_rn(fmaxf(__uint_as_float(hm), 6.0f * 0x1p-126f), 1.0f / 6.0f)) : 255u;
+  e8 = block_code(hm);
   const float ei = proj::pow2_of(254u - min(e8, 254u));
 #pragma unroll
   for (int v = 0; v < 8; ++v) k[v] *= ei;
-  return finite ? e2m1_pack8(k) : 0u;
+  return e8 < 255 ? e2m1_pack8(k) : 0u;
 }
 
 }  // namespace prompt
