@@ -185,11 +185,13 @@ MONO_DEV void node_reads(const Paged& a, int64_t t, int req, Reads& rd) {
   rd.draft = (uint64_t)a.mask[t];
 }
 
-// Request r's nodes and pages (the last one or two hold the draft's keys).
+// Request r's nodes and pages (the last one or two hold the draft's keys; MOST_PAGES: more than the
+// card's memory holds, and PLANNED times as many are counted in 32 bits).
+constexpr int MOST_PAGES = (1 << 23) - 16;
 MONO_DEV void request_of(const Paged& a, int r, int64_t& first, int& n, int& pages) {
   first = min((int64_t)max(a.starts[r], 0), a.tokens);
   n = (int)max(min((int64_t)a.starts[r + 1], a.tokens) - first, (int64_t)0);
-  pages = n ? (int)min((int64_t)min(a.pt_stride, 1 << 20), ((int64_t)max(a.prefix[r], 0) + PAGE - 1) / PAGE + 1) : 0;
+  pages = n ? (int)min((int64_t)min(a.pt_stride, MOST_PAGES), ((int64_t)max(a.prefix[r], 0) + PAGE - 1) / PAGE + 1) : 0;
 }
 
 // Trees of few nodes: each node's pages in chunks of so many, a request's nodes side by side over

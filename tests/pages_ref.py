@@ -31,7 +31,7 @@ def index_query(x, pos, cos, sin):
 
 
 def page_scores(iq, iqs, iw, req, pos, table, ikv, iks, columns):
-    """(scores, the largest sum of a key's terms' magnitudes), f64 [tokens, columns]."""
+    """(scores, the largest sum of a key's |weight x product|), f64 [tokens, columns]."""
     out = torch.full((len(iq), columns), -torch.inf, dtype=torch.float64)
     mag = torch.zeros(len(iq), columns, dtype=torch.float64)
     for n, (r, p) in enumerate(zip(req.tolist(), pos.tolist())):
@@ -46,7 +46,7 @@ def page_scores(iq, iqs, iw, req, pos, table, ikv, iks, columns):
             terms = w[:, None] * torch.where(dot.isnan(), dot, dot.clamp_min(0))
             s = terms.sum(0)
             out[n, c] = torch.nan if bool(s.isnan().any()) else s.max()
-            mag[n, c] = terms.abs().sum(0).max()
+            mag[n, c] = (w[:, None] * dot).abs().sum(0).max()
     return out, mag
 
 
@@ -67,11 +67,14 @@ def select_pages(scores, pos, picks, first, last):
 
 def _over(q, kv, kv_scale, slots, scale):
     """One token's attention over `slots` (any order, any number of times): (out, sum of p |v|,
-    the largest sum of a logit's terms' magnitudes), f64."""
+    how far a logit may be off), f64. A logit: 578 roundings of f32 of its terms' magnitudes, and
+    q's elements off by 2^-21.8 of their head's largest, in the last 64 dims by 2^-17.8."""
     rows = oatt.kv_rows(kv, kv_scale, slots).double()
     q = q.double()
     p = torch.softmax(q @ rows.T * scale, -1)
-    return p @ rows[:, :LATENT], p @ rows[:, :LATENT].abs(), float((q.abs() @ rows.abs().T).max()) * abs(scale)
+    k = rows.abs()
+    off = 578 * 2.0**-24 * (q.abs() @ k.T) + q.abs().amax(-1, keepdim=True) * (2.0**-21.8 * k[:, :LATENT].sum(-1) + 2.0**-17.8 * k[:, LATENT:].sum(-1))
+    return p @ rows[:, :LATENT], p @ k[:, :LATENT], float(off.max()) * abs(scale)
 
 
 def _empty(q):
