@@ -185,13 +185,20 @@ MONO_DEV void node_reads(const Paged& a, int64_t t, int req, Reads& rd) {
   rd.draft = (uint64_t)a.mask[t];
 }
 
-// Request r's nodes and pages (the last one or two hold the draft's keys; MOST_PAGES: more than the
+// A request's nodes and pages (the last one or two hold the draft's keys; MOST_PAGES: more than the
 // card's memory holds, and PLANNED times as many are counted in 32 bits).
 constexpr int MOST_PAGES = (1 << 23) - 16;
-MONO_DEV void request_of(const Paged& a, int r, int64_t& first, int& n, int& pages) {
-  first = min((int64_t)max(a.starts[r], 0), a.tokens);
-  n = (int)max(min((int64_t)a.starts[r + 1], a.tokens) - first, (int64_t)0);
-  pages = n ? (int)min((int64_t)min(a.pt_stride, MOST_PAGES), ((int64_t)max(a.prefix[r], 0) + PAGE - 1) / PAGE + 1) : 0;
+struct Request {
+  int64_t first;
+  int n, pages;
+};
+MONO_DEV Request request_of(const Paged& a, int r) {
+  Request q = {0, 0, 0};
+  if (r >= a.requests) return q;
+  q.first = min((int64_t)max(a.starts[r], 0), a.tokens);
+  q.n = (int)max(min((int64_t)a.starts[r + 1], a.tokens) - q.first, (int64_t)0);
+  q.pages = q.n ? (int)min((int64_t)min(a.pt_stride, MOST_PAGES), ((int64_t)max(a.prefix[r], 0) + PAGE - 1) / PAGE + 1) : 0;
+  return q;
 }
 
 // Trees of few nodes: each node's pages in chunks of so many, a request's nodes side by side over
@@ -199,21 +206,21 @@ MONO_DEV void request_of(const Paged& a, int r, int64_t& first, int& n, int& pag
 // all pages and that of all pages beside a short chunk a node. Two workgroups a CU, but one where
 // that leaves it a few pages only: fewer parts to write and join are then worth more. `tasks`
 // comes to be how many there are.
-constexpr int FEW_PAGES = 8;
-MONO_DEV int chunk_pages(const Paged& a, int lane, int64_t& tasks) {
+constexpr int FEW_PAGES = 8, JOIN_PAGES = 4;
+MONO_DEV int chunk_pages(const Paged& a, int lane, const Request& head, int64_t& tasks) {  // (head: request `lane`)
   const auto over = [&](auto of) {  // the requests' sum
-    int total = 0;
-    for (int r0 = 0; r0 < a.requests; r0 += WAVE) {
-      int64_t first;
-      int n = 0, pages = 0;
-      if (r0 + lane < a.requests) request_of(a, r0 + lane, first, n, pages);
-      total += wave_sum_i(n * of(pages));
+    int total = wave_sum_i(head.n * of(head.pages));
+    for (int r0 = WAVE; r0 < a.requests; r0 += WAVE) {
+      const Request q = request_of(a, r0 + lane);
+      total += wave_sum_i(q.n * of(q.pages));
     }
     return total * a.head_tiles;
   };
   const auto share = [](int n, int by) { return max((n + by - 1) / by, 1); };
   const int total = over([](int pages) { return pages; }), least = (int)a.tokens * a.head_tiles;
   const int most = total <= FULL / 2 * FEW_PAGES && least <= FULL / 4 ? FULL / 2 : FULL;
+  uint32_t longest = wave_umax((uint32_t)head.pages);
+  for (int r0 = WAVE; r0 < a.requests; r0 += WAVE) longest = max(longest, wave_umax((uint32_t)request_of(a, r0 + lane).pages));
   int lo = share(total, most), hi = share(total, most - least);
   const auto made = [&](int each) { return over([&](int pages) { return (pages + each - 1) / each; }); };
   while (lo < hi) {
@@ -221,33 +228,32 @@ MONO_DEV int chunk_pages(const Paged& a, int lane, int64_t& tasks) {
     if (made(mid) <= most) hi = mid;
     else lo = mid + 1;
   }
+  if ((int)longest <= hi + JOIN_PAGES) hi = max((int)longest, 1);
   tasks = min(made(hi), FULL);  // (more only by starts that do not ascend)
   return hi;
 }
 
 // Task `id` of them; false behind the last.
-MONO_DEV bool planned_task(const Paged& a, int lane, int each, int id, Task& k, Reads& rd) {
+MONO_DEV bool planned_task(const Paged& a, int lane, const Request& head, int each, int id, Task& k, Reads& rd) {
   k.ht = id % a.head_tiles;
   id /= a.head_tiles;
   int part = 0;
   for (int r0 = 0; r0 < a.requests; r0 += WAVE) {
-    int64_t first = 0;
-    int n = 0, pages = 0;
-    if (r0 + lane < a.requests) request_of(a, r0 + lane, first, n, pages);
-    const int chunks = (pages + each - 1) / each, tasks = n * chunks, parts = chunks > 1 ? tasks : 0;
+    const Request q = r0 ? request_of(a, r0 + lane) : head;
+    const int chunks = (q.pages + each - 1) / each, tasks = q.n * chunks, parts = chunks > 1 ? tasks : 0;
     const int upto = wave_incl_scan(tasks), parts_upto = wave_incl_scan(parts);
     const uint64_t here = __ballot(upto > id);
     if (here) {
       const int l = __builtin_ctzll(here);
       const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-      const int nodes = of(n), at = id - (of(upto) - of(tasks)), node = at % nodes;
+      const int nodes = of(q.n), at = id - (of(upto) - of(tasks)), node = at % nodes;
       k.chunk = at / nodes;
       k.chunks = of(chunks);
       k.part = part + of(parts_upto) - of(parts) + node * k.chunks + k.chunk;
-      k.t = (int64_t)of((int)first) + node;
+      k.t = (int64_t)of((int)q.first) + node;
       node_reads(a, k.t, r0 + l, rd);
       rd.lo = k.chunk * each;
-      rd.hi = min(rd.lo + each, of(pages));
+      rd.hi = min(rd.lo + each, of(q.pages));
       k.any = true;
       return k.part < a.parts;  // (starts that do not ascend: nothing is written behind the parts)
     }
@@ -623,10 +629,12 @@ __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
   const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   int64_t tasks = a.work;
   int pages = 0;
+  Request head;
   if (PLANNED) {
     for (int64_t t = (int64_t)blockIdx.x * T + threadIdx.x; t < a.tokens; t += (int64_t)gridDim.x * T)
       if (t < a.starts[0] || t >= a.starts[a.requests]) a.plan[t] = NodePlan{0, 0};  // nodes of no request
-    pages = chunk_pages(a, lane, tasks);
+    head = request_of(a, lane);
+    pages = chunk_pages(a, lane, head, tasks);
   }
   const int64_t id = task_id(blockIdx.x, tasks);
   if (id < 0) return;
@@ -635,7 +643,7 @@ __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
   if (!PLANNED)
     task_of<TREE>(a, lane, id, task, rd);
   else {
-    if (!planned_task(a, lane, pages, (int)id, task, rd)) return;
+    if (!planned_task(a, lane, head, pages, (int)id, task, rd)) return;
     if (threadIdx.x == 0 && task.ht == 0 && task.chunk == 0) a.plan[task.t] = NodePlan{task.chunks, (int)task.part};
   }
   attend<MT, TREE>(a, L, lane, wave, task, rd);

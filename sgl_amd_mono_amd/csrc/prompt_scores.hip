@@ -146,7 +146,7 @@ __global__ __launch_bounds__(WAVES * WAVE, 4) void k_scores(mono_prompt_scores_a
 hipError_t page_scores(const mono_prompt_scores_args& a, hipStream_t st) {
   const int64_t groups = (a.tokens + WAVES - 1) / WAVES;
   // pages a workgroup: as many as leave 4096 workgroups, four rounds of them (a run's query is loaded once)
-  const int run = (int)std::min<int64_t>(std::max<int64_t>(groups * a.columns / 4096, 1), 16);
+  const int run = (int)std::min<int64_t>(std::max<int64_t>(groups * a.columns / 2048, 1), 32);
   const int64_t runs = (a.columns + run - 1) / run;
   k_scores<<<(uint32_t)(groups * runs), WAVES * WAVE, 0, st>>>(a, run, (uint32_t)groups);
   return hipGetLastError();

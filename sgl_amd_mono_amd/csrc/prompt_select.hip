@@ -16,36 +16,48 @@ MONO_DEV uint32_t order_key(float f) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// the sum over a row's waves
+// What the waves of a row have each, in every one of them. (Two places in turn: one barrier a time.)
 template <int W>
-MONO_DEV int row_count(int n, int* lds, int wave) {
-  if (W == 1) return n;
-  __syncthreads();
-  if (threadIdx.x % WAVE == 0) lds[wave] = n;
-  __syncthreads();
-  n = 0;
+struct RowWaves {
+  int (*lds)[W];
+  int wave, turn;
+  template <class Op>
+  MONO_DEV uint32_t all(uint32_t v, Op op) {
+    if (W == 1) return v;
+    int* at = lds[turn];
+    turn ^= 1;
+    if (threadIdx.x % WAVE == 0) at[wave] = (int)v;
+    __syncthreads();
+    v = (uint32_t)at[0];
 #pragma unroll
-  for (int w = 0; w < W; ++w) n += lds[w];
-  return n;
-}
-
-// the largest of a row's waves
-template <int W>
-MONO_DEV uint32_t row_max(uint32_t v, int* lds, int wave) {
-  if (W == 1) return v;
-  __syncthreads();
-  if (threadIdx.x % WAVE == 0) lds[wave] = (int)v;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < W; ++w) v = max(v, (uint32_t)lds[w]);
-  return v;
-}
+    for (int w = 1; w < W; ++w) v = op(v, (uint32_t)at[w]);
+    return __builtin_amdgcn_readfirstlane((int)v);
+  }
+  MONO_DEV int sum(int v) {
+    return (int)all((uint32_t)v, [](uint32_t a, uint32_t b) { return a + b; });
+  }
+  MONO_DEV uint32_t most(uint32_t v) {
+    return all(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+  }
+  // the sum over the waves before this one
+  MONO_DEV int before(int v) {
+    if (W == 1) return 0;
+    int* at = lds[turn];
+    turn ^= 1;
+    if (threadIdx.x % WAVE == 0) at[wave] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < wave; ++w) v += at[w];
+    return v;
+  }
+};
 
 // W waves a row, N values a lane: value i of lane l of wave w is column (w N + i) 64 + l.
 template <int W, int N>
 __global__ __launch_bounds__(256) void k_select(mono_prompt_select_args a) {
-  __shared__ int lds[4];
+  __shared__ int lds[2][W];
   const int lane = threadIdx.x % WAVE, wv = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), w = wv % W;
+  RowWaves<W> row_waves{lds, w, 0};
   const int64_t t = (int64_t)blockIdx.x * (4 / W) + wv / W;
   if (t >= a.tokens) return;  // (W > 1: of the whole workgroup)
   const int pos = __builtin_amdgcn_readfirstlane(a.pos[t]);
@@ -67,7 +79,7 @@ __global__ __launch_bounds__(256) void k_select(mono_prompt_select_args a) {
     key[i] = c < n && !f ? k : 0u;  // (only what is open is above 0)
   }
   const auto open = [&](int i) { return (w * N + i) * WAVE + lane < n && !(always >> i & 1); };
-  forced = row_count<W>(forced, lds, w);
+  forced = row_waves.sum(forced);
   // picks left for the scores; an open key above `top` is taken, and of those equal to it the
   // first `border`
   const int need = a.picks - forced, rest = n - forced;
@@ -79,15 +91,15 @@ __global__ __launch_bounds__(256) void k_select(mono_prompt_select_args a) {
       int m = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i) m += __popcll(__ballot(at_least(key[i])));
-      return row_count<W>(m, lds, w);
+      return row_waves.sum(m);
     };
     // Bounds of the k-th largest: the largest key above; below, as many keys as there are lanes
     // with one, each lane's largest, are at least the smallest of those.
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) most = max(most, key[i]);
-    uint32_t hi = row_max<W>(wave_umax(most), lds, w);
-    top = row_max<W>(need <= WAVE ? ~wave_umax(~most) : 0u, lds, w);
+    uint32_t hi = row_waves.most(wave_umax(most));
+    top = row_waves.most(need <= WAVE ? ~wave_umax(~most) : 0u);
     int kept = 0;  // keys that are at least `top` (0: not counted)
 #pragma unroll 1
     while (top < hi && kept != need) {
@@ -106,14 +118,8 @@ __global__ __launch_bounds__(256) void k_select(mono_prompt_select_args a) {
       eq += __popcll(__ballot(open(i) && key[i] == top));
       gt += __popcll(__ballot((always >> i & 1) || (key[i] > top)));
     }
-    __syncthreads();
-    if (lane == 0) lds[w] = eq;
-    __syncthreads();
-    for (int v = 0; v < w; ++v) ties_before += lds[v];
-    __syncthreads();
-    if (lane == 0) lds[w] = gt;
-    __syncthreads();
-    for (int v = 0; v < w; ++v) taken_before += lds[v];
+    ties_before = row_waves.before(eq);
+    taken_before = row_waves.before(gt);
     taken_before += min(ties_before, border);
   }
   int at = taken_before, ties = ties_before;
@@ -143,6 +149,7 @@ hipError_t select_pages(const mono_prompt_select_args& a, hipStream_t st) {
   if (a.columns <= 128) return launch(k_select<1, 2>, 4);
   if (a.columns <= 256) return launch(k_select<1, 4>, 4);
   if (a.columns <= 512) return launch(k_select<1, 8>, 4);
+  if (a.columns <= 1024) return launch(k_select<1, 16>, 4);
   if (a.columns <= 2048) return launch(k_select<4, 8>, 1);
   return launch(k_select<4, 32>, 1);  // 8192 columns: MAX_COLUMNS
 }
