@@ -6,18 +6,33 @@
 // A workgroup takes a token and up to 32 of its heads, and walks through pages of 64 keys with
 // a running maximum and sum. A page is one piece of 36 KB, brought to LDS as it lies by DMA
 // (global_load_lds), the next one while this one is worked on, and read from there twice: as
-// rows for q . c and transposed (ds_read_b64_tr_b8) for p . v, widened to bf16 in registers
-// each time, exactly.
+// rows for q . c and transposed (ds_read_b64_tr_b8) for p . v.
 //
-//   q . c   wave w: keys 16 w .. + 15 against every head, whose q stays in registers
-//   p . v   wave w: dims 128 w .. + 127 over all 64 keys; the probabilities meet in LDS
+//   q . c   wave w: keys 16 w .. + 15 against every head, in E4M3 as the cache has them
+//   p . v   wave w: dims 128 w .. + 127 over all 64 keys, widened to bf16 in registers, exactly;
+//           the probabilities meet in LDS
 //
-// The maximum that the sums refer to stays as it is until a logit passes it by 2^8 (a ratio of
-// sums does not depend on it, bf16 and f32 hold 2^8 as well as 1): the waves' maxima then meet
+// q is split into two E4M3 pieces of four significant bits, which hold bf16's eight: q . c is then
+// two FP8 products of twice bf16's rate and the keys are not widened. What is below 2^-14 of its head's
+// largest element loses bits: an element is off by 2^-21.8 of the largest at most, in the last 64
+// dims, whose pieces share an instruction and so a scale, by 2^-17.8 (a logit's f32 sum over 576
+// terms is off by as much). When this came in place of q in bf16 and widened keys, 4096 tokens went from
+// 648 to 624 us and one from 17 to 14.
+//
+// Probabilities times their key's scale are rounded to bf16, off by 2^-8 of each at most and at random,
+// beside the output's own 2^-8; their sum adds up the f32 values. (Two E4M3 pieces of them were tried:
+// small ones lose bits against the largest, which outputs that hang on many keys show.)
+//
+// The maximum that the sums refer to stays as it is until a probability passes 2^4 (a ratio of
+// sums does not depend on it, and bf16 and f32 hold 2^4 as well as 1): the waves' maxima then meet
 // and the sums are scaled, which happens on a token's first page and rarely after it.
 //
-// Probabilities are rounded to bf16 for the matrix unit, 2^-9 of each at random beside the
-// output's own 2^-9; their sum adds up the f32 values.
+// Two workgroups a CU (80 KB of LDS, 256 registers a lane), a page of 32 heads in 1.2 us a CU:
+// 4096 tokens of 32 heads over 2048 keys 606 us, 950 TFLOP/s; a large bf16 product reaches 1180. Matrix
+// instructions, the widening and the probabilities' vector work, at a clock that power holds at
+// 1.75 to 1.9 GHz, are what bounds it. Heads of up to 16 take one tile of 16 (2000 tokens 265 us,
+// in a half-empty tile of 32 304), up to 32 two side by side (2000 tokens 314 us, as two workgroups
+// 516, which read the pages twice).
 #include "prompt_common.h"
 
 namespace mono {
@@ -203,9 +218,13 @@ MONO_DEV Request request_of(const Paged& a, int r) {
 
 // Trees of few nodes: each node's pages in chunks of so many, a request's nodes side by side over
 // the same chunk: the fewest pages a chunk that make at most `most` tasks, between their share of
-// all pages and that of all pages beside a short chunk a node. Two workgroups a CU, but one where
-// that leaves it a few pages only: fewer parts to write and join are then worth more. `tasks`
-// comes to be how many there are.
+// all pages and that of all pages beside a short chunk a node. `tasks` comes to be how many there are.
+//
+// Two workgroups a CU, but one where that has FEW_PAGES pages at most: fewer parts to write and
+// join are then worth more (20000 keys, 512 and 256 tasks: 4 nodes 33.1 and 31.9 us, 8 nodes 38.3 and
+// 40.0, 16 nodes 46.8 and 51.4; 4000 keys, 16 nodes 33.4 and 27.6). And whole nodes where chunks save
+// at most JOIN_PAGES pages (9 pages a node, 128 nodes: in twos 34 us, whole 28.5; 64 nodes, in threes 25,
+// whole 27).
 constexpr int FEW_PAGES = 8, JOIN_PAGES = 4;
 MONO_DEV int chunk_pages(const Paged& a, int lane, const Request& head, int64_t& tasks) {  // (head: request `lane`)
   const auto over = [&](auto of) {  // the requests' sum
@@ -649,8 +668,9 @@ __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
   attend<MT, TREE>(a, L, lane, wave, task, rd);
 }
 
-// A head's parts as one, each scaled to the largest of their maxima. A workgroup takes 512 / S of
-// its dims, wave w of W every W-th part, eight of them in flight; the waves' sums meet in LDS.
+// A head's parts as one, each scaled to the largest of their maxima, in the parts' order. A
+// workgroup takes 512 / S of its dims, wave w of W every W-th part, eight of them in flight; the waves'
+// sums meet in LDS.
 constexpr int MAX_SPLITS = 512, JOIN_AHEAD = 8;
 template <int W, int S>
 __global__ __launch_bounds__(W * WAVE) void k_join(Paged a) {
@@ -726,6 +746,9 @@ hipError_t paged_attention(const Paged& a, hipStream_t st) {
 
 hipError_t join_attention(const Paged& a, hipStream_t st) {
   const int64_t heads = a.tokens * a.heads;
+  // Few heads have many parts each, and too few workgroups: four waves each and four workgroups
+  // (attention and join: 1 node of 32 heads, 20000 keys 25.6 us, one wave 37.5; 4 nodes 32.7 and 36.2).
+  // From 512 heads on one wave does (16 nodes, 1000 keys 23.1 and 23.9, 64 nodes 32.3 and 42.0).
   if (heads <= 256)
     k_join<4, 4><<<(uint32_t)(4 * heads), 4 * WAVE, 0, st>>>(a);
   else

@@ -7,7 +7,12 @@
 // wants it, with half its heads' weights, the next page's keys come ahead. A 32 x 32 MFMA's lanes
 // hold one key each and 16 heads: the ReLU and the weighted sum are two FMAs a value, and a key's
 // heads meet in one swap of halves. They bound the kernel: some 150 vector operations a token and
-// page beside 256 cycles of MFMA.
+// page beside 256 cycles of MFMA. 8192 tokens from position 0: 200 us, 2.75 PFLOP/s (a maximum and an
+// FMA a value: 290 us; the products alone would take some 65).
+//
+// FP4 products and their sum are exact in f32 where a query's and a key's scales lie close; the weighted sum is
+// f32 throughout. As x / 2 + |x| / 2 a head's ReLU leaves a rounding of the size of a product that it
+// cuts off, 2^-24 of it.
 #include <algorithm>
 
 #include "prompt_common.h"
@@ -145,7 +150,9 @@ __global__ __launch_bounds__(WAVES * WAVE, 4) void k_scores(mono_prompt_scores_a
 
 hipError_t page_scores(const mono_prompt_scores_args& a, hipStream_t st) {
   const int64_t groups = (a.tokens + WAVES - 1) / WAVES;
-  // pages a workgroup: as many as leave 4096 workgroups, four rounds of them (a run's query is loaded once)
+  // pages a workgroup: as many as leave 2048 workgroups, two rounds of them (a run's query is loaded
+  // once; 64 tokens of 30000 keys: 2048 workgroups 16.8 us, 4096 24.5, 512 19.7), but 32 at most
+  // (8192 tokens: 16 pages a run 235 us, 32 230)
   const int run = (int)std::min<int64_t>(std::max<int64_t>(groups * a.columns / 2048, 1), 32);
   const int64_t runs = (a.columns + run - 1) / run;
   k_scores<<<(uint32_t)(groups * runs), WAVES * WAVE, 0, st>>>(a, run, (uint32_t)groups);
