@@ -13,11 +13,11 @@
 //           the probabilities meet in LDS
 //
 // q is split into two E4M3 pieces of four significant bits, which hold bf16's eight: q . c is then
-// two FP8 products of twice bf16's rate and the keys are not widened. What is below 2^-14 of its head's
-// largest element loses bits: an element is off by 2^-21.8 of the largest at most, in the last 64
-// dims, whose pieces share an instruction and so a scale, by 2^-17.8 (a logit's f32 sum over 576
-// terms is off by as much). When this came in place of q in bf16 and widened keys, 4096 tokens went from
-// 648 to 624 us and one from 17 to 14.
+// two FP8 products of twice bf16's rate and the keys are not widened. Elements below 2^-14 of their
+// head's largest (2^-10 in the last 64 dims, whose pieces share an instruction and so a scale) lose
+// bits: they are off by 2^-21.8 (2^-17.8) of the largest at most, as a logit's f32 sum over 576 terms
+// is of its own. When this came in place of q in bf16 and widened keys, 4096 tokens went from 648 to
+// 624 us and one from 17 to 14.
 //
 // Probabilities times their key's scale are rounded to bf16, off by 2^-8 of each at most and at random,
 // beside the output's own 2^-8; their sum adds up the f32 values. (Two E4M3 pieces of them were tried:

@@ -23,7 +23,8 @@ A call takes at most 1048576 rows (``experts``: tokens times (picks + 1), 116508
 8 picks) and 2^35 elements of them. Scratch: a product K * (1 + 1/32) bytes a row, and f32
 parts where its tiles are few; ``experts`` mostly 2 * H bytes for each token's every pick
 (1.2 GB for 8192 tokens of 7168 with 8 picks and the shared expert), so a long prompt goes
-through it in pieces of some thousand tokens. A captured graph keeps its calls' scratch.
+through it in pieces of some thousand tokens; both attentions f32 parts of up to 256 tokens' (nodes')
+pages, 512 of [heads, 512] at most (34 MB at 32 heads). A captured graph keeps its calls' scratch.
 """
 
 from __future__ import annotations
@@ -390,7 +391,8 @@ def attention(q: torch.Tensor, req: torch.Tensor, pos: torch.Tensor, pages: torc
     Token i is position ``pos[i]`` of request ``req[i]``, a row of ``page_table`` [requests,
     pages] (all i32). A listed page outside the table or the pool is none, one that is listed
     twice counts twice. A token that sees no key has zeros. Keys that a token does not see may
-    hold anything. ``out`` must share no memory with ``q``."""
+    hold anything. An element of ``q`` is held to 2^-21.8 of its head's largest (2^-17.8 in the
+    last 64 dims), which is all of bf16 for those above 2^-14 (2^-10) of it. ``out`` must share no memory with ``q``."""
     dev = _gpu(q, "q")
     n_pages, out = _latents(q, caches, out, dev)
     t, heads = q.shape[:2]
