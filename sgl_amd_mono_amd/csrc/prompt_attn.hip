@@ -201,22 +201,34 @@ MONO_DEV void node_reads(const Paged& a, int64_t t, int req, Reads& rd) {
 }
 
 // A request's nodes and pages (the last one or two hold the draft's keys; MOST_PAGES: more than the
-// card's memory holds, and PLANNED times as many are counted in 32 bits).
-constexpr int MOST_PAGES = (1 << 23) - 16;
+// card's memory holds).
+constexpr int MOST_PAGES = 1 << 23;
 struct Request {
   int64_t first;
   int n, pages;
 };
 MONO_DEV Request request_of(const Paged& a, int r) {
-  Request q = {0, 0, 0};
-  if (r >= a.requests) return q;
-  q.first = min((int64_t)max(a.starts[r], 0), a.tokens);
-  q.n = (int)max(min((int64_t)a.starts[r + 1], a.tokens) - q.first, (int64_t)0);
-  q.pages = q.n ? (int)min((int64_t)min(a.pt_stride, MOST_PAGES), ((int64_t)max(a.prefix[r], 0) + PAGE - 1) / PAGE + 1) : 0;
+  const int at = min(r, a.requests - 1);
+  const int from = a.starts[at], to = a.starts[at + 1], prefix = a.prefix[at];
+  Request q;
+  q.first = min((int64_t)max(from, 0), a.tokens);
+  q.n = r < a.requests ? (int)max(min((int64_t)to, a.tokens) - q.first, (int64_t)0) : 0;
+  q.pages = q.n ? (int)min((int64_t)min(a.pt_stride, MOST_PAGES), ((int64_t)max(prefix, 0) + PAGE - 1) / PAGE + 1) : 0;
   return q;
 }
+// Lane l: requests l, 64 + l, .. of up to PLAN_REQUESTS.
+constexpr int REQUEST_SETS = PLAN_REQUESTS / WAVE;
+struct Requests {
+  Request of[REQUEST_SETS];
+};
+template <class F>
+MONO_DEV void each_set(const Paged& a, F f) {
+#pragma unroll
+  for (int i = 0; i < REQUEST_SETS; ++i)
+    if (i == 0 || WAVE * i < a.requests) f(i);
+}
 
-// Trees of few nodes: each node's pages in chunks of so many, a request's nodes side by side over
+// Planned trees: each node's pages in chunks of so many, a request's nodes side by side over
 // the same chunk: the fewest pages a chunk that make at most `most` tasks, between their share of
 // all pages and that of all pages beside a short chunk a node. `tasks` comes to be how many there are.
 //
@@ -224,45 +236,49 @@ MONO_DEV Request request_of(const Paged& a, int r) {
 // join are then worth more (20000 keys, 512 and 256 tasks: 4 nodes 33.1 and 31.9 us, 8 nodes 38.3 and
 // 40.0, 16 nodes 46.8 and 51.4; 4000 keys, 16 nodes 33.4 and 27.6). And whole nodes where chunks save
 // at most JOIN_PAGES pages (9 pages a node, 128 nodes: in twos 34 us, whole 28.5; 64 nodes, in threes 25,
-// whole 27).
+// whole 27). More nodes than one round's half are whole but for those longer than a workgroup's share.
 constexpr int FEW_PAGES = 8, JOIN_PAGES = 4;
-MONO_DEV int chunk_pages(const Paged& a, int lane, const Request& head, int64_t& tasks) {  // (head: request `lane`)
-  const auto over = [&](auto of) {  // the requests' sum
-    int total = wave_sum_i(head.n * of(head.pages));
-    for (int r0 = WAVE; r0 < a.requests; r0 += WAVE) {
-      const Request q = request_of(a, r0 + lane);
-      total += wave_sum_i(q.n * of(q.pages));
-    }
-    return total * a.head_tiles;
+MONO_DEV int chunk_pages(const Paged& a, const Requests& r, int64_t& tasks) {
+  int64_t total = 0;
+  uint32_t longest = 0;
+  each_set(a, [&](int i) {
+    const int64_t pages = (int64_t)r.of[i].n * r.of[i].pages;
+    total += wave_sum_i((int)(pages & 0xffff)) + ((int64_t)wave_sum_i((int)(pages >> 16)) << 16);
+    longest = max(longest, wave_umax((uint32_t)r.of[i].pages));
+  });
+  total *= a.head_tiles;
+  const auto share = [](int64_t n, int by) { return (int)max((n + by - 1) / by, (int64_t)1); };
+  const auto made = [&](int each) {
+    int n = 0;
+    each_set(a, [&](int i) { n += wave_sum_i(r.of[i].n * ((r.of[i].pages + each - 1) / each)); });
+    return n * a.head_tiles;
   };
-  const auto share = [](int n, int by) { return max((n + by - 1) / by, 1); };
-  const int total = over([](int pages) { return pages; }), least = (int)a.tokens * a.head_tiles;
-  const int most = total <= FULL / 2 * FEW_PAGES && least <= FULL / 4 ? FULL / 2 : FULL;
-  uint32_t longest = wave_umax((uint32_t)head.pages);
-  for (int r0 = WAVE; r0 < a.requests; r0 += WAVE) longest = max(longest, wave_umax((uint32_t)request_of(a, r0 + lane).pages));
-  int lo = share(total, most), hi = share(total, most - least);
-  const auto made = [&](int each) { return over([&](int pages) { return (pages + each - 1) / each; }); };
+  const int least = (int)a.tokens * a.head_tiles;
+  const int most = total <= FULL / 2 * FEW_PAGES && least <= FULL / 4 ? FULL / 2 : (int)a.work;
+  int lo = share(total, min(most, FULL)), hi = max(share(total, most - least), lo);
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
     if (made(mid) <= most) hi = mid;
     else lo = mid + 1;
   }
   if ((int)longest <= hi + JOIN_PAGES) hi = max((int)longest, 1);
-  tasks = min(made(hi), FULL);  // (more only by starts that do not ascend)
+  tasks = min((int64_t)made(hi), a.work);  // (more only by starts that do not ascend)
   return hi;
 }
 
 // Task `id` of them; false behind the last.
-MONO_DEV bool planned_task(const Paged& a, int lane, const Request& head, int each, int id, Task& k, Reads& rd) {
+MONO_DEV bool planned_task(const Paged& a, const Requests& r, int each, int id, Task& k, Reads& rd) {
   k.ht = id % a.head_tiles;
   id /= a.head_tiles;
   int part = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += WAVE) {
-    const Request q = r0 ? request_of(a, r0 + lane) : head;
+  bool found = false;
+  each_set(a, [&](int i) {
+    const Request q = r.of[i];
     const int chunks = (q.pages + each - 1) / each, tasks = q.n * chunks, parts = chunks > 1 ? tasks : 0;
     const int upto = wave_incl_scan(tasks), parts_upto = wave_incl_scan(parts);
     const uint64_t here = __ballot(upto > id);
-    if (here) {
+    if (here && !found) {
+      found = true;
       const int l = __builtin_ctzll(here);
       const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
       const int nodes = of(q.n), at = id - (of(upto) - of(tasks)), node = at % nodes;
@@ -270,16 +286,15 @@ MONO_DEV bool planned_task(const Paged& a, int lane, const Request& head, int ea
       k.chunks = of(chunks);
       k.part = part + of(parts_upto) - of(parts) + node * k.chunks + k.chunk;
       k.t = (int64_t)of((int)q.first) + node;
-      node_reads(a, k.t, r0 + l, rd);
+      node_reads(a, k.t, WAVE * i + l, rd);
       rd.lo = k.chunk * each;
       rd.hi = min(rd.lo + each, of(q.pages));
       k.any = true;
-      return k.part < a.parts;  // (starts that do not ascend: nothing is written behind the parts)
     }
     id -= __builtin_amdgcn_readlane(upto, WAVE - 1);
     part += __builtin_amdgcn_readlane(parts_upto, WAVE - 1);
-  }
-  return false;
+  });
+  return found && (k.chunks == 1 || k.part < a.parts);  // (more parts only by starts that do not ascend)
 }
 
 template <bool TREE>
@@ -648,12 +663,12 @@ __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
   const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   int64_t tasks = a.work;
   int pages = 0;
-  Request head;
+  Requests requests;
   if (PLANNED) {
     for (int64_t t = (int64_t)blockIdx.x * T + threadIdx.x; t < a.tokens; t += (int64_t)gridDim.x * T)
       if (t < a.starts[0] || t >= a.starts[a.requests]) a.plan[t] = NodePlan{0, 0};  // nodes of no request
-    head = request_of(a, lane);
-    pages = chunk_pages(a, lane, head, tasks);
+    each_set(a, [&](int i) { requests.of[i] = request_of(a, WAVE * i + lane); });
+    pages = chunk_pages(a, requests, tasks);
   }
   const int64_t id = task_id(blockIdx.x, tasks);
   if (id < 0) return;
@@ -662,26 +677,33 @@ __global__ __launch_bounds__(T, 2) void k_pages(Paged a) {
   if (!PLANNED)
     task_of<TREE>(a, lane, id, task, rd);
   else {
-    if (!planned_task(a, lane, head, pages, (int)id, task, rd)) return;
+    if (!planned_task(a, requests, pages, (int)id, task, rd)) return;
     if (threadIdx.x == 0 && task.ht == 0 && task.chunk == 0) a.plan[task.t] = NodePlan{task.chunks, (int)task.part};
   }
   attend<MT, TREE>(a, L, lane, wave, task, rd);
 }
 
-// A head's parts as one, each scaled to the largest of their maxima, in the parts' order. A
-// workgroup takes 512 / S of its dims, wave w of W every W-th part, eight of them in flight; the waves'
-// sums meet in LDS.
-constexpr int MAX_SPLITS = 512, JOIN_AHEAD = 8;
-template <int W, int S>
-__global__ __launch_bounds__(W * WAVE) void k_join(Paged a) {
-  __shared__ float by[MAX_SPLITS + JOIN_AHEAD * W];
+// A head's parts as one, each scaled to the largest of their maxima, in the parts' order. Wave w of
+// W takes every W-th part, eight of them in flight; the waves' sums meet in LDS. A workgroup takes
+// 512 / S dims of a head, or H heads, a wave each.
+constexpr int MAX_SPLITS = FULL + 1, JOIN_AHEAD = 8;  // (a node alone beside FULL more tasks)
+template <int W, int S, int H>
+__global__ __launch_bounds__(W * H * WAVE) void k_join(Paged a) {
+  static_assert(W == 1 || H == 1, "waves share a head or have one each");
   constexpr int N = LATENT / S, V = N / WAVE;  // dims: of the workgroup, of a lane
   typedef float Vec __attribute__((ext_vector_type(V < 4 ? V : 4)));
   constexpr int VECS = V < 4 ? 1 : V / 4, EACH = V / VECS;
-  __shared__ alignas(16) float sums[W][N];
-  const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-  const int slice = blockIdx.x % S, h = blockIdx.x / S % a.heads;
-  const int64_t t = blockIdx.x / S / a.heads;
+  __shared__ float weights[H][MAX_SPLITS + JOIN_AHEAD * W];
+  __shared__ alignas(16) float sums[W * H][N];
+  const int lane = threadIdx.x % WAVE, wv = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), wave = wv % W, tid = WAVE * wave + lane;
+  float* by = weights[wv / W];
+  const auto meet_waves = [&]() {
+    if (W > 1) __syncthreads();
+    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
+  const int64_t row = (int64_t)(blockIdx.x / S) * H + wv / W, t = row / a.heads;
+  const int slice = blockIdx.x % S, h = (int)(row % a.heads);
+  if (t >= a.tokens) return;
   int splits = a.splits;
   int64_t part = t * a.splits;
   if (a.plan) {
@@ -702,7 +724,7 @@ __global__ __launch_bounds__(W * WAVE) void k_join(Paged a) {
   if (wave == 0)
     for (int i = lane; i < JOIN_AHEAD * W; i += WAVE) by[splits + i] = -1.f;
   l = wave_sum(l);
-  __syncthreads();
+  meet_waves();
   float o[V] = {};
   for (int s0 = wave; s0 < splits; s0 += JOIN_AHEAD * W) {
     Vec v[JOIN_AHEAD][VECS];
@@ -720,14 +742,14 @@ __global__ __launch_bounds__(W * WAVE) void k_join(Paged a) {
     }
   }
 #pragma unroll
-  for (int j = 0; j < V; ++j) sums[wave][N / VECS * (j / EACH) + EACH * lane + j % EACH] = o[j];
-  __syncthreads();
+  for (int j = 0; j < V; ++j) sums[wv][N / VECS * (j / EACH) + EACH * lane + j % EACH] = o[j];
+  meet_waves();
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   uint32_t* out = static_cast<uint32_t*>(a.out) + (t * a.heads + h) * (LATENT / 2) + N / 2 * slice;
   for (int u = tid; u < N / 2; u += W * WAVE) {
     float r[2] = {0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < W; ++w) r[0] += sums[w][2 * u], r[1] += sums[w][2 * u + 1];
+    for (int w = 0; w < W; ++w) r[0] += sums[wv - wave + w][2 * u], r[1] += sums[wv - wave + w][2 * u + 1];
     out[u] = pack2(r[0] * inv, r[1] * inv);
   }
 }
@@ -748,11 +770,15 @@ hipError_t join_attention(const Paged& a, hipStream_t st) {
   const int64_t heads = a.tokens * a.heads;
   // Few heads have many parts each, and too few workgroups: four waves each and four workgroups
   // (attention and join: 1 node of 32 heads, 20000 keys 25.6 us, one wave 37.5; 4 nodes 32.7 and 36.2).
-  // From 512 heads on one wave does (16 nodes, 1000 keys 23.1 and 23.9, 64 nodes 32.3 and 42.0).
+  // From 512 heads on one wave does (16 nodes, 1000 keys 23.1 and 23.9, 64 nodes 32.3 and 42.0). Of
+  // thousands of heads most were written whole: four a workgroup (1000 nodes, 500 keys 64 us and 68, but
+  // 16 nodes 24.9 and 22.3).
   if (heads <= 256)
-    k_join<4, 4><<<(uint32_t)(4 * heads), 4 * WAVE, 0, st>>>(a);
+    k_join<4, 4, 1><<<(uint32_t)(4 * heads), 4 * WAVE, 0, st>>>(a);
+  else if (heads <= 2048)
+    k_join<1, 1, 1><<<(uint32_t)heads, WAVE, 0, st>>>(a);
   else
-    k_join<1, 1><<<(uint32_t)heads, WAVE, 0, st>>>(a);
+    k_join<1, 1, 4><<<(uint32_t)((heads + 3) / 4), 4 * WAVE, 0, st>>>(a);
   return hipGetLastError();
 }
 

@@ -192,11 +192,12 @@ struct NodePlan {
 
 // How the pages are shared out. Only where the tokens' heads alone would leave CUs without
 // work: two workgroups a CU (FULL), a page each at least. A tree's pages are known on the device
-// only; up to PLANNED nodes' tiles of heads its workgroups plan there, so that there are workgroups
-// enough to give long nodes two or more. Planned and not, 4000 keys: 64 nodes 44 and 101 us, 256 nodes
-// 98 and 114, 256 of ragged requests 49 and 97; 500 keys: 64 nodes 24.4 and 23.5, 256 nodes 30 and 28
-// (the plan and a join that finds nothing cost 1 to 3 us).
-constexpr int FULL = 512, PLANNED = FULL / 2;
+// only; with up to PLANNED nodes' tiles of heads, of up to PLAN_REQUESTS requests, its workgroups plan
+// there, FULL of them or FULL more than tiles, so that long nodes have two or more. Planned and not:
+// 4000 keys, 64 nodes 44 and 101 us, 256 nodes 98 and 114, 256 of ragged requests 49 and 97; 8 nodes of 30000
+// keys beside 480 shorter ones 139 and 616. The plan and a join that finds little cost what it
+// costs: 500 keys, 64 nodes 24.4 and 23.5, 512 nodes 37 and 34, 1000 nodes 64 and 59.
+constexpr int FULL = 512, PLANNED = 1024, PLAN_REQUESTS = 256;
 inline void paged_plan(Paged& a, int pages) {
   a.head_rows = a.heads <= 16 ? 16 : 32;
   a.head_tiles = (a.heads + a.head_rows - 1) / a.head_rows;
@@ -204,7 +205,12 @@ inline void paged_plan(Paged& a, int pages) {
   a.splits = 1;
   a.work = whole;
   if (a.starts) {
-    if (whole <= PLANNED && pages > 1) a.tasks = a.work = FULL, a.parts = std::min<int64_t>(FULL / a.head_tiles, a.tokens * pages);
+    if (whole <= PLANNED && pages > 1 && a.requests > 0 && a.requests <= PLAN_REQUESTS) {
+      const int64_t spare = whole <= FULL / 2 ? FULL - whole : FULL;  // tasks beside one a node's tile
+      a.tasks = a.work = whole + spare;
+      // nodes of two chunks or more: with as many nodes as spare tasks they have most parts
+      a.parts = std::min<int64_t>((spare + std::min(spare, whole)) / a.head_tiles, a.tokens * pages);
+    }
     return;
   }
   const int64_t fit = FULL / whole;

@@ -49,7 +49,7 @@ size_t paged_space(void* ws, int pages, Paged& p) {
 int64_t paged_workspace(int64_t tokens, int32_t heads, int pages, bool tree) {
   Paged p{};
   const int32_t some = 0;
-  p.tokens = tokens, p.heads = heads, p.starts = tree ? &some : nullptr;
+  p.tokens = tokens, p.heads = heads, p.requests = 1, p.starts = tree ? &some : nullptr;
   mono::abi_ok();
   return tokens ? (int64_t)paged_space(nullptr, pages, p) : 0;
 }
@@ -63,8 +63,8 @@ int run_paged(Paged& p, int pages, float scale, void* ws, int64_t ws_bytes, void
   if (p.kv_scale)
     if (int rc = need(p.kv_scale, "kv_scale", 16)) return rc;
   if (int rc = need(p.out, "out", 16)) return rc;
-  if (!std::isfinite(scale)) return refuse("softmax_scale must be finite, got %f", (double)scale);
   p.scale_log2 = (float)(scale * 1.4426950408889634);
+  if (!std::isfinite(p.scale_log2)) return refuse("softmax_scale must be finite, also times log2(e), got %g", (double)scale);
   if (const size_t bytes = paged_space(nullptr, pages, p)) {
     if (int rc = need_space(ws, ws_bytes, bytes)) return rc;
     paged_space(ws, pages, p);

@@ -23,8 +23,8 @@ A call takes at most 1048576 rows (``experts``: tokens times (picks + 1), 116508
 8 picks) and 2^35 elements of them. Scratch: a product K * (1 + 1/32) bytes a row, and f32
 parts where its tiles are few; ``experts`` mostly 2 * H bytes for each token's every pick
 (1.2 GB for 8192 tokens of 7168 with 8 picks and the shared expert), so a long prompt goes
-through it in pieces of some thousand tokens; both attentions f32 parts of up to 256 tokens' (nodes')
-pages, 512 of [heads, 512] at most (34 MB at 32 heads). A captured graph keeps its calls' scratch.
+through it in pieces of some thousand tokens; both attentions f32 parts, of up to 256 tokens or 1024
+nodes of 32 heads 512 or 1024 of [heads, 512] at most (34 or 67 MB). A captured graph keeps its calls' scratch.
 """
 
 from __future__ import annotations

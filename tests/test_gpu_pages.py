@@ -493,6 +493,9 @@ def test_tree_attention_wide(gpu_device):
     ([(255 * PAGE, 8)], 16), ([(255 * PAGE + 1, 8)], 16),  # 2048 nodes' pages, 2056
     ([(50 * PAGE, 16)], 16), ([(50 * PAGE, 17)], 16),  # 256 heads, 272
     ([(9, 64), (700, 64)], 16), ([(9, 64), (700, 65)], 16),  # 128 nodes, 129
+    ([(3000, 2)] + [(10, 30)] * 20, 8), ([(10, 64)] * 5 + [(2000, 5), (0, 0), (64, 63)], 64),  # long nodes among 602, 388 x 2 tiles
+    ([(0, 64)] * 15 + [(1200, 64)], 4), ([(0, 64)] * 15 + [(1200, 65)], 4),  # 1024 nodes, 1025
+    ([(30, 1)] * 255 + [(1500, 1)], 4), ([(30, 1)] * 256 + [(1500, 1)], 4), ([(30, 2)] * 200 + [(0, 0)] * 55 + [(2500, 1)], 4),  # requests: 256, 257
     ([(140_000, 1)], 4), ([(40_000, 1)], 33), ([(5, 1)] * 64 + [(3000, 2)] * 3 + [(0, 0)] * 70 + [(64, 1)], 16),
 ])  # fmt: skip
 def test_tree_attention_shared_out_or_not(gpu_device, trees, heads):

@@ -71,6 +71,7 @@ SHARED = [
     (dict(n_pages=-1), "n_pages"), (dict(q=None), "q must"), (dict(q=P + 8), "q must"), (dict(page_table=None), "page_table"),
     (dict(kv=P + 8), "kv must"), (dict(kv_scale=P + 4), "kv_scale"), (dict(out=None), "out"), (dict(out=P + 8), "out"),
     (dict(softmax_scale=float("nan")), "softmax_scale"), (dict(softmax_scale=float("inf")), "softmax_scale"),
+    (dict(softmax_scale=3e38), "softmax_scale"),
     (dict(workspace=None), "workspace"), (dict(workspace=P + 16), "workspace"), (dict(workspace_bytes=100), "workspace must hold"),
 ]  # fmt: skip
 
