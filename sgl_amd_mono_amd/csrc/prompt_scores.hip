@@ -87,14 +87,14 @@ MONO_DEV float key_scores(const Query& q, const Keys& k) {
   return swap_halves(s[0], s[1], OpAdd());
 }
 
-__global__ __launch_bounds__(WAVES * WAVE, 4) void k_scores(mono_prompt_scores_args a, int run, uint32_t groups) {
+__global__ __launch_bounds__(WAVES * WAVE, 4) void k_scores(mono_prompt_scores_args a, int run) {
   const int lane = threadIdx.x % WAVE, half = lane / 32, r = lane % 32;
   // the workgroup's waves take neighbouring tokens over the same pages, which the CU's cache then holds
   // (and the runs of pages lie far apart in the grid: late pages are seen by late tokens only, and
   // workgroups a few apart share an XCD)
-  const int64_t t = (int64_t)(blockIdx.x % groups) * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int64_t t = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   if (t >= a.tokens) return;
-  const int p0 = (int)(blockIdx.x / groups) * run, p1 = min(p0 + run, a.columns);
+  const int p0 = (int)blockIdx.y * run, p1 = min(p0 + run, a.columns);
   const int pos = min(a.pos[t], PAGE * p1 - 1), req = a.req[t];
   // how many keys from page p0 on the token sees, and in how many pages
   const int seen = pos >= 0 && req >= 0 && req < a.requests ? max(pos + 1 - PAGE * p0, 0) : 0, n = (seen + PAGE - 1) / PAGE;
@@ -155,7 +155,7 @@ hipError_t page_scores(const mono_prompt_scores_args& a, hipStream_t st) {
   // (8192 tokens: 16 pages a run 235 us, 32 230)
   const int run = (int)std::min<int64_t>(std::max<int64_t>(groups * a.columns / 2048, 1), 32);
   const int64_t runs = (a.columns + run - 1) / run;
-  k_scores<<<(uint32_t)(groups * runs), WAVES * WAVE, 0, st>>>(a, run, (uint32_t)groups);
+  k_scores<<<dim3((uint32_t)groups, (uint32_t)runs), WAVES * WAVE, 0, st>>>(a, run);  // (one dim holds 2^32 threads)
   return hipGetLastError();
 }
 

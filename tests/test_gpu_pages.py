@@ -736,3 +736,45 @@ def test_captured_trees_follow_their_lengths(gpu_device):
             assert torch.equal(out, prompt.tree_attention(**s, page_table=table, caches=c))
     s = held[0][0]
     _tree_near(s["q"], s["starts"], s["prefix"], s["mask"], table, c)
+
+
+def test_rows_far_into_their_tensors(gpu_device):
+    """Offsets past 2^31 elements: the last rows of wide calls are those of small ones."""
+    dev = gpu_device
+    torch.cuda.empty_cache()
+    tokens, last = 270_000, 5
+    req, pos, table, pages = _requests(dev, [(300, last)])
+    iq, iqs, iw, caches = _index(dev, last, pages)
+    cos, sin = workloads.rope_tables(400, dev)
+
+    def behind(t, fill=0):  # the rows of t behind so many others
+        wide = torch.empty(tokens, *t.shape[1:], dtype=t.dtype, device=dev)
+        wide[:-last] = fill
+        wide[-last:] = t
+        return wide
+
+    x = torch.randn(last, 8192, device=dev).to(torch.bfloat16)
+    for got, want in zip(prompt.index_query(behind(x), behind(pos, -1), cos, sin), prompt.index_query(x, pos, cos, sin)):
+        assert torch.equal(got[-last:], want)
+        del got
+    want = prompt.page_scores(iq, iqs, iw, req, pos, table, caches, 8192)
+    scores = prompt.page_scores(behind(iq), behind(iqs), behind(iw), behind(req, -1), behind(pos), table, caches, 8192)
+    assert torch.equal(scores[-last:], want) and bool((scores[-last - 1] == -torch.inf).all())
+    picked = prompt.select_pages(scores, behind(pos, -1), 8000)
+    assert torch.equal(picked[-last:], prompt.select_pages(want, pos, 8000)) and bool((picked[-last - 1] == -1).all())
+    del scores, picked
+    torch.cuda.empty_cache()
+    tokens = 70_000
+    c, q = _pool(dev, pages, False), _q(dev, last, 64)
+    ids = torch.tensor([[0, 3, 4]] * last, dtype=torch.int32, device=dev)
+    want = prompt.attention(q, req, pos, ids, table, c)
+    wide = behind(q)
+    got = prompt.attention(wide, behind(req, -1), behind(pos), behind(ids), table, c)
+    assert float((got[-last:] - want).float().norm() / want.float().norm()) <= 2.0**-7 and bool((got[-last - 1] == 0).all())
+    del got
+    tree = (torch.tensor([300], dtype=torch.int32, device=dev), torch.arange(1, last + 1, device=dev))
+    want = prompt.tree_attention(q, torch.tensor([0, last], dtype=torch.int32, device=dev), *tree, table, c)
+    got = prompt.tree_attention(wide, torch.tensor([tokens - last, tokens], dtype=torch.int32, device=dev), tree[0], behind(tree[1]), table, c)
+    assert float((got[-last:] - want).float().norm() / want.float().norm()) <= 2.0**-7 and bool((got[-last - 1] == 0).all())
+    del got, wide
+    torch.cuda.empty_cache()
