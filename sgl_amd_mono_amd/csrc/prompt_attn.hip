@@ -470,9 +470,15 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
           const uint32_t ln = lane_now(lane), at_lane = lane_place();
           const uint8_t* key = &st.kv[(16 * wave + ln % 16) * 64 + 16 * unit_of(ln % 16, ln / 16)];
           const auto unit = [&](int b) { return *reinterpret_cast<const u32x4*>(key + BLOCK_BYTES * b); };
+          i32x8 coming = join(unit(0), unit(1));  // (the next step's keys, read while this one's MFMAs run)
 #pragma unroll
           for (int k = 0; k < BLOCKS / 2 + 1; ++k) {
-            const i32x8 keys = k < BLOCKS / 2 ? join(unit(2 * k), unit(2 * k + 1)) : join(unit(2 * k), unit(2 * k));
+            const i32x8 keys = coming;
+            if (k < BLOCKS / 2) {
+              const u32x4 lo = unit(2 * k + 2), hi = k + 1 < BLOCKS / 2 ? unit(2 * k + 3) : lo;
+              coming = join(lo, hi);
+              __builtin_amdgcn_sched_barrier(0);
+            }
             if (k < BLOCKS / 2) {
 #pragma unroll
               for (int c = 0; c < MT; ++c) s[c] = c ? mfma_16<2>(keys, q[c][2 * k], s[c], q_scale) : mfma_16<0>(keys, q[c][2 * k], s[c], q_scale);
