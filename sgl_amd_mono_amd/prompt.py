@@ -23,8 +23,9 @@ A call takes at most 1048576 rows (``experts``: tokens times (picks + 1), 116508
 8 picks) and 2^35 elements of them. Scratch: a product K * (1 + 1/32) bytes a row, and f32
 parts where its tiles are few; ``experts`` mostly 2 * H bytes for each token's every pick
 (1.2 GB for 8192 tokens of 7168 with 8 picks and the shared expert), so a long prompt goes
-through it in pieces of some thousand tokens; both attentions f32 parts, of up to 256 tokens or 1024
-nodes of 32 heads 512 or 1024 of [heads, 512] at most (34 or 67 MB). A captured graph keeps its calls' scratch.
+through it in pieces of some thousand tokens; both attentions f32 parts, for up to 256 tokens
+or 1024 nodes of 32 heads at most 512 or 1024 of [heads, 512] (34 or 67 MB). A captured graph
+keeps its calls' scratch.
 """
 
 from __future__ import annotations
@@ -265,9 +266,10 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: torc
 def index_query(x: torch.Tensor, pos: torch.Tensor, rope_cos: torch.Tensor,
                 rope_sin: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The FP4 index queries of tokens at ``pos`` (i32 [tokens]): ``x`` [tokens, 64 * 128] bf16
-    or f32 (rows may lie apart) is the projection before its rotation. Returns ``(iq, iqs)``, u8
-    [tokens, 64, 64] and [tokens, 64, 4], as ``attn.AttnStep`` and ``page_scores`` take them. A
-    token whose position has no row in ``rope_cos`` / ``rope_sin`` is a pad: zeros."""
+    or f32 (rows may lie apart, each 16-byte aligned) is the projection before its rotation.
+    Returns ``(iq, iqs)``, u8 [tokens, 64, 64] and [tokens, 64, 4], as ``attn.AttnStep`` and
+    ``page_scores`` take them. A token whose position has no row in ``rope_cos`` / ``rope_sin`` is
+    a pad: zeros."""
     dev = _gpu(x, "x")
     if x.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"x: expected dtype torch.bfloat16 or torch.float32, got {x.dtype}")
@@ -374,9 +376,11 @@ def _latents(q: torch.Tensor, caches: AttnCaches, out: torch.Tensor | None, dev:
         out = torch.empty(t, heads, KV_LORA, dtype=torch.bfloat16, device=dev)
     else:
         need(out, "out", (t, heads, KV_LORA), torch.bfloat16, dev)
-        a, b = q.data_ptr(), out.data_ptr()
-        if a < b + 2 * out.numel() and b < a + 2 * q.numel():
-            raise ValueError("out: shares memory with q")
+        b = out.data_ptr()
+        for name, v in (("q", q), ("kv", kv)):
+            a = v.data_ptr()
+            if a < b + 2 * out.numel() and b < a + v.element_size() * v.numel():
+                raise ValueError(f"out: shares memory with {name}")
     return slots // PAGE, out
 
 
@@ -392,7 +396,8 @@ def attention(q: torch.Tensor, req: torch.Tensor, pos: torch.Tensor, pages: torc
     pages] (all i32). A listed page outside the table or the pool is none, one that is listed
     twice counts twice. A token that sees no key has zeros. Keys that a token does not see may
     hold anything. An element of ``q`` is held to 2^-21.8 of its head's largest (2^-17.8 in the
-    last 64 dims), which is all of bf16 for those above 2^-14 (2^-10) of it. ``out`` must share no memory with ``q``."""
+    last 64 dims), which is all of bf16 for those above 2^-14 (2^-10) of it. ``out`` must share
+    no memory with ``q`` or the cache."""
     dev = _gpu(q, "q")
     n_pages, out = _latents(q, caches, out, dev)
     t, heads = q.shape[:2]
@@ -420,7 +425,8 @@ def tree_attention(q: torch.Tensor, starts: torch.Tensor, prefix: torch.Tensor, 
     (i32 [requests] and [requests + 1]); the key of its node i lies at position ``prefix[r]`` + i
     (``append`` with ``slot_pos``). A node sees the prefix and, for each bit j of its ``mask``
     (i64 [nodes]: the node itself and its ancestors), the key at ``prefix[r]`` + j. A node of no
-    request, and one that sees nothing, has zeros. ``out`` must share no memory with ``q``."""
+    request, and one that sees nothing, has zeros. ``out`` must share no memory with ``q`` or the
+    cache."""
     dev = _gpu(q, "q")
     n_pages, out = _latents(q, caches, out, dev)
     t, heads = q.shape[:2]

@@ -409,6 +409,9 @@ def test_attention_out_and_no_rows(gpu_device):
     with pytest.raises(ValueError, match="shares memory with q"):
         prompt.attention(buf[:4 * 32 * 576].view(4, 32, 576), req, pos, ids, table, c,
                          out=buf[4 * 32 * 576 - 8:4 * 32 * 1088 - 8].view(4, 32, 512))
+    with pytest.raises(ValueError, match="shares memory with kv"):
+        prompt.attention(q, req, pos, ids, table, AttnCaches(None, None, buf.view(torch.uint8)[:64 * 576].view(64, 576), None),
+                         out=buf[:4 * 32 * 512].view(4, 32, 512))
 
 
 @pytest.mark.parametrize("tokens,heads", [(8, 32), (9, 32), (31, 16), (32, 16), (33, 16), (256, 16), (257, 16), (512, 4), (513, 4), (65, 128)])
