@@ -30,7 +30,7 @@
 // Two workgroups a CU (80 KB of LDS, 256 registers a lane), a page of 32 heads in 1.2 us a CU:
 // 4096 tokens of 32 heads over 2048 keys 606 us, 950 TFLOP/s; a large bf16 product reaches 1180. Matrix
 // instructions (42 % of the cycles) and vector issue (53 %: the widening, the probabilities,
-// addresses), at a clock that power holds at 1.75 to 1.9 GHz, are what bounds it. Heads of up to 16 take one tile of 16 (2000 tokens 265 us,
+// addresses), at a clock that power holds at 1.75 to 1.9 GHz, are what bounds it. Heads of up to 16 take one tile of 16 (2000 tokens 234 us,
 // in a half-empty tile of 32 304), up to 32 two side by side (2000 tokens 314 us, as two workgroups
 // 516, which read the pages twice).
 #include "prompt_common.h"
@@ -41,8 +41,7 @@ namespace {
 
 constexpr int T = 256, WAVES = 4, ROW = LATENT + PE, PAGE_BYTES = PAGE * ROW;
 constexpr int BLOCKS = ROW / 64, BLOCK_BYTES = PAGE * 64;  // a page's rows in blocks of 64 dims
-constexpr int DT = LATENT / WAVES / 32;                   // tiles of 32 dims a wave
-constexpr int HEADS = 32;                                 // columns of the values' MFMAs
+constexpr int HEADS = 32;
 // NONE: no maximum yet, so low that any logit passes it (and finite: what is taken from it is a number)
 constexpr float NEG_INF = -__builtin_inff(), NONE = -1e38f, EXP2_SLACK = 16.0f;
 
@@ -96,8 +95,17 @@ template <int B>
 MONO_DEV f32x4 mfma_16(const i32x8& a, const i32x8& b, const f32x4& c, int scale) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 127, B, scale);
 }
-// C[32 x 32] += A[32 x 16] B[16 x 32] in bf16; lane l: row / column l % 32, k 8 (l / 32) .. + 7
-MONO_DEV f32x16 mfma_32(const bf16x8& a, const bf16x8& b, const f32x16& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+// The values' MFMAs, dims x keys against keys x heads in bf16, as wide as there are tiles of heads.
+// Of C[S x S] += A[S x K] B[K x S] lane l has row / column l % S, k 8 (l / S) .. + 7, and of C rows
+// 8 (i / 4) + 4 (l / S) + i % 4 of column l % S.
+MONO_DEV f32x16 values_mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+MONO_DEV f32x4 values_mfma(const bf16x8& a, const bf16x8& b, const f32x4& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+template <int MT>
+struct Values {
+  static constexpr int S = 16 * MT, K = 512 / S, R = S * S / WAVE;  // R: registers of C
+  static constexpr int TILES = LATENT / WAVES / S;                 // of dims, a wave
+  typedef float C __attribute__((ext_vector_type(R)));
+};
 MONO_DEV bf16x8 widen8(const u32x2& w) {
   bf16x8 v;
   widen4(w[0], v, 0);
@@ -332,14 +340,15 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
   const int64_t t = task.t;
   const int h0 = task.ht * 16 * MT;
   const bool any = task.any;
-  f32x16 o[DT];  // of lane l: dims 128 wave + 32 t + 8 (i / 4) + 4 (l / 32) + i % 4 of head l % 32
+  using V = Values<MT>;
+  typename V::C o[V::TILES];  // of lane l: dims 128 wave + S t + 8 (i / 4) + 4 (l / S) + i % 4 of head l % S
   float m_ref[MT], l_run[MT];
 #pragma unroll
   for (int c = 0; c < MT; ++c) m_ref[c] = NONE, l_run[c] = 0.f;
 #pragma unroll
-  for (int b = 0; b < DT; ++b)
+  for (int b = 0; b < V::TILES; ++b)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+    for (int i = 0; i < V::R; ++i) o[b][i] = 0.f;
   if (any) {
     int buf = 0;
     uint64_t live = 0;  // pages left of a run of 64 of the list
@@ -414,8 +423,6 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
       }
     }
     static_assert(2 * HEADS * ROW <= PAGE_BYTES, "q's pieces fit a page's place");
-    if (MT == 1 && wave == 3)  // columns that are no heads
-      for (int u = lane; u < 16 * P_PITCH / 8; u += WAVE) reinterpret_cast<u32x4*>(L.p[16])[u] = u32x4{0u, 0u, 0u, 0u};
     meet();
     // lane (g, r): of head 16 c + r units g of the blocks of 64 dims, two blocks an MFMA; of the last
     // block both pieces in one
@@ -552,29 +559,30 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
             if (wave == 0 && lane_now(lane) < 16) L.by[16 * c + lane_now(lane)] = by;
           }
           weigh();
-          const float by = L.by[lane_now(lane) % HEADS];
+          const float by = L.by[lane_now(lane) % V::S];
 #pragma unroll
-          for (int b = 0; b < DT; ++b)
+          for (int b = 0; b < V::TILES; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[b][i] *= by;
+            for (int i = 0; i < V::R; ++i) o[b][i] *= by;
         }
 #pragma unroll
         for (int c = 0; c < MT; ++c) l_run[c] += ps[c];
 
-        // the values, transposed and widened: 32 dims x 16 keys against 16 keys x 32 heads
+        // the values, transposed and widened: S dims x K keys against K keys x S heads
         {
-          const uint32_t ln = lane_now(lane), half = ln / 32;
-          const uint16_t* pr = &L.p[ln % 32][8 * half];
-          // lane l reads bytes of key 16 k + 8 half + l % 16 / 2 and gets one dim of the eight keys
-          const uint8_t* keys = &st.kv[2 * wave * BLOCK_BYTES + (8 * half + ln % 16 / 2) * 64 + 8 * (ln % 2)];
-          const uint32_t swap = unit_of(ln % 16 / 2, ln / 16 % 2);
-          constexpr int N = PAGE / 16 * DT, VAHEAD = 4;  // (tile i % DT of keys 16 (i / DT) ..)
+          const uint32_t ln = lane_now(lane), group = ln / V::S;
+          const uint16_t* pr = &L.p[ln % V::S][8 * group];
+          // lane l reads bytes of key K k + 8 group + l % 16 / 2 and gets one dim of the eight keys
+          const uint8_t* keys = &st.kv[2 * wave * BLOCK_BYTES + (8 * group + ln % 16 / 2) * 64 + 8 * (ln % 2)];
+          const uint32_t swap = unit_of(ln % 16 / 2, ln / 16 % MT);
+          constexpr int N = PAGE / V::K * V::TILES, VAHEAD = 4;  // (tile i % TILES of keys K (i / TILES) ..)
           u32x2 w[VAHEAD];
           bf16x8 pk[2];
           const auto read = [&](int i) {
-            w[i % VAHEAD] = lds_transposed(keys + i % DT / 2 * BLOCK_BYTES + 16 * (swap ^ 2 * (i % 2)) + 1024 * (i / DT));
+            const int unit = i % V::TILES * MT;  // of 16 dims, four a block
+            w[i % VAHEAD] = lds_transposed(keys + unit / 4 * BLOCK_BYTES + 16 * (swap ^ unit % 4) + i / V::TILES * V::K * 64);
           };
-          const auto read_p = [&](int k) { pk[k % 2] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(pr + 16 * k)); };
+          const auto read_p = [&](int k) { pk[k % 2] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(pr + V::K * k)); };
           read_p(0);
 #pragma unroll
           for (int i = 0; i < VAHEAD; ++i) read(i);
@@ -584,10 +592,10 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
           const int after_slot = L.slot[after_i];
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            if (i % DT == 0 && i + DT < N) read_p(i / DT + 1);
+            if (i % V::TILES == 0 && i + V::TILES < N) read_p(i / V::TILES + 1);
             const bf16x8 v = widen8(w[i % VAHEAD]);
             if (i + VAHEAD < N) read(i + VAHEAD);
-            o[i % DT] = mfma_32(v, pk[i / DT % 2], o[i % DT]);
+            o[i % V::TILES] = values_mfma(v, pk[i / V::TILES % 2], o[i % V::TILES]);
             __builtin_amdgcn_sched_barrier(0);
           }
           mask = seen_at(next_seen);
@@ -613,7 +621,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
   __syncthreads();
   const auto sum_of = [&](int head) { return (L.top[0][head] + L.top[1][head]) + (L.top[2][head] + L.top[3][head]); };
   // the outputs through LDS, so that rows go out whole
-  const int head = ln % HEADS, dim0 = 128 * wave + 4 * (ln / HEADS);
+  const int head = ln % V::S, dim0 = 128 * wave + 4 * (ln / V::S);
   if (task.chunks > 1) {
     const int64_t first = task.part * a.heads + h0;  // this chunk's rows of the parts
     if (tid < heads) {
@@ -626,10 +634,10 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
     constexpr int PITCH = LATENT + 4;
     static_assert(HEADS * PITCH * 4 <= sizeof L.stage, "the parts fit the pages' places");
 #pragma unroll
-    for (int b = 0; b < DT; ++b)
+    for (int b = 0; b < V::TILES; ++b)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4*>(stage + head * PITCH + dim0 + 32 * b + 8 * i) = f32x4{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]};
+      for (int i = 0; i < V::R / 4; ++i)
+        *reinterpret_cast<f32x4*>(stage + head * PITCH + dim0 + V::S * b + 8 * i) = f32x4{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]};
     __syncthreads();
     float* part = a.part + first * LATENT;
     for (int u = tid; u < heads * (LATENT / 4); u += T)
@@ -638,12 +646,12 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
   }
   uint16_t* stage = reinterpret_cast<uint16_t*>(&L.stage);
   constexpr int PITCH = LATENT + 8;
-  const float l = sum_of(head < 16 * MT ? head : 0), inv = l == 0.f ? 0.f : 1.0f / l;
+  const float l = sum_of(head), inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-  for (int b = 0; b < DT; ++b)
+  for (int b = 0; b < V::TILES; ++b)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<u32x2*>(stage + head * PITCH + dim0 + 32 * b + 8 * i) =
+    for (int i = 0; i < V::R / 4; ++i)
+      *reinterpret_cast<u32x2*>(stage + head * PITCH + dim0 + V::S * b + 8 * i) =
           u32x2{pack2(o[b][4 * i] * inv, o[b][4 * i + 1] * inv), pack2(o[b][4 * i + 2] * inv, o[b][4 * i + 3] * inv)};
   __syncthreads();
   uint16_t* out = static_cast<uint16_t*>(a.out) + (t * a.heads + h0) * LATENT;
