@@ -31,7 +31,7 @@
 // 4096 tokens of 32 heads over 2048 keys 606 to 632 us, 910 to 950 TFLOP/s; a large bf16 product reaches
 // 1180. Matrix instructions (42 % of the cycles) and vector issue (53 %: the widening, the
 // probabilities, addresses), at a clock that power holds at 1.75 to 1.9 GHz, are what bounds it.
-// Heads of up to 16 take one tile of 16 (2000 tokens 234 us, in a half-empty pair of them 304), up
+// Heads of up to 16 take one tile of 16 (2000 tokens 224 us, in a half-empty pair of them 304), up
 // to 32 two side by side (2000 tokens 314 us, as two workgroups 516, which read the pages twice).
 #include "prompt_common.h"
 
@@ -337,6 +337,8 @@ MONO_DEV void task_of(const Paged& a, int lane, int64_t id, Task& k, Reads& rd) 
 
 template <int MT, bool TREE>
 MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& task, const Reads& rd) {
+  // (one tile of heads leaves registers to hold addresses in: 2000 tokens 237 -> 224 us)
+  const auto here = [&]() { return MT == 1 ? (uint32_t)lane : lane_now(lane); };
   const int64_t t = task.t;
   const int h0 = task.ht * 16 * MT;
   const bool any = task.any;
@@ -355,14 +357,14 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
     // page i's way to LDS: this wave's 16 keys, a block of dims at a time, and the scales
     const auto place_of = [&](int i) { return (int64_t)__builtin_amdgcn_readfirstlane(L.slot[i]) * PAGE; };
     const auto lane_place = [&]() {
-      const uint32_t ln = lane_now(lane);
+      const uint32_t ln = here();
       return ln / 4 * ROW + 16 * unit_of(ln / 4, ln % 4);
     };
     const auto bring = [&](int64_t first, uint32_t at, Stage& to, int b, bool go) {
       dma16(static_cast<const uint8_t*>(a.kv) + (first + 16 * wave) * ROW + 64 * b, at, &to.kv[b * BLOCK_BYTES + wave * 1024], go);
     };
     const auto bring_scales = [&](int64_t first, Stage& to) {
-      if (wave == 0 && a.kv_scale) dma4(a.kv_scale + first, 4 * lane_now(lane), to.scale);
+      if (wave == 0 && a.kv_scale) dma4(a.kv_scale + first, 4 * here(), to.scale);
     };
     const auto run_from = [&](int at) {  // the run that begins at page `at` of the list, and its first page on its way
       int page = -1, slot = -1;
@@ -388,7 +390,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
     // q's heads as two pieces (behind the first page, which more steps led to): wave w's eight
     // heads, 8 lanes each, through LDS to all the waves
     if (wave < 2 * MT) {
-      const uint32_t ln = lane_now(lane), head = 8 * wave + ln / 8;
+      const uint32_t ln = here(), head = 8 * wave + ln / 8;
       const uint16_t* row = static_cast<const uint16_t*>(a.q) + (t * a.heads + min(h0 + (int)head, a.heads - 1)) * ROW + 8 * (ln % 8);
       u32x4 v[BLOCKS];
       uint32_t most = 0;
@@ -429,7 +431,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
     i32x8 q[MT][BLOCKS];  // pieces of blocks 0 and 1, 2 and 3, ..; then the last
     int q_scale = 0;
     {
-      const uint32_t ln = lane_now(lane), r = ln % 16, g = ln / 16;
+      const uint32_t ln = here(), r = ln % 16, g = ln / 16;
 #pragma unroll
       for (int c = 0; c < MT; ++c) {
         const uint8_t* row = &L.stage[1].kv[(16 * c + r) * ROW + 16 * unit_of(r, g)];
@@ -461,7 +463,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
         meet_after_loads();  // the page has come, and every wave is done with the one before
         const bool partial = mask != ~0ull, more = live != 0;
         if (partial) {  // what is not seen may hold anything, a NaN too: zeros instead
-          const uint32_t ln = lane_now(lane);
+          const uint32_t ln = here();
           if (!(mask >> (16 * wave + ln / 4) & 1)) {
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) *reinterpret_cast<u32x4*>(&st.kv[b * BLOCK_BYTES + 1024 * wave + 16 * ln]) = u32x4{0u, 0u, 0u, 0u};
@@ -474,7 +476,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
 #pragma unroll
         for (int c = 0; c < MT; ++c) s[c] = f32x4{0.f, 0.f, 0.f, 0.f};
         {
-          const uint32_t ln = lane_now(lane), at_lane = lane_place();
+          const uint32_t ln = here(), at_lane = lane_place();
           const uint8_t* key = &st.kv[(16 * wave + ln % 16) * 64 + 16 * unit_of(ln % 16, ln / 16)];
           const auto unit = [&](int b) { return *reinterpret_cast<const u32x4*>(key + BLOCK_BYTES * b); };
           i32x8 coming = join(unit(0), unit(1));  // (the next step's keys, read while this one's MFMAs run)
@@ -504,7 +506,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
 #pragma unroll
         for (int c = 0; c < MT; ++c) asm volatile("" : "+v"(s[c]));  // (formed here, not where they are used)
         // lane (g, r): keys 16 wave + 4 g + j of head 16 c + r
-        const uint32_t first_key = 16 * wave + lane_now(lane) / 16 * 4;
+        const uint32_t first_key = 16 * wave + here() / 16 * 4;
         f32x4 ks = {1.f, 1.f, 1.f, 1.f}, by;
         if (a.kv_scale) ks = *reinterpret_cast<const f32x4*>(&st.scale[first_key]);
 #pragma unroll
@@ -520,7 +522,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
         }
         float ps[MT];
         const auto weigh = [&]() {  // the probabilities to LDS, and whether one of the workgroup's is over EXP2_SLACK
-          const uint32_t ln = lane_now(lane);
+          const uint32_t ln = here();
           uint16_t* to = &L.p[ln % 16][16 * wave + ln / 16 * 4];
           float top = 0.f;
 #pragma unroll
@@ -545,21 +547,21 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
 #pragma unroll
             for (int j = 0; j < 4; ++j) m = fmaxf(m, s[c][j] * by[j]);
             m = groups_max(m);
-            if (lane_now(lane) < 16) L.top[wave][16 * c + lane_now(lane)] = m;
+            if (here() < 16) L.top[wave][16 * c + here()] = m;
           }
           meet();
 #pragma unroll
           for (int c = 0; c < MT; ++c) {
             float m = m_ref[c];
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) m = fmaxf(m, L.top[w][16 * c + lane_now(lane) % 16]);
+            for (int w = 0; w < WAVES; ++w) m = fmaxf(m, L.top[w][16 * c + here() % 16]);
             const float by = __builtin_amdgcn_exp2f(m_ref[c] - m);
             m_ref[c] = m;
             l_run[c] *= by;
-            if (wave == 0 && lane_now(lane) < 16) L.by[16 * c + lane_now(lane)] = by;
+            if (wave == 0 && here() < 16) L.by[16 * c + here()] = by;
           }
           weigh();
-          const float by = L.by[lane_now(lane) % V::S];
+          const float by = L.by[here() % V::S];
 #pragma unroll
           for (int b = 0; b < V::TILES; ++b)
 #pragma unroll
@@ -570,7 +572,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
 
         // the values, transposed and widened: S dims x K keys against K keys x S heads
         {
-          const uint32_t ln = lane_now(lane), group = ln / V::S;
+          const uint32_t ln = here(), group = ln / V::S;
           const uint16_t* pr = &L.p[ln % V::S][8 * group];
           // lane l reads bytes of key K k + 8 group + l % 16 / 2 and gets one dim of the eight keys
           const uint8_t* keys = &st.kv[2 * wave * BLOCK_BYTES + (8 * group + ln % 16 / 2) * 64 + 8 * (ln % 2)];
@@ -610,7 +612,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
   }
 
   // the heads' sums: over the lane groups, then the waves
-  const int tid = wave * WAVE + (int)lane_now(lane), ln = tid % WAVE, heads = min(16 * MT, a.heads - h0);
+  const int tid = wave * WAVE + (int)here(), ln = tid % WAVE, heads = min(16 * MT, a.heads - h0);
   __syncthreads();  // (the last page's readers)
 #pragma unroll
   for (int c = 0; c < MT; ++c) {
