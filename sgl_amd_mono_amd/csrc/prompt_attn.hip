@@ -444,6 +444,21 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
         q_scale |= (int)(L.q_scale[16 * c + r] << 16 * c);
       }
     }
+    // The lane's places that every page uses, held across pages: in a page's DMA, its keys for q . c and
+    // as values (the unit's swap apart), and in the probabilities as they are written and read. No more
+    // registers are left with two tiles of heads (32 trees of 32 nodes 597 -> 572 us).
+    uint32_t dma_place, key_place, value_place, value_swap, to_place, from_place;
+    {
+      const uint32_t ln = here(), group = ln / V::S, row = ln % 16 / 2;
+      dma_place = lane_place();
+      key_place = (16 * wave + ln % 16) * 64 + 16 * unit_of(ln % 16, ln / 16);
+      // (lane l reads bytes of key 8 group + l % 16 / 2 and gets one dim of the eight keys)
+      value_place = 2 * wave * BLOCK_BYTES + (8 * group + row) * 64 + 8 * (ln % 2);
+      value_swap = 16 * unit_of(row, ln / 16 % MT);
+      to_place = ln % 16 * P_PITCH + 16 * wave + ln / 16 * 4;
+      from_place = ln % V::S * P_PITCH + 8 * group;
+      asm volatile("" : "+v"(dma_place), "+v"(key_place), "+v"(value_place), "+v"(value_swap), "+v"(to_place), "+v"(from_place));
+    }
     for (;;) {
       // of the page that comes first, which keys are seen; where the one after it lies
       uint64_t mask = 0;
@@ -476,8 +491,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
 #pragma unroll
         for (int c = 0; c < MT; ++c) s[c] = f32x4{0.f, 0.f, 0.f, 0.f};
         {
-          const uint32_t ln = here(), at_lane = lane_place();
-          const uint8_t* key = &st.kv[(16 * wave + ln % 16) * 64 + 16 * unit_of(ln % 16, ln / 16)];
+          const uint8_t* key = &st.kv[key_place];
           const auto unit = [&](int b) { return *reinterpret_cast<const u32x4*>(key + BLOCK_BYTES * b); };
           i32x8 coming = join(unit(0), unit(1));  // (the next step's keys, read while this one's MFMAs run)
 #pragma unroll
@@ -491,14 +505,14 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
             if (k < BLOCKS / 2) {
 #pragma unroll
               for (int c = 0; c < MT; ++c) s[c] = c ? mfma_16<2>(keys, q[c][2 * k], s[c], q_scale) : mfma_16<0>(keys, q[c][2 * k], s[c], q_scale);
-              bring(ahead, at_lane, next, 2 * k, more);  // (nine DMAs at once hold the wave up for 1000 cycles)
+              bring(ahead, dma_place, next, 2 * k, more);  // (nine DMAs at once hold the wave up for 1000 cycles)
 #pragma unroll
               for (int c = 0; c < MT; ++c) s[c] = c ? mfma_16<3>(keys, q[c][2 * k + 1], s[c], q_scale) : mfma_16<1>(keys, q[c][2 * k + 1], s[c], q_scale);
-              bring(ahead, at_lane, next, 2 * k + 1, more);
+              bring(ahead, dma_place, next, 2 * k + 1, more);
             } else {
 #pragma unroll
               for (int c = 0; c < MT; ++c) s[c] = c ? mfma_16<2>(keys, q[c][2 * k], s[c], q_scale) : mfma_16<0>(keys, q[c][2 * k], s[c], q_scale);
-              bring(ahead, at_lane, next, 2 * k, more);
+              bring(ahead, dma_place, next, 2 * k, more);
             }
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -522,8 +536,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
         }
         float ps[MT];
         const auto weigh = [&]() {  // the probabilities to LDS, and whether one of the workgroup's is over EXP2_SLACK
-          const uint32_t ln = here();
-          uint16_t* to = &L.p[ln % 16][16 * wave + ln / 16 * 4];
+          uint16_t* to = &L.p[0][to_place];
           float top = 0.f;
 #pragma unroll
           for (int c = 0; c < MT; ++c) {
@@ -572,17 +585,14 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
 
         // the values, transposed and widened: S dims x K keys against K keys x S heads
         {
-          const uint32_t ln = here(), group = ln / V::S;
-          const uint16_t* pr = &L.p[ln % V::S][8 * group];
-          // lane l reads bytes of key K k + 8 group + l % 16 / 2 and gets one dim of the eight keys
-          const uint8_t* keys = &st.kv[2 * wave * BLOCK_BYTES + (8 * group + ln % 16 / 2) * 64 + 8 * (ln % 2)];
-          const uint32_t swap = unit_of(ln % 16 / 2, ln / 16 % MT);
-          constexpr int N = PAGE / V::K * V::TILES, VAHEAD = 4;  // (tile i % TILES of keys K (i / TILES) ..)
+          const uint16_t* pr = &L.p[0][from_place];
+          const uint8_t* keys = &st.kv[value_place];
+                    constexpr int N = PAGE / V::K * V::TILES, VAHEAD = 4;  // (tile i % TILES of keys K (i / TILES) ..)
           u32x2 w[VAHEAD];
           bf16x8 pk[2];
           const auto read = [&](int i) {
             const int unit = i % V::TILES * MT;  // of 16 dims, four a block
-            w[i % VAHEAD] = lds_transposed(keys + unit / 4 * BLOCK_BYTES + 16 * (swap ^ unit % 4) + i / V::TILES * V::K * 64);
+            w[i % VAHEAD] = lds_transposed(keys + unit / 4 * BLOCK_BYTES + (value_swap ^ unit % 4 * 16) + i / V::TILES * V::K * 64);
           };
           const auto read_p = [&](int k) { pk[k % 2] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(pr + V::K * k)); };
           read_p(0);
