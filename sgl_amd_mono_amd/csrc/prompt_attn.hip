@@ -27,9 +27,9 @@
 // sums does not depend on it, and bf16 and f32 hold 2^4 as well as 1): the waves' maxima then meet
 // and the sums are scaled, which happens on a token's first page and rarely after it.
 //
-// Two workgroups a CU (80 KB of LDS, 256 registers a lane), a page of 32 heads in 1.2 us a CU:
-// 4096 tokens of 32 heads over 2048 keys 606 to 632 us, 910 to 950 TFLOP/s; a large bf16 product reaches
-// 1180. Matrix instructions (42 % of the cycles) and vector issue (53 %: the widening, the
+// Two workgroups a CU (80 KB of LDS, 256 registers a lane), a page of 32 heads in 1.15 us a CU:
+// 4096 tokens of 32 heads over 2048 keys 596 to 606 us, 950 to 965 TFLOP/s; a large bf16 product reaches
+// 1180. Matrix instructions (44 % of the cycles) and vector issue (50 %: the widening, the
 // probabilities, addresses), at a clock that power holds at 1.75 to 1.9 GHz, are what bounds it.
 // Heads of up to 16 take one tile of 16 (2000 tokens 224 us, in a half-empty pair of them 304), up
 // to 32 two side by side (2000 tokens 314 us, as two workgroups 516, which read the pages twice).
