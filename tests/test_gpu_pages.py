@@ -414,7 +414,7 @@ def test_attention_out_and_no_rows(gpu_device):
                          out=buf[:4 * 32 * 512].view(4, 32, 512))
 
 
-@pytest.mark.parametrize("tokens,heads", [(8, 32), (9, 32), (31, 16), (32, 16), (33, 16), (256, 16), (257, 16), (512, 4), (513, 4), (65, 128)])
+@pytest.mark.parametrize("tokens,heads", [(8, 32), (9, 32), (51, 32), (52, 32), (12, 128), (13, 128), (31, 16), (32, 16), (33, 16), (256, 16), (257, 16), (512, 4), (513, 4), (65, 128)])
 def test_attention_shared_out_or_not(gpu_device, tokens, heads):
     """Around the token counts at which pages are shared out, or joined, in another way."""
     req, pos, table, pages = _requests(gpu_device, [(400, tokens)])
@@ -493,6 +493,7 @@ def test_tree_attention_wide(gpu_device):
 @pytest.mark.parametrize("trees,heads", [
     ([(100 + i, 32) for i in range(8)], 16), ([(100 + i, 32) for i in range(8)] + [(500, 1)], 16),  # 256 nodes, 257
     ([(90, 30), (300, 34)], 128), ([(90, 30), (300, 35)], 128),  # 256 nodes' tiles of heads, 260
+    ([(30 * PAGE, 8)], 32), ([(31 * PAGE, 8)], 32), ([(7, 3)], 100), ([(300, 9)], 33),  # 512 nodes' pages and tiles, 528
     ([(255 * PAGE, 8)], 16), ([(255 * PAGE + 1, 8)], 16),  # 2048 nodes' pages, 2056
     ([(50 * PAGE, 16)], 16), ([(50 * PAGE, 17)], 16),  # 256 heads, 272
     ([(9, 64), (700, 64)], 16), ([(9, 64), (700, 65)], 16),  # 128 nodes, 129
