@@ -7,6 +7,7 @@
 // spends: a compare a score, a ballot and a scalar sum each, some ten of them (bit by bit from the
 // top eighteen). 8192 rows of 512 columns: 11.3 us, 9 rows 4.3 us.
 #include "prompt_common.h"
+#include "prompt_search.h"
 
 namespace mono {
 namespace prompt {
@@ -100,16 +101,10 @@ __global__ __launch_bounds__(256) void k_select(mono_prompt_select_args a) {
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) most = max(most, key[i]);
-    uint32_t hi = row_waves.most(wave_umax(most));
+    const uint32_t hi = row_waves.most(wave_umax(most));
     top = row_waves.most(need <= WAVE ? ~wave_umax(~most) : 0u);
-    int kept = 0;  // keys that are at least `top` (0: not counted)
-#pragma unroll 1
-    while (top < hi && kept != need) {
-      const uint32_t mid = top + (hi - top + 1) / 2;
-      const int m = count([&](uint32_t k) { return k >= mid; });
-      if (m >= need) top = mid, kept = m;
-      else hi = mid - 1;
-    }
+    int kept;
+    top = largest_kept_by(need, top, hi, kept, [&](uint32_t mid) { return count([&](uint32_t k) { return k >= mid; }); });
     if (kept != need) border = need - count([&](uint32_t k) { return k > top; });
   }
   int ties_before = 0, taken_before = 0;

@@ -205,6 +205,26 @@ def test_select_pages(gpu_device, columns):
             assert torch.equal(got.cpu(), ref.select_pages(scores[:, 3:], pos, picks, first, last)), (values, picks, first, last)
 
 
+@pytest.mark.parametrize("columns", [2, 40, 64, 100, 128, 300, 1000, 2048, 2049, 8192])
+def test_select_pages_scores_of_any_bits(gpu_device, columns):
+    """NaNs of the largest and the smallest bits of either sign among scores, and rows of them alone:
+    where the search begins, at either end of 32 bits."""
+    g = torch.Generator().manual_seed(columns)
+    t = 9
+    pos = torch.randint(0, columns * PAGE, (t,), generator=g).int()
+    pos[0], pos[1] = columns * PAGE - 1, columns * PAGE // 2
+    scores = torch.randn(t, columns, generator=g)
+    bits = scores.view(torch.int32)
+    odd = torch.tensor([0x7FFFFFFF, 0x7F800001, -1, -0x7FFFFF, 0x7FFFFFFE, -2, 0x7F7FFFFF, -0x800001], dtype=torch.int32)
+    place = torch.rand(t, columns, generator=g)
+    bits[2:] = torch.where(place < 0.5, odd[torch.randint(0, len(odd), (t, columns), generator=g)], bits)[2:]
+    bits[0, columns // 3] = bits[1, 0] = 0x7FFFFFFF  # one alone
+    bits[2], bits[3] = 0x7FFFFFFF, -1  # a row of each
+    for picks, first, last in ((1, 0, 0), (2, 0, 1), (31, 0, 1), (64, 0, 1), (70, 1, 2), (columns, 0, 0), (max(columns - 1, 1), 0, 1)):
+        got = prompt.select_pages(scores.to(gpu_device), pos.to(gpu_device), picks, first, last)
+        assert torch.equal(got.cpu(), ref.select_pages(scores, pos, picks, first, last)), (picks, first, last)
+
+
 def test_select_pages_default_takes_all_of_2048_keys(gpu_device):
     pos = torch.tensor([0, 64, 2047, 2048], dtype=torch.int32, device=gpu_device)
     got = prompt.select_pages(torch.randn(4, 40, device=gpu_device), pos).cpu()
