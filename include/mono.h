@@ -610,8 +610,11 @@ int mono_prompt_query(const mono_prompt_query_args* args, void* stream);
 
 /* out[t, p] = the largest over the keys j of page p of token t's request at positions
  * <= pos[t] of sum_h iw[t, h] max(0, q[t, h] . k[j]): mono_attn_forward's index scores, by
- * page. -infinity where the token sees no key of the page (behind its position, a page outside
- * the table or the pool, a pad: req outside [0, requests) or pos < 0); NaN where a key's is. */
+ * page, but for a product that is NaN: it makes the page's score NaN, where that launch takes it
+ * for 0. -infinity where the token sees no key of the page (behind its position, a page outside
+ * the table or the pool, a pad: req outside [0, requests) or pos < 0). Products and sums are f32
+ * (past its range infinite); a score is off by 12 roundings, 2^-24 each, of sum_h |iw (q . k)| at
+ * most, of the heads too that the maximum cuts off. */
 typedef struct {
   const void* iq;            /* u8 [tokens, 64, 64], 16-byte aligned */
   const void* iqs;           /* u8 [tokens, 64, 4] */

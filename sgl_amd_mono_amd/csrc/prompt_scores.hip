@@ -12,7 +12,8 @@
 //
 // FP4 products and their sum are exact in f32 where a query's and a key's scales lie close; the weighted sum is
 // f32 throughout. As x / 2 + |x| / 2 a head's ReLU leaves a rounding of the size of a product that it
-// cuts off, 2^-24 of it.
+// cuts off, 2^-24 of it. A page with a score that is not finite is formed again with the ReLU as a
+// maximum: one half may leave f32's range where their sum does not (the test for it: 2 us of 208).
 #include <algorithm>
 
 #include "prompt_common.h"
@@ -87,6 +88,24 @@ MONO_DEV float key_scores(const Query& q, const Keys& k) {
   return swap_halves(s[0], s[1], OpAdd());
 }
 
+// The same with the ReLU formed before the weight, a maximum and an FMA a value: where a sum of the two
+// halves left f32's range, or met an infinity of either sign in it, this one need not (and a NaN
+// that is left is one of the definition's). The weights are twice their halves, exactly.
+MONO_DEV float cut_off(const float (&halves)[16], const f32x16& d) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s = fmaf(2.0f * halves[i], __builtin_elementwise_maximum(d[i], 0.f), s);
+  return s;
+}
+MONO_DEV float key_scores_cut_off(const Query& q, const Keys& k) {
+  float s[KT];
+  s[0] = cut_off(q.halves[0], dots<0, 0>(q, k));
+  s[0] += cut_off(q.halves[1], dots<1, 0>(q, k));
+  s[1] = cut_off(q.halves[0], dots<0, 1>(q, k));
+  s[1] += cut_off(q.halves[1], dots<1, 1>(q, k));
+  return swap_halves(s[0], s[1], OpAdd());
+}
+
 __global__ __launch_bounds__(WAVES * WAVE, 4) void k_scores(mono_prompt_scores_args a, int run) {
   const int lane = threadIdx.x % WAVE, half = lane / 32, r = lane % 32;
   // the workgroup's waves take neighbouring tokens over the same pages, which the CU's cache then holds
@@ -133,12 +152,23 @@ __global__ __launch_bounds__(WAVES * WAVE, 4) void k_scores(mono_prompt_scores_a
         for (int e = 0; e < 4; ++e) q.halves[h][4 * i + e] = 0.5f * (e & 1 ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2]));
       }
     }
+    uint64_t again = 0;  // pages with a score that is not finite
     while (live) {
       const int p = __builtin_ctzll(live);
       live &= live - 1;
       k = next;
       load(live ? __builtin_ctzll(live) : p, next);
       const float key = key_scores(q, k);
+      const bool mine = lane < seen - PAGE * p;
+      if (__any(mine && !__builtin_isfinite(key))) again |= 1ull << p;
+      const float top = wave_reduce(mine ? key : NEG_INF, OpNanMax());
+      best = lane == p ? top : best;
+    }
+    while (again) {  // (by itself, so that the loop above holds no more registers: it has none to spare)
+      const int p = __builtin_ctzll(again);
+      again &= again - 1;
+      load(p, k);
+      const float key = key_scores_cut_off(q, k);
       const float top = wave_reduce(lane < seen - PAGE * p ? key : NEG_INF, OpNanMax());
       best = lane == p ? top : best;
     }

@@ -312,8 +312,9 @@ def page_scores(iq: torch.Tensor, iqs: torch.Tensor, iw: torch.Tensor, req: torc
     .. ``columns`` - 1 of its request (default: all that ``page_table`` [requests, pages] has;
     at most 8192). ``iq`` / ``iqs`` are the tokens' index queries (``index_query``), ``iw`` bf16
     [tokens, 64] their head weights; token i is position ``pos[i]`` of request ``req[i]`` (i32),
-    and a key's score the decode launches' index score. -infinity where the token sees no key
-    of the page, NaN where the score of one is."""
+    and a key's score the decode launches' index score, summed in f32: off by 12 roundings at most,
+    2^-24 each, of the sum of all heads' |weight x product|. -infinity where the token sees no key
+    of the page, NaN where the score of one is (a NaN product, which the decode launches take for 0)."""
     dev = _gpu(iq, "iq")
     t = iq.shape[0] if iq.dim() == 3 else -1
     need(iq, "iq", (t, INDEX_HEADS, INDEX_DIM // 2), torch.uint8, dev)

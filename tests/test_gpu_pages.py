@@ -162,6 +162,37 @@ def test_page_scores_bad_pages_requests_and_values(gpu_device):
     assert bool((got[12:, 1:] == -torch.inf).all())
 
 
+@pytest.mark.parametrize("tokens", [1, 5, 300])
+def test_page_scores_of_heads_below_f32_s_range(gpu_device, tokens):
+    """A head whose product, or weight times product, is below zero adds nothing however far below it is:
+    minus infinity, too. A sum of the other heads' in f32: 16 FMAs a lane, a sum of two tiles' and one of
+    two lanes', 18 roundings of what is not cut off."""
+    req, pos, table, pages = _requests(gpu_device, [(140, tokens)])
+    iq, iqs, iw, caches = _index(gpu_device, tokens, pages)
+    caches.ikv[int(table[0, 1])] = 0xAA  # a page's keys: every dim -1 x 2^127
+    caches.iks[int(table[0, 1])] = 254
+    iqs[:] = 2  # the heads beside: 2^-125 of their codes
+    iqs[:, 3] = iqs[:, 40] = 254  # 128 x -2^254
+    iqs[:, 8:11] = 120  # 128 x -2^120 = -2^127, which a weight of 16 takes out of the range
+    iq[:, [3, 40, 8, 9, 10]] = 0x22
+    iw[:, 8], iw[:, 9], iw[:, 10] = 16.0, -16.0, 1.5
+    got = prompt.page_scores(iq, iqs, iw, req, pos, table, caches).cpu().double()
+    keep = sorted({0, tokens // 2, tokens - 1})
+    cpu = (v[keep].cpu() for v in (iq, iqs, iw, req, pos))
+    want, _ = ref.page_scores(*cpu, table.cpu(), caches.ikv.cpu(), caches.iks.cpu(), table.shape[1])
+    for n, at in enumerate(keep):
+        dot = -ref.oatt.index_query(iq[at].cpu(), iqs[at].cpu()).double().sum(-1) * 2.0**127
+        mag = float((iw[at].cpu().double().abs() * dot.clamp_min(0)).sum())
+        assert abs(float(got[at, 1] - want[n, 1])) <= 18 * 2.0**-24 * mag and mag > 0
+    # upwards: infinite, of the weight's sign; and with both a NaN
+    caches.ikv[int(table[0, 1])] = 0x22
+    for weights, what in (((1.0, 2.0), torch.inf), ((-1.0, -2.0), -torch.inf), ((1.0, -2.0), torch.nan)):
+        iw[:, 3], iw[:, 40] = weights
+        iw[:, 8:11] = 1e-3
+        got = prompt.page_scores(iq, iqs, iw, req, pos, table, caches)[:, 1].cpu()
+        assert torch.equal(got, torch.full((tokens,), what)) or (what != what and bool(got.isnan().all()))
+
+
 def test_page_scores_are_the_decode_launch_s(gpu_device):
     """The largest in each page of the index scores that the attention launch computes: the same
     products, 64 heads' sums in another order at most."""
