@@ -378,9 +378,9 @@ def _latents(q: torch.Tensor, caches: AttnCaches, out: torch.Tensor | None, dev:
     else:
         need(out, "out", (t, heads, KV_LORA), torch.bfloat16, dev)
         b = out.data_ptr()
-        for name, v in (("q", q), ("kv", kv)):
-            a = v.data_ptr()
-            if a < b + 2 * out.numel() and b < a + v.element_size() * v.numel():
+        for name, v in (("q", q), ("kv", kv), ("kv_scale", caches.kv_scale)):
+            a = 0 if v is None else v.data_ptr()
+            if a and a < b + 2 * out.numel() and b < a + v.element_size() * v.numel():
                 raise ValueError(f"out: shares memory with {name}")
     return slots // PAGE, out
 

@@ -173,6 +173,22 @@ def test_cpu_and_misshapen_tensors_are_refused(monkeypatch):
     refused("mask", prompt.tree_attention, q, at, at[:1], at, table, c)
 
 
+def test_out_over_the_cache_s_scales_is_refused(monkeypatch):
+    monkeypatch.setattr(prompt, "_gpu", lambda t, name: t.device)  # the checks alone, on CPU tensors
+    at, table, mask = torch.zeros(2, dtype=torch.int32), torch.zeros(1, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int64)
+    q, kv = torch.zeros(2, 4, 576, dtype=torch.bfloat16), torch.zeros(64 * 64, 576, dtype=torch.uint8)
+    buf = torch.zeros(4096 + 2048)  # 4096 scales, and behind them as much as an out takes
+    c = AttnCaches(None, None, kv, buf[:4096])
+    out = buf.view(torch.bfloat16)
+    for first in (0, 4096, 8192 - 8):  # the first scales, some in the middle, the last four
+        o = out[first:first + 2 * 4 * 512].view(2, 4, 512)
+        with pytest.raises(ValueError, match="out: shares memory with kv_scale"):
+            prompt.attention(q, at, at, at.view(2, 1), table, c, out=o)
+        with pytest.raises(ValueError, match="out: shares memory with kv_scale"):
+            prompt.tree_attention(q, torch.zeros(2, dtype=torch.int32), at[:1], mask, table, c, out=o)
+    assert prompt._latents(q, c, out[8192:].view(2, 4, 512), q.device)[0] == 64  # right behind them: nothing shared
+
+
 def test_the_restated_queries_and_scores_are_the_decode_oracle_s():
     torch.manual_seed(5)
     cos, sin = olayer.rope_tables(9)
