@@ -208,8 +208,9 @@ MONO_DEV void node_reads(const Paged& a, int64_t t, int req, Reads& rd) {
   rd.draft = (uint64_t)a.mask[t];
 }
 
-// A request's nodes and pages (the last one or two hold the draft's keys; MOST_PAGES: more than the
-// card's memory holds).
+// A request's nodes and pages (the last one or two hold the draft's keys, the last one perhaps none and
+// then, perhaps, behind the table: how pages are shared out hangs on the prefix alone and not on how wide
+// the table is. MOST_PAGES: more than the card's memory holds).
 constexpr int MOST_PAGES = 1 << 23;
 struct Request {
   int64_t first;
@@ -221,7 +222,7 @@ MONO_DEV Request request_of(const Paged& a, int r) {
   Request q;
   q.first = min((int64_t)max(from, 0), a.tokens);
   q.n = r < a.requests ? (int)max(min((int64_t)to, a.tokens) - q.first, (int64_t)0) : 0;
-  q.pages = q.n ? (int)min((int64_t)min(a.pt_stride, MOST_PAGES), ((int64_t)max(prefix, 0) + PAGE - 1) / PAGE + 1) : 0;
+  q.pages = q.n ? (int)min((int64_t)min(a.pt_stride, MOST_PAGES), ((int64_t)max(prefix, 0) + PAGE - 1) / PAGE) + 1 : 0;
   return q;
 }
 // Lane l: requests l, 64 + l, .. of up to PLAN_REQUESTS.

@@ -197,12 +197,18 @@ struct NodePlan {
 // 4000 keys, 64 nodes 44 and 101 us, 256 nodes 98 and 114, 256 of ragged requests 49 and 97; 8 nodes of 30000
 // keys beside 480 shorter ones 139 and 616. The plan and a join that finds little cost what it
 // costs: 500 keys, 64 nodes 24.4 and 23.5, 512 nodes 37 and 34, 1000 nodes 64 and 59.
-constexpr int FULL = 512, PLANNED = 1024, PLAN_REQUESTS = 256;
+//
+// 32 heads a workgroup read a page once for two tiles of 16. But where the slots are not full, tiles by
+// themselves end sooner: of tokens, where a page a tile is FULL tasks at most (1 token, 32 pages 10.9 us
+// and 12.3; 8 tokens, 512 such tasks, 20.8 and 22.3; 2000 tokens 516 and 314). Of trees the host knows no
+// lengths, and the width of their tables says nothing of them (nor is a node's rounding to hang on it): up
+// to TREE_TILES tiles go by themselves. Alone and in pairs, us at 1000, 4000, 16000, 32000 and 64000 keys,
+// 32 heads: 1 node 11.5 13.4 18.7 21.7 25.8 and 13.1 14.7 25.6 26.7 28.3; 8 nodes 15.9 20.0 30.3 41.0 62.8 and
+// 16.5 23.8 33.6 40.8 56.0; 16 nodes 17.0 24.8 41.2 63.2 and 22.0 27.9 40.5 55.6.
+constexpr int FULL = 512, PLANNED = 1024, PLAN_REQUESTS = 256, TREE_TILES = 16;
 inline void paged_plan(Paged& a, int pages) {
-  // 32 heads a workgroup read a page once for two tiles of 16; but where a page a tile leaves slots
-  // empty, tiles by themselves end sooner (1 token, 32 pages 10.9 us and 12.3; 8 tokens, 512 such
-  // tasks, 20.8 and 22.3; 1 node, 4000 keys 13.3 and 14.6; 2000 tokens 516 and 314)
-  a.head_rows = a.heads <= 16 || a.tokens * ((a.heads + 15) / 16) * pages <= FULL ? 16 : 32;
+  const int64_t tiles = a.tokens * ((a.heads + 15) / 16);
+  a.head_rows = a.heads <= 16 || (a.starts ? tiles <= TREE_TILES : tiles * pages <= FULL) ? 16 : 32;
   a.head_tiles = (a.heads + a.head_rows - 1) / a.head_rows;
   const int64_t whole = a.tokens * a.head_tiles;
   a.splits = 1;
@@ -212,7 +218,7 @@ inline void paged_plan(Paged& a, int pages) {
       const int64_t spare = whole <= FULL / 2 ? FULL - whole : FULL;  // tasks beside one a node's tile
       a.tasks = a.work = whole + spare;
       // nodes of two chunks or more: with as many nodes as spare tasks they have most parts
-      a.parts = std::min<int64_t>((spare + std::min(spare, whole)) / a.head_tiles, a.tokens * pages);
+      a.parts = std::min<int64_t>((spare + std::min(spare, whole)) / a.head_tiles, a.tokens * (pages + 1ll));
     }
     return;
   }

@@ -559,6 +559,21 @@ def test_tree_attention_shared_out_or_not(gpu_device, trees, heads):
     _tree_near(_q(gpu_device, len(mask), heads), starts, prefix, mask, table, _pool(gpu_device, pages, True))
 
 
+@pytest.mark.parametrize("trees,heads", [
+    ([(1, 1)], 32), ([(4000, 1)], 32), ([(4000, 1)], 16), ([(4027, 5)], 32), ([(19990, 10)], 32), ([(2500, 3), (0, 2), (900, 33)], 32),
+    ([(12000, 1)], 32), ([(6000, 2)], 32), ([(3000, 1), (2400, 2)], 64), ([(16383, 1)], 16), ([(16383, 1)], 4),
+    ([(1275, 5), (640, 64)], 64), ([(60, 4)], 32), ([(64, 1)], 128), ([(8000, 2), (7990, 10)], 17), ([(300, 60)] * 20, 32),
+])  # fmt: skip
+def test_tree_attention_does_not_hang_on_the_table_s_width(gpu_device, trees, heads):
+    """The same bits from a table that just holds the keys as from one with room for more."""
+    starts, prefix, mask, table, pages = _tree(gpu_device, trees)
+    c, q = _pool(gpu_device, pages, False), _q(gpu_device, len(mask), heads)
+    want = _tree_near(q, starts, prefix, mask, table, c) if heads * len(mask) < 400 else prompt.tree_attention(q, starts, prefix, mask, table, c)
+    for more in (1, 2, 700):
+        wide = torch.cat([table, torch.full((len(table), more), -1, dtype=torch.int32, device=gpu_device)], 1)
+        assert torch.equal(prompt.tree_attention(q, starts, prefix, mask, wide, c), want), more
+
+
 def test_tree_attention_sees_each_key_once(gpu_device):
     starts, prefix, mask, table, pages = _tree(gpu_device, [(100, 60), (37, 64)])
     mask[3], mask[70], mask[71] = 0, -1, -(1 << 63)  # the prefix alone; every drafted key; the last alone
