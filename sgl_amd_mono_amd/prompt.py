@@ -344,7 +344,8 @@ def select_pages(scores: torch.Tensor, pos: torch.Tensor, picks: int = TOPK // P
     ``first`` first and the ``last`` last (the token's own page among them), and the best-scored
     others, exactly, the lowest page of equal ones first (+0 above -0, a NaN by its bits). A token that
     sees at most ``picks`` pages reads all of them (with the default 32, every key of up to
-    2048, as a decode step's row does). ``pos[i]`` < 0 is a pad: all -1."""
+    2048, as a decode step's row does). ``pos[i]`` < 0 is a pad: all -1, and so are all rows of
+    ``scores`` without columns."""
     dev = _gpu(scores, "scores")
     if scores.dim() != 2:
         raise ValueError(f"scores: expected [tokens, columns], got {tuple(scores.shape)}")
@@ -354,7 +355,10 @@ def select_pages(scores: torch.Tensor, pos: torch.Tensor, picks: int = TOPK // P
     stride = max(_rows(scores, "scores", (t, columns), torch.float32, dev), columns)
     need(pos, "pos", (t,), torch.int32, dev)
     pages = torch.empty(t, picks, dtype=torch.int32, device=dev)
-    args = _lib.PromptSelectArgs(scores=scores.data_ptr(), stride=stride, tokens=t, columns=columns, pos=pos.data_ptr(),
+    if columns == 0:  # of no pages none is picked (a call of no tokens looks at the numbers all the same)
+        pages.fill_(-1)
+        t = 0
+    args = _lib.PromptSelectArgs(scores=scores.data_ptr(), stride=stride, tokens=t, columns=columns or 1, pos=pos.data_ptr(),
                                  picks=picks, first=first, last=last, pages=pages.data_ptr())
     _enqueue(dev, _lib.lib().mono_prompt_select, args)
     return pages

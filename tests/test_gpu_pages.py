@@ -256,6 +256,16 @@ def test_select_pages_scores_of_any_bits(gpu_device, columns):
         assert torch.equal(got.cpu(), ref.select_pages(scores, pos, picks, first, last)), (picks, first, last)
 
 
+def test_a_table_of_no_pages_from_its_scores_to_its_attention(gpu_device):
+    req, pos, table, pages = _requests(gpu_device, [(70, 5)])
+    iq, iqs, iw, caches = _index(gpu_device, 5, pages)
+    table = table[:, :0].contiguous()
+    scores = prompt.page_scores(iq, iqs, iw, req, pos, table, caches)
+    ids = prompt.select_pages(scores, pos)
+    assert scores.shape == (5, 0) and torch.equal(ids.cpu(), torch.full((5, 32), -1, dtype=torch.int32))
+    assert bool((prompt.attention(_q(gpu_device, 5, 32), req, pos, ids, table, _pool(gpu_device, pages, False)) == 0).all())
+
+
 def test_select_pages_default_takes_all_of_2048_keys(gpu_device):
     pos = torch.tensor([0, 64, 2047, 2048], dtype=torch.int32, device=gpu_device)
     got = prompt.select_pages(torch.randn(4, 40, device=gpu_device), pos).cpu()

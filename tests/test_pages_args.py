@@ -173,6 +173,18 @@ def test_cpu_and_misshapen_tensors_are_refused(monkeypatch):
     refused("mask", prompt.tree_attention, q, at, at[:1], at, table, c)
 
 
+def test_of_no_columns_no_page_is_selected(monkeypatch):
+    """page_scores has no columns where the page table has none (or it is asked for none)."""
+    monkeypatch.setattr(prompt, "_gpu", lambda t, name: t.device)
+    monkeypatch.setattr(prompt, "_enqueue", lambda dev, fn, args: _lib.check(fn(C.byref(args), None)))
+    for tokens in (0, 1, 3):
+        got = prompt.select_pages(torch.empty(tokens, 0), torch.arange(tokens, dtype=torch.int32), 5)
+        assert got.dtype == torch.int32 and torch.equal(got, torch.full((tokens, 5), -1, dtype=torch.int32))
+    for kw in (dict(picks=0), dict(picks=2, first=2, last=1)):
+        with pytest.raises(ValueError, match="picks"):
+            prompt.select_pages(torch.empty(3, 0), torch.zeros(3, dtype=torch.int32), **kw)
+
+
 def test_out_over_the_cache_s_scales_is_refused(monkeypatch):
     monkeypatch.setattr(prompt, "_gpu", lambda t, name: t.device)  # the checks alone, on CPU tensors
     at, table, mask = torch.zeros(2, dtype=torch.int32), torch.zeros(1, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int64)
