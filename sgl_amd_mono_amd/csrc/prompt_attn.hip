@@ -536,6 +536,8 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
           }
         }
         float ps[MT];
+        // (a logit is rounded before the maximum is taken from it, as the maximum was: at 2^31 one FMA for both
+        // leaves half a step of the product, 2^7, and the largest key's own power overflows)
         const auto weigh = [&]() {  // the probabilities to LDS, and whether one of the workgroup's is over EXP2_SLACK
           uint16_t* to = &L.p[0][to_place];
           float top = 0.f;
@@ -543,7 +545,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
           for (int c = 0; c < MT; ++c) {
             float y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = __builtin_amdgcn_exp2f(fmaf(s[c][j], by[j], -m_ref[c]));
+            for (int j = 0; j < 4; ++j) y[j] = __builtin_amdgcn_exp2f(__fsub_rn(__fmul_rn(s[c][j], by[j]), m_ref[c]));
             ps[c] = (y[0] + y[1]) + (y[2] + y[3]);
             top = fmaxf(fmaxf(top, fmaxf(y[0], y[1])), fmaxf(y[2], y[3]));
             *reinterpret_cast<u32x2*>(to + c * 16 * P_PITCH) = u32x2{pack2(y[0] * ks[0], y[1] * ks[1]), pack2(y[2] * ks[2], y[3] * ks[3])};
@@ -559,7 +561,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
           for (int c = 0; c < MT; ++c) {
             float m = NONE;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) m = fmaxf(m, s[c][j] * by[j]);
+            for (int j = 0; j < 4; ++j) m = fmaxf(m, __fmul_rn(s[c][j], by[j]));
             m = groups_max(m);
             if (here() < 16) L.top[wave][16 * c + here()] = m;
           }

@@ -503,6 +503,31 @@ def test_attention_queries_of_unlike_elements(gpu_device, tokens):
         _near(got[:, h:h + 1], want, mag, top, 4 * PAGE, norm=False)
 
 
+@pytest.mark.parametrize("power,sign,scale", [(10, 1, 0.07), (24, -1, 0.07), (31, 1, 0.07), (40, -1, 0.07), (70, 1, 1.3), (118, 1, 0.6)])
+@pytest.mark.parametrize("tokens", [1, 600])
+def test_attention_logits_of_any_size(gpu_device, tokens, power, sign, scale):
+    """Logits of thousands to 3e37, of either sign: one key's is the largest by far more than an
+    exponential's range, so its row is the output, exactly."""
+    req, pos, table, pages = _requests(gpu_device, [(640, tokens)])
+    c, best = _pool(gpu_device, pages, False), [3, 200, 500, 639]
+    pe = torch.tensor([1.0, 1.25, 1.5] if sign > 0 else [2.0, 2.5, 3.0], device=gpu_device)
+    rows = c.kv.view(torch.float8_e4m3fn)
+    rows[:, 512:] = pe[torch.arange(len(rows), device=gpu_device) % 3, None].to(torch.float8_e4m3fn)
+    c.kv_scale.fill_(1.0)
+    q = torch.zeros(tokens, 32, 576, dtype=torch.bfloat16, device=gpu_device)
+    q[:, :, 512:] = sign * 2.0**power
+    ids = torch.arange(10, dtype=torch.int32, device=gpu_device).repeat(tokens, 1)
+    starts, prefix = (torch.tensor(v, dtype=torch.int32, device=gpu_device) for v in ([0, tokens], [640]))
+    mask = torch.zeros(tokens, dtype=torch.int64, device=gpu_device)
+    for p in best:
+        d = AttnCaches(None, None, c.kv.clone(), c.kv_scale)
+        slot = int(table[0, p // PAGE]) * PAGE + p % PAGE
+        d.kv.view(torch.float8_e4m3fn)[slot, 512:] = torch.tensor(1.75, device=gpu_device).to(torch.float8_e4m3fn)
+        want = d.kv.view(torch.float8_e4m3fn)[slot, :512].to(torch.bfloat16).expand(tokens, 32, 512)
+        assert torch.equal(prompt.attention(q, req, pos, ids, table, d, softmax_scale=scale), want), p
+        assert torch.equal(prompt.tree_attention(q, starts, prefix, mask, table, d, softmax_scale=scale), want), p
+
+
 # ------------------------------------------------------------------------ tree
 def _tree(dev, trees, seed=2, spare=0):
     """(starts, prefix, mask, table, pages) of trees (prefix, nodes): a node hangs from one of
