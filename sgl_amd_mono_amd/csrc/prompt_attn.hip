@@ -42,8 +42,8 @@ namespace {
 constexpr int T = 256, WAVES = 4, ROW = LATENT + PE, PAGE_BYTES = PAGE * ROW;
 constexpr int BLOCKS = ROW / 64, BLOCK_BYTES = PAGE * 64;  // a page's rows in blocks of 64 dims
 constexpr int HEADS = 32;
-// NONE: no maximum yet, so low that any logit passes it (and finite: what is taken from it is a number)
-constexpr float NEG_INF = -__builtin_inff(), NONE = -1e38f, EXP2_SLACK = 16.0f;
+// NONE: no maximum yet, the lowest there can be (and finite: what is taken from it is a number)
+constexpr float NEG_INF = -__builtin_inff(), NONE = -__FLT_MAX__, EXP2_SLACK = 16.0f;
 
 // A page and its keys' scales.
 struct Stage {

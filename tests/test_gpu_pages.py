@@ -503,10 +503,10 @@ def test_attention_queries_of_unlike_elements(gpu_device, tokens):
         _near(got[:, h:h + 1], want, mag, top, 4 * PAGE, norm=False)
 
 
-@pytest.mark.parametrize("power,sign,scale", [(10, 1, 0.07), (24, -1, 0.07), (31, 1, 0.07), (40, -1, 0.07), (70, 1, 1.3), (118, 1, 0.6)])
+@pytest.mark.parametrize("power,sign,scale", [(10, 1, 0.07), (24, -1, 0.07), (31, 1, 0.07), (40, -1, 0.07), (70, 1, 1.3), (118, 1, 0.6), (121, -1, 0.6)])
 @pytest.mark.parametrize("tokens", [1, 600])
 def test_attention_logits_of_any_size(gpu_device, tokens, power, sign, scale):
-    """Logits of thousands to 3e37, of either sign: one key's is the largest by far more than an
+    """Logits of thousands to 2.6e38, of either sign: one key's is the largest by far more than an
     exponential's range, so its row is the output, exactly."""
     req, pos, table, pages = _requests(gpu_device, [(640, tokens)])
     c, best = _pool(gpu_device, pages, False), [3, 200, 500, 639]
