@@ -591,8 +591,8 @@ int mono_prompt_experts(const mono_prompt_experts_args* args, void* stream);
 /* The index queries of tokens at pos[t], in the format that mono_front_forward hands to
  * mono_attn_forward: of each of 64 heads' 128 dims bf16(x), RoPE on dims [0, 64), bf16,
  * Hadamard, bf16 and FP4, each value formed in f64 between its roundings. A token whose
- * position is outside [0, max_pos) is a pad: zeros. A head that is not finite has zero codes
- * and scale bytes 255 (NaN). */
+ * position is outside [0, max_pos) is a pad: zeros. A block of 32 dims that is not finite (all four
+ * of a head with a NaN or an infinity in it) has zero codes and scale byte 255 (NaN). */
 typedef struct {
   const void* x;          /* bf16 or f32 [tokens, 64 x 128], before RoPE */
   int64_t x_stride;       /* elements from a row to the next; rows 16-byte aligned */
@@ -614,7 +614,8 @@ int mono_prompt_query(const mono_prompt_query_args* args, void* stream);
  * for 0. -infinity where the token sees no key of the page (behind its position, a page outside
  * the table or the pool, a pad: req outside [0, requests) or pos < 0). Products and sums are f32
  * (past its range infinite); a score is off by 12 roundings, 2^-24 each, of sum_h |iw (q . k)| at
- * most, of the heads too that the maximum cuts off. */
+ * most, of the heads too that the maximum cuts off (where a query's and a key's scales lie within 2^7
+ * of each other, so that f32 holds their products exactly). */
 typedef struct {
   const void* iq;            /* u8 [tokens, 64, 64], 16-byte aligned */
   const void* iqs;           /* u8 [tokens, 64, 4] */
@@ -653,7 +654,14 @@ int mono_prompt_select(const mono_prompt_select_args* args, void* stream);
  * lists: s_j = softmax_scale (q . c_j), p = softmax(s), out = sum_j p_j c_j[:512], with c_j =
  * kv_scale[j] kv[j]. A page below 0, outside the table or the pool is none; one that is listed
  * twice counts twice. A token that sees no key (a pad: req outside [0, requests) or pos < 0)
- * has zeros. What lies in keys that are not seen does not matter. */
+ * has zeros. What lies in keys that are not seen does not matter. out must share no memory with
+ * the other arguments.
+ *
+ * An element of q is held to 2^-21.8 of its head's largest (2^-17.8 in the last 64 dims), which is
+ * all of bf16 above 2^-14 (2^-10) of it; a head of q that is not finite has NaN outputs. A logit is
+ * off by 2^-16 of the sum of its terms' magnitudes at most (the FP8 matrix instruction's sum), p is
+ * rounded to bf16, and sums are f32. The same call gives the same bits; how many tokens (nodes,
+ * requests) it has decides whether one's pages are summed in parts, and so its rounding. */
 typedef struct {
   const void* q;             /* bf16 [tokens, heads, 576] (latent 512 | pe 64) */
   int64_t tokens;            /* 0..1048576 */
@@ -679,7 +687,8 @@ int mono_prompt_attention(const mono_prompt_attention_args* args, void* stream);
 /* MLA attention of drafted tokens. Request r's nodes are rows starts[r] .. starts[r + 1] - 1 of
  * q; its node i's key lies at position prefix[r] + i. Node n of it sees every key at positions
  * below prefix[r], and key prefix[r] + j for each bit j of mask[n] (its ancestors and itself;
- * any bits are good). Nodes of no request, and nodes that see nothing, have zeros. */
+ * any bits are good). Nodes of no request, and nodes that see nothing, have zeros. Held and rounded
+ * as in mono_prompt_attention; pt_stride beyond the keys changes no bit. */
 typedef struct {
   const void* q;             /* bf16 [nodes, heads, 576] */
   int64_t nodes;             /* 0..1048576 */

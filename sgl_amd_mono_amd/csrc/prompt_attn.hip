@@ -13,23 +13,29 @@
 //           the probabilities meet in LDS
 //
 // q is split into two E4M3 pieces of four significant bits, which hold bf16's eight: q . c is then
-// two FP8 products of twice bf16's rate and the keys are not widened. Elements below 2^-14 of their
-// head's largest (2^-10 in the last 64 dims, whose pieces share an instruction and so a scale) lose
-// bits: they are off by 2^-21.8 (2^-17.8) of the largest at most, as a logit's f32 sum over 576 terms
-// is of its own. When this came in place of q in bf16 and widened keys, 4096 tokens went from 648 to
-// 624 us and one from 17 to 14.
+// two FP8 products of twice bf16's rate and the keys are not widened. Two things are less exact so.
+// Elements below 2^-14 of their head's largest (2^-10 in the last 64 dims, whose pieces share an
+// instruction and so a scale) lose bits: they are off by 2^-21.8 (2^-17.8) of the largest at most. And
+// the FP8 instruction does not sum in full f32: it lines its products up with the largest and cuts what
+// is below, up to 2^-16 of a logit's terms' magnitudes (seen of unlike elements; of random ones two logits'
+// difference is off by 2^-18 of both at most, 2^-20.5 in the root of squares). Outputs in bf16 do not show
+// it: against 64 bits they are off by 0.00211, 0.00169 and 0.00201 of their norm (777 tokens, 5 nodes, 129
+// nodes) here and with q in bf16 against widened keys; with q 64 times as large, logits of 110, by 0.00069,
+// 0.00051 and 0.00069 here and 0.00067, 0.00050 and 0.00068 there. That form takes longer: 4096 tokens 648 us
+// for 604, 777 tokens 49 for 43, 129 nodes 38.7 for 33.7, 1024 nodes 592 for 550 (side by side on one card).
 //
 // Probabilities times their key's scale are rounded to bf16, off by 2^-8 of each at most and at random,
-// beside the output's own 2^-8; their sum adds up the f32 values. (Two E4M3 pieces of them were tried:
-// small ones lose bits against the largest, which outputs that hang on many keys show.)
+// beside the output's own 2^-8, which alone is 0.0017 of the norm; their sum adds up the f32 values. (Two
+// E4M3 pieces of them were tried: small ones lose bits against the largest, which outputs that hang on many
+// keys show.)
 //
 // The maximum that the sums refer to stays as it is until a probability passes 2^4 (a ratio of
 // sums does not depend on it, and bf16 and f32 hold 2^4 as well as 1): the waves' maxima then meet
 // and the sums are scaled, which happens on a token's first page and rarely after it.
 //
 // Two workgroups a CU (80 KB of LDS, 256 registers a lane), a page of 32 heads in 1.15 us a CU:
-// 4096 tokens of 32 heads over 2048 keys 596 to 606 us, 950 to 965 TFLOP/s; a large bf16 product reaches
-// 1180. Matrix instructions (44 % of the cycles) and vector issue (50 %: the widening, the
+// 4096 tokens of 32 heads over 2048 keys 584 to 632 us by the card, 910 to 985 TFLOP/s; a large bf16 product
+// reaches 1180 to 1200. Matrix instructions (44 % of the cycles) and vector issue (50 %: the widening, the
 // probabilities, addresses), at a clock that power holds at 1.75 to 1.9 GHz, are what bounds it.
 // Heads of up to 16 take one tile of 16 (2000 tokens 224 us, in a half-empty pair of them 304), up
 // to 32 two side by side (2000 tokens 314 us, as two workgroups 516, which read the pages twice).
@@ -242,8 +248,9 @@ MONO_DEV void each_set(const Paged& a, F f) {
 // all pages and that of all pages beside a short chunk a node. `tasks` comes to be how many there are.
 //
 // Two workgroups a CU, but one where that has FEW_PAGES pages at most: fewer parts to write and
-// join are then worth more (20000 keys, 512 and 256 tasks: 4 nodes 33.1 and 31.9 us, 8 nodes 38.3 and
-// 40.0, 16 nodes 46.8 and 51.4; 4000 keys, 16 nodes 33.4 and 27.6). And whole nodes where chunks save
+// join are then worth more (20000 keys, 512 and 256 tasks: 1 node 21.9 and 19.0 us, 4 nodes 26.8 and 26.7,
+// 8 nodes 32.5 and 36.1, 16 nodes 44.0 and 49.6; 4000 keys, 8 nodes 23.7 and 20.0, 16 nodes 30.6 and 27.3).
+// And whole nodes where chunks save
 // at most JOIN_PAGES pages (9 pages a node, 128 nodes: in twos 34 us, whole 28.5; 64 nodes, in threes 25,
 // whole 27). More nodes than one round's half are whole but for those longer than a workgroup's share.
 constexpr int FEW_PAGES = 8, JOIN_PAGES = 4;
@@ -590,7 +597,7 @@ MONO_DEV void attend(const Paged& a, Lds& L, int lane, int wave, const Task& tas
         {
           const uint16_t* pr = &L.p[0][from_place];
           const uint8_t* keys = &st.kv[value_place];
-                    constexpr int N = PAGE / V::K * V::TILES, VAHEAD = 4;  // (tile i % TILES of keys K (i / TILES) ..)
+          constexpr int N = PAGE / V::K * V::TILES, VAHEAD = 4;  // (tile i % TILES of keys K (i / TILES) ..)
           u32x2 w[VAHEAD];
           bf16x8 pk[2];
           const auto read = [&](int i) {
@@ -798,7 +805,7 @@ hipError_t paged_attention(const Paged& a, hipStream_t st) {
 hipError_t join_attention(const Paged& a, hipStream_t st) {
   const int64_t heads = a.tokens * a.heads;
   // Few heads have many parts each, and too few workgroups: four waves each and four workgroups
-  // (attention and join: 1 node of 32 heads, 20000 keys 25.6 us, one wave 37.5; 4 nodes 32.7 and 36.2).
+  // (attention and join: 1 node of 32 heads, 20000 keys 19.0 us, one wave 26.9; 4 nodes 26.7 and 30.8).
   // From 512 heads on one wave does (16 nodes, 1000 keys 23.1 and 23.9, 64 nodes 32.3 and 42.0). Of
   // thousands of heads most were written whole: four a workgroup (1000 nodes, 500 keys 64 us and 68, but
   // 16 nodes 24.9 and 22.3).

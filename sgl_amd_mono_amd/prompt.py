@@ -10,7 +10,8 @@ and caches, where the decode launches take a step of a few.
   ``moe.MoeRuntime.forward_fp8``, behind a router of the caller's)
 * ``index_query``, ``page_scores``, ``select_pages``, ``attention``: a prompt's own sparse
   attention. Where a decode step's row selects its 2048 best keys one at a time, a prompt's
-  token selects pages of 64 keys by the best index score in each, and attends to their keys.
+  token selects pages of 64 keys by the best index score in each, and attends to their keys:
+  beyond 2048 keys not those of the layer's definition.
 * ``tree_attention``: attention of a tree of drafted tokens to its request's keys and to
   those of the draft that each token's mask lets it see
 
@@ -313,7 +314,8 @@ def page_scores(iq: torch.Tensor, iqs: torch.Tensor, iw: torch.Tensor, req: torc
     at most 8192). ``iq`` / ``iqs`` are the tokens' index queries (``index_query``), ``iw`` bf16
     [tokens, 64] their head weights; token i is position ``pos[i]`` of request ``req[i]`` (i32),
     and a key's score the decode launches' index score, summed in f32: off by 12 roundings at most,
-    2^-24 each, of the sum of all heads' |weight x product|. -infinity where the token sees no key
+    2^-24 each, of the sum of all heads' |weight x product| (where a query's and a key's scales lie
+    within 2^7 of each other, so that f32 holds their products exactly). -infinity where the token sees no key
     of the page, NaN where the score of one is (a NaN product, which the decode launches take for 0)."""
     dev = _gpu(iq, "iq")
     t = iq.shape[0] if iq.dim() == 3 else -1
@@ -400,9 +402,16 @@ def attention(q: torch.Tensor, req: torch.Tensor, pos: torch.Tensor, pages: torc
     Token i is position ``pos[i]`` of request ``req[i]``, a row of ``page_table`` [requests,
     pages] (all i32). A listed page outside the table or the pool is none, one that is listed
     twice counts twice. A token that sees no key has zeros. Keys that a token does not see may
-    hold anything. An element of ``q`` is held to 2^-21.8 of its head's largest (2^-17.8 in the
-    last 64 dims), which is all of bf16 for those above 2^-14 (2^-10) of it. ``out`` must share
-    no memory with ``q`` or the cache."""
+    hold anything. ``out`` must share no memory with the other arguments (``q`` and the cache are
+    looked at).
+
+    An element of ``q`` is held to 2^-21.8 of its head's largest (2^-17.8 in the last 64 dims),
+    which is all of bf16 for those above 2^-14 (2^-10) of it; a head of ``q`` that is not finite has
+    NaN outputs. A logit is summed on the FP8 matrix instruction, off by 2^-16 of the sum of its terms'
+    magnitudes at most; a probability is rounded to bf16 before the values' sum, which is f32.
+    Outputs are 0.0017 to 0.0021 of their norm from 64 bits, of which bf16 alone makes 0.0017. The
+    same call gives the same bits, but a token's bits are not its own in any company: how many
+    tokens a call has decides whether a token's pages are summed in parts."""
     dev = _gpu(q, "q")
     n_pages, out = _latents(q, caches, out, dev)
     t, heads = q.shape[:2]
@@ -430,8 +439,10 @@ def tree_attention(q: torch.Tensor, starts: torch.Tensor, prefix: torch.Tensor, 
     (i32 [requests] and [requests + 1]); the key of its node i lies at position ``prefix[r]`` + i
     (``append`` with ``slot_pos``). A node sees the prefix and, for each bit j of its ``mask``
     (i64 [nodes]: the node itself and its ancestors), the key at ``prefix[r]`` + j. A node of no
-    request, and one that sees nothing, has zeros. ``out`` must share no memory with ``q`` or the
-    cache."""
+    request, and one that sees nothing, has zeros. ``out`` must share no memory with the other
+    arguments (``q`` and the cache are looked at). ``q``, logits and probabilities are held as in
+    ``attention``; a node's bits hang on the call's other trees, which decide the parts that its
+    pages are summed in, but not on how wide ``page_table`` is."""
     dev = _gpu(q, "q")
     n_pages, out = _latents(q, caches, out, dev)
     t, heads = q.shape[:2]
