@@ -7,8 +7,8 @@
 // wants it, with half its heads' weights, the next page's keys come ahead. A 32 x 32 MFMA's lanes
 // hold one key each and 16 heads: the ReLU and the weighted sum are two FMAs a value, and a key's
 // heads meet in one swap of halves. They bound the kernel: some 180 vector operations a token and
-// page, issuing 97 % of the time, beside 256 cycles of MFMA. 8192 tokens from position 0: 200 us, 2.75 PFLOP/s (a maximum and an
-// FMA a value: 290 us; the products alone would take some 65).
+// page, issuing 97 % of the time, beside 256 cycles of MFMA. 8192 tokens from position 0: 205 to 213 us by the
+// card, 2.6 to 2.7 PFLOP/s (a maximum and an FMA a value: 290 us; the products alone would take some 65).
 //
 // FP4 products and their sum are exact in f32 where a query's and a key's scales lie close; the weighted sum is
 // f32 throughout. As x / 2 + |x| / 2 a head's ReLU leaves a rounding of the size of a product that it
