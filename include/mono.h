@@ -659,7 +659,7 @@ int mono_prompt_select(const mono_prompt_select_args* args, void* stream);
  *
  * An element of q is held to 2^-21.8 of its head's largest (2^-17.8 in the last 64 dims), which is
  * all of bf16 above 2^-14 (2^-10) of it; a head of q that is not finite has NaN outputs. A logit is
- * off by 2^-16 of the sum of its terms' magnitudes at most (the FP8 matrix instruction's sum), p is
+ * off by up to 2^-16 of the sum of its terms' magnitudes (the FP8 matrix instruction's, measured), p is
  * rounded to bf16, and sums are f32. The same call gives the same bits; how many tokens (nodes,
  * requests) it has decides whether one's pages are summed in parts, and so its rounding. */
 typedef struct {

@@ -407,8 +407,8 @@ def attention(q: torch.Tensor, req: torch.Tensor, pos: torch.Tensor, pages: torc
 
     An element of ``q`` is held to 2^-21.8 of its head's largest (2^-17.8 in the last 64 dims),
     which is all of bf16 for those above 2^-14 (2^-10) of it; a head of ``q`` that is not finite has
-    NaN outputs. A logit is summed on the FP8 matrix instruction, off by 2^-16 of the sum of its terms'
-    magnitudes at most; a probability is rounded to bf16 before the values' sum, which is f32.
+    NaN outputs. A logit is summed on the FP8 matrix instruction, off by up to 2^-16 of the sum of its
+    terms' magnitudes (as measured); a probability is rounded to bf16 before the values' sum, which is f32.
     Outputs are 0.0017 to 0.0021 of their norm from 64 bits, of which bf16 alone makes 0.0017. The
     same call gives the same bits, but a token's bits are not its own in any company: how many
     tokens a call has decides whether a token's pages are summed in parts."""
